@@ -62,6 +62,20 @@ SIGNATURES = {
                                + [c_int64] * 4 + [c_void_p, c_void_p]),
     "ffnk_ffn_backward": (c_int, [c_void_p, c_int64] + [c_void_p] * 10 + [c_int64] * 4 + [c_void_p] * 6 + [c_int64]
                           + [c_void_p] * 6 + [c_int64] * 3 + [c_void_p, c_void_p]),
+    "ffnk_mxfp4_code_bytes": (c_int64, [c_int64, c_int64]),
+    "ffnk_mxfp4_scale_bytes": (c_int64, [c_int64, c_int64]),
+    "ffnk_mxfp4_quantize": (c_int, [c_void_p, c_int] + [c_int64] * 4 + [c_void_p] * 3),
+    "ffnk_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p]),
+    "ffnk_mxfp4_workspace_bytes": (c_int64, [c_int64] * 3),
+    "ffnk_mxfp4_linear_forward": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + [c_int64, c_void_p] + [c_int64] * 4
+                                  + [c_void_p, c_void_p]),
+    "ffnk_mxfp4_ffn_forward": (c_int, [c_void_p, c_int64, POINTER(c_void_p), POINTER(c_void_p)] + [c_void_p] * 4
+                               + [c_int64, c_void_p, c_void_p, c_void_p] + [c_int64] * 4 + [c_void_p, c_void_p]),
+    "ffnk_mxfp4_backward_workspace_bytes": (c_int64, [c_int64] * 4),
+    "ffnk_mxfp4_linear_backward": (c_int, [c_void_p, c_int64] + [c_void_p] * 7 + [c_int64, c_void_p] + [c_int64] * 4
+                                   + [c_void_p, c_void_p]),
+    "ffnk_mxfp4_ffn_backward": (c_int, [c_void_p, c_int64, POINTER(c_void_p), POINTER(c_void_p)] + [c_void_p] * 5
+                                + [c_int64, c_void_p] + [c_int64] * 4 + [c_void_p, c_void_p]),
     "ffnk_read_status": (c_int, [c_void_p, c_int, c_void_p]),
     "ffnk_selftest_bounded_wait": (c_int, [c_void_p, c_int64, c_void_p]),
     "ffnk_set_sm_margin": (c_int, [c_int]),

@@ -46,8 +46,8 @@ static EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
-int make_tensor_map_2d(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride,
-                       uint32_t box_inner, uint32_t box_outer) {
+int make_tensor_map_2d_of(CUtensorMap* out, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
+                          uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return FFNK_ERR_DRIVER;
   // The encoder is a driver-API call and needs the device's primary context current on the
@@ -62,20 +62,25 @@ int make_tensor_map_2d(CUtensorMap* out, const void* base, uint64_t inner, uint6
       bound_device = dev;
     }
   }
-  if ((reinterpret_cast<uintptr_t>(base) & 15) || ((row_stride * 2) & 15)) return FFNK_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || (row_bytes & 15)) return FFNK_ERR_ALIGN;
   if (inner == 0 || outer == 0) return FFNK_ERR_SHAPE;
   const cuuint64_t dims[2] = {inner, outer};
-  const cuuint64_t strides[1] = {row_stride * 2};
+  const cuuint64_t strides[1] = {row_bytes};
   const cuuint32_t box[2] = {box_inner, box_outer};
   const cuuint32_t elem[2] = {1, 1};
-  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, elem,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = fn(out, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS && tune_overrides().verbose > 0)
     fprintf(stderr, "ffnk: cuTensorMapEncodeTiled failed (CUresult %d): base %p dims {%llu, %llu} row stride %llu B box {%u, %u}\n",
             static_cast<int>(r), base, static_cast<unsigned long long>(inner), static_cast<unsigned long long>(outer),
-            static_cast<unsigned long long>(row_stride * 2), box_inner, box_outer);
+            static_cast<unsigned long long>(row_bytes), box_inner, box_outer);
   return r == CUDA_SUCCESS ? 0 : FFNK_ERR_TENSORMAP;
+}
+
+int make_tensor_map_2d(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride,
+                       uint32_t box_inner, uint32_t box_outer) {
+  return make_tensor_map_2d_of(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, inner, outer, row_stride * 2, box_inner, box_outer,
+                               CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // One CTA, one barrier that nobody arrives on.  The wait must return false after the budget,

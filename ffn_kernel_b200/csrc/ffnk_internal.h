@@ -30,6 +30,13 @@ const DeviceInfo& device_info();
 int make_tensor_map_2d(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride,
                        uint32_t box_inner, uint32_t box_outer);
 
+// The same for any element type and swizzle: extents and boxes in elements, row stride in bytes (a multiple of 16).
+int make_tensor_map_2d_of(CUtensorMap* out, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
+                          uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);
+
+// SMs a persistent grid may occupy (all but the margin of ffnk_set_sm_margin, at least two).
+int usable_sms();
+
 // Overrides of single tile-table entries, for measuring a choice against its alternatives
 // (ffnk_tune_override; `python -m ffn_kernel_b200.tune`).  -1 = the table decides.  The library reads
 // no environment variables: whoever wants an override sets it through the C ABI.
@@ -65,6 +72,21 @@ int ffn_gateup_early(const void* x, int64_t ldx, const void* w1, const void* w3,
                      int64_t w_stride_k, int64_t w_stride_n, const int32_t* perm, const int32_t* counts, void* out,
                      int64_t ldo, int routed_in, int routed_out, int64_t M, int64_t d, int64_t h, int early,
                      int32_t* status, void* stream);
+
+// Routing of the mask and the activations in MXFP4 in routed order (codes [(cap + 512), ceil(d/32)*16], scales), in one
+// launch for masks of one routing tile.
+int mx_route_quantize(const void* mask, int64_t M, const void* x, int64_t ldx, int64_t d, int32_t* perm, int32_t* counts,
+                      void* scan, void* codes, void* scales, int32_t* status, void* stream);
+
+// n <= 6 MXFP4 matrices to contiguous bf16 in one launch; matrix i is left out when counts[gate[i]] is zero.
+int mx_dequantize_weights(const void* const* codes, const void* const* scales, const int64_t* rows, const int64_t* cols,
+                          const int* gate, int n, const int32_t* counts, void* const* out, void* stream);
+
+// dx of the FFN backward alone (frozen weights): w1, w3, u1, u3 bf16 [h, d], w2, u2 [d, h], contiguous; t1, t3 fp32 in
+// the tiled order (pre_tile_offset).  gr bf16 [rows, d], dt1, dt3 bf16 [rows, h] scratch, rows = cap + 512.
+int ffn_backward_dx(const void* gy, int64_t ldg, const void* t1, const void* t3, const void* w1, const void* w2, const void* w3,
+                    const void* u1, const void* u2, const void* u3, const int32_t* perm, const int32_t* counts, void* gr,
+                    void* dt1, void* dt3, void* dx, int64_t lddx, int64_t M, int64_t d, int64_t h, int32_t* status, void* stream);
 
 // permute_rows with an optional device-side gate: with only_if_scattered = T > 0 the kernel returns at
 // once unless the mask's runs of same-modality tokens average fewer than T rows.

@@ -1,0 +1,704 @@
+// Routed GEMMs on MXFP4 operands (format: mxfp4.cuh) and the forward passes made of them.
+//
+// D[r, n] = sum over blocks b of 2^(Ea[r,b] + Ew[n,b]) * sum over the 32 values of block b of a * w, the rows r
+// of one modality by that modality's weight.  tcgen05.mma.kind::mxf4.block_scale does both sums: codes come
+// from shared memory (64 values of a row an instruction, four times the bf16 instruction's K for the same bytes),
+// the scales from tensor memory, where tcgen05.cp puts each 512-byte scale atom (128 rows x 4 blocks).  Products
+// of codes are exact, sums are fp32.
+//
+// Both operands are K-major: activations quantised into routed order (mxfp4.cu) and weights in nn.Linear order.
+// Epilogues: bf16 rows scattered to token order; or silu(gate) * up, which leaves as MXFP4 again: the 32
+// accumulator columns a lane reads at a time are one block of its row, so the maximum, the scale and the codes
+// need no other lane.
+#include "ffnk_internal.h"
+#include "mxfp4.cuh"
+#include "ptx.cuh"
+
+namespace ffnk {
+
+// ---------------------------------------------------------------------------------------------
+// block-scaled tcgen05
+// ---------------------------------------------------------------------------------------------
+// Instruction descriptor of kind::mxf4: E2M1 operands, scales in powers of two (UE8M0).  sf: which half of
+// the four scale bytes of a tensor-memory word this instruction's two blocks use (0: bytes 0,1; 2: bytes 2,3).
+__host__ __device__ constexpr uint32_t mx_idesc(int m, int n, uint32_t sf) {
+  return (sf << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(m >> 7) << 27) | (sf << 29);
+}
+template <int CTAS>
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t sfa,
+                                          uint32_t sfb, uint32_t accumulate) {
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// One scale atom (512 consecutive bytes: 32 rows of 16 bytes) from shared memory to four tensor-memory columns,
+// the same 32 lanes in all four lane quarters.  In issue order with the MMAs of the same thread.
+template <int CTAS>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t tmem, uint32_t smem) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem & 0x3FFFFu) >> 4);
+  d |= 1ull << 16;      // leading offset: unused, one 16-byte column
+  d |= 8ull << 32;      // 128 bytes between groups of eight rows
+  d |= 1ull << 46;      // descriptor version for sm_100; no swizzle
+  if constexpr (CTAS == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------
+// geometry
+// ---------------------------------------------------------------------------------------------
+constexpr int MX_BM = 128;                    // rows of a CTA's tile
+constexpr int MX_BN = 256;                    // accumulator columns (gate/up tiles: 128 gate | 128 up)
+constexpr int MX_BK = 256;                    // values of a k-step: 128 bytes, one swizzle row; two scale atoms
+constexpr int MX_A_BYTES = MX_BM * 128;       // 16 KiB of codes
+constexpr int MX_SF_BYTES = 2 * kMxAtomBytes; // scales of 128 rows x one k-step
+constexpr int MX_THREADS = 320;               // producer, MMA, eight epilogue warps
+constexpr int MX_STAGING = 8 * 2048;          // one 32-row x 64-byte transposition buffer per epilogue warp
+
+enum { MX_EPI_STORE = 0, MX_EPI_GLU = 1, MX_EPI_GLU_SAVE = 2 };
+__host__ __device__ constexpr bool mx_glu(int e) { return e != MX_EPI_STORE; }
+
+struct MxParams {
+  const int* perm;
+  const int* counts;
+  int* status;
+  int n_out;               // output columns: N, or h for the gate/up tiles
+  int k_bytes;             // code bytes of a row along the contraction (a multiple of 16)
+  int a_rows;              // rows of an A box (fewer than 128 when no tile has more)
+  int group_m;
+  // MX_EPI_STORE: out[token][n]; MX_EPI_GLU_SAVE: t1, t3 fp32 in routed rows, tiled (pre_tile_offset)
+  __nv_bfloat16* out;
+  int64_t ldo;
+  float* t1;
+  float* t3;
+  // MX_EPI_GLU*: codes [routed row][code_ld] and scales of the quantised product
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t code_ld;
+  int k_atoms_out;
+  int pdl;
+};
+
+struct MxMaps {
+  CUtensorMap a, sa;       // activations: codes, scales
+  CUtensorMap b[4];        // weight codes: visual 0/1, text 0/1 (gate, up)
+  CUtensorMap sb[4];       // weight scales
+};
+
+struct MxTile {
+  int nt, row0, rows, list_off;
+  int64_t routed0;         // first routed-order row of the tile
+  bool text;
+};
+
+__device__ __forceinline__ int mx_text_base(int Mv) { return ((Mv + 255) >> 8) << 8; }
+
+// Tile t: super-tiles of group_m row tiles x all column tiles, rows fastest.  bm: rows of the (pair) tile,
+// half: this CTA's offset inside it.
+__device__ __forceinline__ MxTile mx_tile(int t, int bm, int half, int tiles_v, int m_tiles, int n_tiles, int group_m, int Mv,
+                                          int Mt, int cap) {
+  MxTile c;
+  const int per_super = group_m * n_tiles;
+  const int st = t / per_super;
+  const int r = t - st * per_super;
+  const int m0 = st * group_m;
+  const int gm = min(group_m, m_tiles - m0);
+  c.nt = r / gm;
+  const int mt = m0 + (r - c.nt * gm);
+  c.text = mt >= tiles_v;
+  c.row0 = (c.text ? mt - tiles_v : mt) * bm + half;
+  c.rows = max(0, min(MX_BM, (c.text ? Mt : Mv) - c.row0));
+  c.list_off = c.text ? cap : 0;
+  c.routed0 = (c.text ? mx_text_base(Mv) : 0) + c.row0;
+  return c;
+}
+
+__device__ __forceinline__ uint32_t mx_pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 32 rows x 32 columns of one warp as bf16 through its 2 KiB of shared memory: 64 contiguous bytes a row, eight
+// rows a store instruction.  `dst`: address of this lane's row (0: none).
+__device__ __forceinline__ void mx_store_rows(const float (&v)[32], unsigned long long dst, int n0, int n_out, uint8_t* stg, int lane) {
+  const int wsw = (lane >> 1) & 3, pc = lane & 3;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(stg + lane * 64 + ((j ^ wsw) << 4)) =
+        make_uint4(mx_pack_bf16(v[8 * j], v[8 * j + 1]), mx_pack_bf16(v[8 * j + 2], v[8 * j + 3]),
+                   mx_pack_bf16(v[8 * j + 4], v[8 * j + 5]), mx_pack_bf16(v[8 * j + 6], v[8 * j + 7]));
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    const unsigned long long rp = __shfl_sync(0xFFFFFFFFu, dst, r);
+    const uint4 val = *reinterpret_cast<const uint4*>(stg + r * 64 + ((pc ^ ((r >> 1) & 3)) << 4));
+    if (rp != 0ull && n0 + pc * 8 < n_out) *reinterpret_cast<uint4*>(rp + 2ull * (n0 + pc * 8)) = val;
+  }
+  __syncwarp();
+}
+
+// silu(t1) * t3 with an exponential and a reciprocal good to a few units in the last fp32 place: what is rounded
+// to four bits next must not sit on the wrong side of a tie more often than fp32 sums put it there anyway
+// (a hyperbolic tangent of 2^-11 would move one value in a thousand by a whole step).
+__device__ __forceinline__ float mx_silu_mul(float t1, float t3) { return __fdividef(t1, 1.0f + __expf(-t1)) * t3; }
+
+// One block (32 values of one row): scale byte and 16 bytes of codes.
+__device__ __forceinline__ uint32_t mx_quantize_block(const float (&v)[32], uint4& codes) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  const uint32_t byte = mx_scale_byte(m);
+  const float inv = mx_inverse_scale(byte);
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = v[8 * j + i] * inv;
+    w[j] = byte == 255u ? 0u : mx_pack8(a);
+  }
+  codes = make_uint4(w[0], w[1], w[2], w[3]);
+  return byte;
+}
+
+__device__ __forceinline__ void mx_report(int* status, int code) {
+  if (status) atomicCAS(status, 0, code);
+}
+
+// Tensor memory.  Two accumulators of 256 columns and 24 columns of scales do not fit into 512, so the second
+// accumulator starts 32 columns before the end of the first: the epilogue of a tile reads the shared 32 columns
+// first, and from then on (the other accumulator's previous tile being drained) the next tile's MMAs may start.
+constexpr uint32_t MX_ACC1 = 224;
+constexpr uint32_t MX_SFA = 480;      // 2 atoms x 4 columns
+constexpr uint32_t MX_SFB = 488;      // 2 atoms x 8 columns (256 weight rows)
+
+// Scales of one k-step from shared memory to tensor memory.  sa: the A atoms [2]; sb: the B atoms [row atom][2].
+template <int CTAS>
+__device__ __forceinline__ void mx_copy_step_scales(uint32_t tmem, uint32_t sa, uint32_t sb, int atoms) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if (j < atoms) {
+      tmem_copy_scales<CTAS>(tmem + MX_SFA + 4 * j, sa + j * kMxAtomBytes);
+      tmem_copy_scales<CTAS>(tmem + MX_SFB + 8 * j, sb + j * kMxAtomBytes);
+      tmem_copy_scales<CTAS>(tmem + MX_SFB + 8 * j + 4, sb + MX_SF_BYTES + j * kMxAtomBytes);
+    }
+  }
+}
+
+// Epilogue of one warp: TMEM lane quarter q, columns of `part` (0/1 of two).  `on_shared` runs once after the
+// first chunk has been read (the chunk holding the columns the two accumulators share, for the part that has it).
+template <int EPI, class F>
+__device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, const MxTile& tc, int acc, int row, int part,
+                                            uint8_t* stg, int lane, F&& on_first) {
+  const bool valid = row < tc.rows;
+  if constexpr (!mx_glu(EPI)) {
+    constexpr int CH = MX_BN / 64;            // 32-column chunks per part
+    unsigned long long dst = 0;
+    if (valid) dst = reinterpret_cast<unsigned long long>(p.out + static_cast<int64_t>(p.perm[tc.list_off + tc.row0 + row]) * p.ldo);
+#pragma unroll 1
+    for (int i = 0; i < CH; ++i) {
+      // accumulator 0 shares its last chunk, accumulator 1 its first
+      const int c = acc == 0 ? (part ? 2 * CH - 1 - i : CH - 1 - i) : part * CH + i;
+      uint32_t v[32];
+      tmem_ld_32x32(taddr + c * 32, v);
+      tmem_ld_wait();
+      if (i == 0) on_first();
+      const int n0 = tc.nt * MX_BN + c * 32;
+      if (n0 >= p.n_out) continue;            // warp-uniform
+      float f[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[e]);
+      mx_store_rows(f, dst, n0, p.n_out, stg, lane);
+    }
+  } else {
+    constexpr int HALF = MX_BN / 2;            // gate columns | up columns
+    constexpr int CH = HALF / 64;             // blocks of the product per part
+    const int64_t drow = tc.routed0 + row;
+#pragma unroll 1
+    for (int i = 0; i < CH; ++i) {
+      // shared columns: up block HALF/32 - 1 of accumulator 0 (part 1's last), gate block 0 of accumulator 1
+      const int c = acc == 0 ? (part ? 2 * CH - 1 - i : CH - 1 - i) : part * CH + i;
+      uint32_t g[32], u[32];
+      tmem_ld_32x32(taddr + c * 32, g);
+      tmem_ld_32x32(taddr + HALF + c * 32, u);
+      tmem_ld_wait();
+      if (i == 0) on_first();
+      const int n0 = tc.nt * HALF + c * 32;
+      float a[32], b[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        a[e] = __uint_as_float(g[e]);
+        b[e] = __uint_as_float(u[e]);
+      }
+      if constexpr (EPI == MX_EPI_GLU_SAVE) {
+        // kept in fp32: the gradients are taken at these values, and bf16 copies of them would add as much error to dx
+        // as its own rounding does
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (valid && n0 + 4 * j < p.n_out) {
+            const int64_t o = pre_tile_offset(drow, n0 + 4 * j, p.n_out);
+            *reinterpret_cast<float4*>(p.t1 + o) = make_float4(a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
+            *reinterpret_cast<float4*>(p.t3 + o) = make_float4(b[4 * j], b[4 * j + 1], b[4 * j + 2], b[4 * j + 3]);
+          }
+        }
+      }
+      // columns past h are weight rows that do not exist: zeros, whatever their scales hold
+#pragma unroll
+      for (int e = 0; e < 32; ++e) a[e] = n0 + e < p.n_out ? mx_silu_mul(a[e], b[e]) : 0.0f;
+      uint4 codes;
+      const uint32_t byte = mx_quantize_block(a, codes);
+      const int block = tc.nt * (HALF / 32) + c;
+      if (valid) {
+        // every scale byte of an atom is written, also those of blocks past h (0): the next contraction reads them
+        if (n0 < p.n_out) *reinterpret_cast<uint4*>(p.codes + drow * p.code_ld + block * 16) = codes;
+        if ((block >> 2) < p.k_atoms_out) p.scales[mx_scale_word(drow, block >> 2, p.k_atoms_out) + (block & 3)] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// One CTA per tile of 128 rows x 256 accumulator columns, persistent, warp specialised: warp 0 producer (TMA),
+// warp 1 scale copies and MMAs, warps 2..9 epilogue.
+// ---------------------------------------------------------------------------------------------
+constexpr int MX_B_BYTES = MX_BN * 128;
+constexpr int MX_STAGE_BYTES = MX_A_BYTES + MX_B_BYTES + 3 * MX_SF_BYTES;   // 51 KiB
+constexpr int MX_STAGES = 4;
+constexpr int MX_SMEM = MX_STAGES * MX_STAGE_BYTES + MX_STAGING + 256 + 1024;
+
+template <int EPI>
+__global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = smem + MX_STAGES * MX_STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + MX_STAGING);
+  uint64_t* empty = full + MX_STAGES;
+  uint64_t* tfull = empty + MX_STAGES;     // accumulator ready for the epilogue [2]
+  uint64_t* tempty = tfull + 2;            // the epilogue has read the first chunk of a tile
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < MX_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+    }
+    mbar_init(tempty, 8);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&maps.a);
+    tma_prefetch_desc(&maps.sa);
+    for (int i = 0; i < 4; ++i) {
+      tma_prefetch_desc(&maps.b[i]);
+      tma_prefetch_desc(&maps.sb[i]);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(tmem_slot, 512);
+    tmem_relinquish<1>();
+  }
+  griddep_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+
+  const int Mv = p.counts[0], Mt = p.counts[1], cap = p.counts[2];
+  const int tiles_v = (Mv + MX_BM - 1) / MX_BM;
+  const int m_tiles = tiles_v + (Mt + MX_BM - 1) / MX_BM;
+  constexpr int N_PER_TILE = mx_glu(EPI) ? MX_BN / 2 : MX_BN;
+  const int n_tiles = (p.n_out + N_PER_TILE - 1) / N_PER_TILE;
+  const int total = m_tiles * n_tiles;
+  const int k_steps = (p.k_bytes + 127) / 128;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t bytes = p.a_rows * 128 + MX_B_BYTES + MX_SF_BYTES + 2 * MX_SF_BYTES;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        const MxTile tc = mx_tile(t, MX_BM, 0, tiles_v, m_tiles, n_tiles, p.group_m, Mv, Mt, cap);
+        const CUtensorMap* b0 = &maps.b[tc.text ? 2 : 0];
+        const CUtensorMap* sb0 = &maps.sb[tc.text ? 2 : 0];
+        for (int ks = 0; ks < k_steps; ++ks) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
+            mx_report(p.status, ST_TIMEOUT_PRODUCER);
+            ok = false;
+            break;
+          }
+          uint8_t* a = smem + stage * MX_STAGE_BYTES;
+          uint8_t* b = a + MX_A_BYTES;
+          uint8_t* sa = b + MX_B_BYTES;
+          uint8_t* sb = sa + MX_SF_BYTES;
+          mbar_arrive_expect_tx(&full[stage], bytes);
+          if constexpr (mx_glu(EPI)) {
+            const int n0 = tc.nt * N_PER_TILE;
+            tma_load_2d(b, b0, &full[stage], ks * 128, n0);
+            tma_load_2d(b + MX_B_BYTES / 2, b0 + 1, &full[stage], ks * 128, n0);
+            tma_load_2d(sb, sb0, &full[stage], ks * 256, n0 / 128);
+            tma_load_2d(sb + MX_SF_BYTES, sb0 + 1, &full[stage], ks * 256, n0 / 128);
+          } else {
+            tma_load_2d(b, b0, &full[stage], ks * 128, tc.nt * MX_BN);
+            tma_load_2d(sb, sb0, &full[stage], ks * 256, tc.nt * (MX_BN / 128));
+          }
+          tma_load_2d(a, &maps.a, &full[stage], ks * 128, static_cast<int>(tc.routed0));
+          tma_load_2d(sa, &maps.sa, &full[stage], ks * 256, static_cast<int>(tc.routed0 >> 7));
+          ++issued;
+          if (++stage == MX_STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (*abort_flag) {
+        // let the copies already issued land before the CTA gives its shared memory back
+        for (int i = 0; i < (issued < MX_STAGES ? issued : MX_STAGES); ++i) {
+          if (--stage < 0) { stage = MX_STAGES - 1; phase ^= 1; }
+          int dummy = 0;
+          mbar_wait(&full[stage], phase, &dummy, 1000000ull);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++it) {
+        const int acc = it & 1;
+        const bool free = it == 0 || mbar_wait(tempty, (it - 1) & 1, abort_flag);
+        if (!free) {
+          mx_report(p.status, ST_TIMEOUT_MMA_TMEM);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + (acc ? MX_ACC1 : 0);
+        for (int ks = 0; ks < k_steps; ++ks) {
+          if (!mbar_wait(&full[stage], phase, abort_flag)) {
+            mx_report(p.status, ST_TIMEOUT_MMA_FULL);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = smem_u32(smem + stage * MX_STAGE_BYTES);
+          const uint32_t b = a + MX_A_BYTES;
+          const uint32_t sa = b + MX_B_BYTES;
+          const int left = p.k_bytes - ks * 128;                       // the contraction may end inside a k-step:
+          const int mmas = left >= 128 ? 4 : (left + 31) / 32;         // no MMA past its last scale atom
+          mx_copy_step_scales<1>(tmem, sa, sa + MX_SF_BYTES, (mmas + 1) / 2);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            if (kk < mmas)
+              umma_mxf4<1>(d, umma_smem_desc(a + kk * 32, 16, 1024), umma_smem_desc(b + kk * 32, 16, 1024),
+                           mx_idesc(MX_BM, MX_BN, (kk & 1) * 2), tmem + MX_SFA + 4 * (kk >> 1), tmem + MX_SFB + 8 * (kk >> 1),
+                           (ks | kk) != 0 ? 1u : 0u);
+          }
+          umma_commit(&empty[stage]);
+          if (++stage == MX_STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (ok) umma_commit(&tfull[acc]);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, part = (warp - 2) >> 2, row = q * 32 + lane;
+    int it = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x, ++it) {
+      const MxTile tc = mx_tile(t, MX_BM, 0, tiles_v, m_tiles, n_tiles, p.group_m, Mv, Mt, cap);
+      const int acc = it & 1;
+      int w = 1;
+      if (lane == 0) w = mbar_wait(&tfull[acc], (it >> 1) & 1, abort_flag) ? 1 : 0;
+      if (!__shfl_sync(0xFFFFFFFFu, w, 0)) {
+        if (lane == 0) mx_report(p.status, ST_TIMEOUT_EPILOGUE);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + (acc ? MX_ACC1 : 0);
+      mx_epilogue<EPI>(taddr, p, tc, acc, row, part, staging + (warp - 2) * 2048, lane, [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty);
+      });
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+struct MxWeight {
+  const void* codes;
+  const void* scales;
+};
+
+// codes [rows, ld bytes], box of 128 bytes x box_rows; scales as [row atoms][k atoms x 128 words], box of two atoms
+// (1 KiB) x box_atoms.  Boxes past the end read zeros.
+static int mx_maps(CUtensorMap* codes, CUtensorMap* scales, const MxWeight& w, int64_t rows, int64_t cols, int box_rows,
+                   int box_atoms) {
+  int r = make_tensor_map_2d_of(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes, mx_code_ld(cols), rows, mx_code_ld(cols), 128,
+                                box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (r) return r;
+  return make_tensor_map_2d_of(scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, w.scales, mx_k_atoms(cols) * (kMxAtomBytes / 4),
+                               mx_row_atoms(rows), mx_k_atoms(cols) * kMxAtomBytes, 256, box_atoms, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+// Row tiles of a super-tile: about 16 MiB of activation codes stay in L2 while the weights pass.
+static int mx_group_m(int64_t k, int64_t rows_per_tile) {
+  int64_t g = (16ll << 20) / (rows_per_tile * mx_code_ld(k) + 1);
+  return static_cast<int>(g < 4 ? 4 : (g > 64 ? 64 : g));
+}
+
+static int mx_a_box_rows(int64_t M) { return M >= MX_BM ? MX_BM : static_cast<int>((M + 7) / 8 * 8); }
+
+template <int EPI>
+static int mx_launch(const MxMaps& maps, const MxParams& p, int64_t M, cudaStream_t stream) {
+  const DeviceInfo& dev = device_info();
+  if (dev.cc_major != 10) return FFNK_ERR_DEVICE;
+  const int n_per_tile = mx_glu(EPI) ? MX_BN / 2 : MX_BN;
+  int64_t grid = ((M + MX_BM - 1) / MX_BM + 1) * ((p.n_out + n_per_tile - 1) / n_per_tile);
+  if (grid > usable_sms()) grid = usable_sms();
+  const cudaError_t e = cudaFuncSetAttribute(mx_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, MX_SMEM);
+  if (e != cudaSuccess) return cuda_status(e);
+  mx_gemm_kernel<EPI><<<static_cast<unsigned>(grid), MX_THREADS, MX_SMEM, stream>>>(maps, p);
+  return cuda_status(cudaGetLastError());
+}
+
+// y[token] = routed rows of (codes, scales) by the modality's weight [N, K]
+static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt, const int32_t* perm, const int32_t* counts,
+                      void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int32_t* status, cudaStream_t s) {
+  MxMaps m;
+  int r;
+  const int64_t rows = ffnk_route_capacity(M) + 512;
+  if ((r = mx_maps(&m.a, &m.sa, a, rows, K, mx_a_box_rows(M), 1))) return r;
+  if ((r = mx_maps(&m.b[0], &m.sb[0], wv, N, K, MX_BN, 2))) return r;
+  if ((r = mx_maps(&m.b[2], &m.sb[2], wt, N, K, MX_BN, 2))) return r;
+  m.b[1] = m.b[0]; m.b[3] = m.b[2]; m.sb[1] = m.sb[0]; m.sb[3] = m.sb[2];
+  MxParams p{};
+  p.perm = perm; p.counts = counts; p.status = status;
+  p.n_out = static_cast<int>(N);
+  p.k_bytes = static_cast<int>(mx_code_ld(K));
+  p.a_rows = mx_a_box_rows(M);
+  p.group_m = mx_group_m(K, MX_BM);
+  p.out = static_cast<__nv_bfloat16*>(y);
+  p.ldo = ldy;
+  return mx_launch<MX_EPI_STORE>(m, p, M, s);
+}
+
+// quantised silu(gate) * up of the routed rows, optionally with the pre-activations kept (t1, t3 both or neither)
+static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* perm, const int32_t* counts, void* codes,
+                     void* scales, void* t1, void* t3, int64_t M, int64_t d, int64_t h, int32_t* status, cudaStream_t s) {
+  MxMaps m;
+  int r;
+  const int64_t rows = ffnk_route_capacity(M) + 512;
+  if ((r = mx_maps(&m.a, &m.sa, a, rows, d, mx_a_box_rows(M), 1))) return r;
+  for (int i = 0; i < 4; ++i)
+    if ((r = mx_maps(&m.b[i], &m.sb[i], w[i], h, d, MX_BN / 2, 1))) return r;
+  MxParams p{};
+  p.perm = perm; p.counts = counts; p.status = status;
+  p.n_out = static_cast<int>(h);
+  p.k_bytes = static_cast<int>(mx_code_ld(d));
+  p.a_rows = mx_a_box_rows(M);
+  p.group_m = mx_group_m(d, MX_BM);
+  p.codes = static_cast<uint8_t*>(codes);
+  p.scales = static_cast<uint8_t*>(scales);
+  p.code_ld = mx_code_ld(h);
+  p.k_atoms_out = static_cast<int>(mx_k_atoms(h));
+  p.t1 = static_cast<float*>(t1);
+  p.t3 = static_cast<float*>(t3);
+  return t1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, s) : mx_launch<MX_EPI_GLU>(m, p, M, s);
+}
+
+static int64_t mx_align(int64_t v) { return (v + 255) & ~int64_t(255); }
+
+// Workspace of one call.  The routing lists come first and have a size of their own, because a backward pass needs
+// them again; everything else is scratch.
+struct MxWorkspace {
+  int64_t scan, xc, xs, hc, hs, total;
+};
+static MxWorkspace mx_workspace(int64_t M, int64_t K, int64_t h) {
+  MxWorkspace w{};
+  const int64_t rows = ffnk_route_capacity(M) + 512;
+  int64_t off = 0;
+  w.scan = off; off += mx_align(ffnk_route_workspace_bytes(M));
+  w.xc = off;   off += mx_align(rows * mx_code_ld(K));
+  w.xs = off;   off += mx_align(mx_row_atoms(rows) * mx_k_atoms(K) * kMxAtomBytes);
+  w.hc = off;   off += h ? mx_align(rows * mx_code_ld(h)) : 0;
+  w.hs = off;   off += h ? mx_align(mx_row_atoms(rows) * mx_k_atoms(h) * kMxAtomBytes) : 0;
+  w.total = off;
+  return w;
+}
+
+static bool mx_bad_dim(int64_t v) { return v < 8 || (v & 7) || v >= (1ll << 30); }
+static bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+}  // namespace ffnk
+
+using namespace ffnk;
+
+extern "C" int64_t ffnk_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t h) {
+  if (M <= 0 || K <= 0 || h < 0) return 256;
+  return mx_workspace(M, K, h).total;
+}
+
+extern "C" int ffnk_mxfp4_linear_forward(const void* x, int64_t ldx, const void* b1_codes, const void* b1_scales,
+                                         const void* b2_codes, const void* b2_scales, const void* mask, int32_t* perm,
+                                         int32_t* counts, void* workspace, int64_t workspace_bytes, void* y, int64_t ldy,
+                                         int64_t M, int64_t N, int64_t K, int32_t* status, void* stream) {
+  if (M == 0) return 0;
+  if (!x || !b1_codes || !b1_scales || !b2_codes || !b2_scales || !mask || !perm || !counts || !workspace || !y || !status)
+    return FFNK_ERR_NULL;
+  if (M < 0 || M >= (1ll << 30) || mx_bad_dim(N) || mx_bad_dim(K)) return FFNK_ERR_SHAPE;
+  if ((ldx & 7) || (ldy & 7) || ldx < K || ldy < N || misaligned(x) || misaligned(y) || misaligned(b1_codes) ||
+      misaligned(b1_scales) || misaligned(b2_codes) || misaligned(b2_scales) || misaligned(perm) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return FFNK_ERR_ALIGN;
+  const MxWorkspace w = mx_workspace(M, K, 0);
+  if (workspace_bytes < w.total) return FFNK_ERR_CAPACITY;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  int r = mx_route_quantize(mask, M, x, ldx, K, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
+  if (r) return r;
+  return mx_product(MxWeight{ws + w.xc, ws + w.xs}, MxWeight{b1_codes, b1_scales}, MxWeight{b2_codes, b2_scales}, perm, counts,
+                    y, ldy, M, N, K, status, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* const* codes, const void* const* scales,
+                                      const void* mask, int32_t* perm, int32_t* counts, void* workspace,
+                                      int64_t workspace_bytes, void* t1, void* t3, void* y, int64_t ldy, int64_t M, int64_t d,
+                                      int64_t h, int32_t* status, void* stream) {
+  if (M == 0) return 0;
+  if (!x || !codes || !scales || !mask || !perm || !counts || !workspace || !y || !status || !t1 != !t3) return FFNK_ERR_NULL;
+  for (int i = 0; i < 6; ++i)
+    if (!codes[i] || !scales[i]) return FFNK_ERR_NULL;
+  if (M < 0 || M >= (1ll << 30) || mx_bad_dim(d) || mx_bad_dim(h)) return FFNK_ERR_SHAPE;
+  if ((ldx & 7) || (ldy & 7) || ldx < d || ldy < d || misaligned(x) || misaligned(y) || misaligned(perm) || misaligned(t1) ||
+      misaligned(t3) || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return FFNK_ERR_ALIGN;
+  for (int i = 0; i < 6; ++i)
+    if (misaligned(codes[i]) || misaligned(scales[i])) return FFNK_ERR_ALIGN;
+  const MxWorkspace w = mx_workspace(M, d, h);
+  if (workspace_bytes < w.total) return FFNK_ERR_CAPACITY;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int r = mx_route_quantize(mask, M, x, ldx, d, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
+  if (r) return r;
+  const MxWeight gu[4] = {{codes[0], scales[0]}, {codes[2], scales[2]}, {codes[3], scales[3]}, {codes[5], scales[5]}};
+  if ((r = mx_gateup(MxWeight{ws + w.xc, ws + w.xs}, gu, perm, counts, ws + w.hc, ws + w.hs, t1, t3, M, d, h, status, s))) return r;
+  return mx_product(MxWeight{ws + w.hc, ws + w.hs}, MxWeight{codes[1], scales[1]}, MxWeight{codes[4], scales[4]}, perm, counts, y,
+                    ldy, M, d, h, status, s);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Backward passes: gradients of the activations, the weights being frozen.  The contraction runs over the other
+// dimension of the weights than their blocks do, so the weights are read back to bf16 (exactly) and the bf16
+// GEMMs of the framework do the rest; the rounding of activations to 4 bits counts as the identity.
+// ---------------------------------------------------------------------------------------------
+namespace ffnk {
+struct MxBackwardSpace {
+  int64_t gr, dt1, dt3, w[6], total;
+};
+static MxBackwardSpace mx_backward_space(int64_t M, int64_t K, int64_t N, int64_t h) {
+  MxBackwardSpace w{};
+  const int64_t rows = ffnk_route_capacity(M) + 512;
+  int64_t off = 0;
+  w.gr = off;
+  off += mx_align(rows * N * 2);
+  if (h) {
+    w.dt1 = off; off += mx_align(rows * h * 2);
+    w.dt3 = off; off += mx_align(rows * h * 2);
+  }
+  for (int i = 0; i < (h ? 6 : 2); ++i) {
+    w.w[i] = off;
+    off += mx_align((h ? h : N) * K * 2);
+  }
+  w.total = off;
+  return w;
+}
+}  // namespace ffnk
+
+extern "C" int64_t ffnk_mxfp4_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t h) {
+  if (M <= 0 || K <= 0 || N <= 0 || h < 0) return 256;
+  return mx_backward_space(M, K, N, h).total;
+}
+
+extern "C" int ffnk_mxfp4_linear_backward(const void* g, int64_t ldg, const void* b1_codes, const void* b1_scales,
+                                          const void* b2_codes, const void* b2_scales, const int32_t* perm,
+                                          const int32_t* counts, void* workspace, int64_t workspace_bytes, void* dx,
+                                          int64_t lddx, int64_t M, int64_t N, int64_t K, int32_t* status, void* stream) {
+  if (M == 0) return 0;
+  if (!g || !b1_codes || !b1_scales || !b2_codes || !b2_scales || !perm || !counts || !workspace || !dx || !status)
+    return FFNK_ERR_NULL;
+  if (M < 0 || M >= (1ll << 30) || mx_bad_dim(N) || mx_bad_dim(K)) return FFNK_ERR_SHAPE;
+  if ((ldg & 7) || (lddx & 7) || ldg < N || lddx < K || misaligned(g) || misaligned(dx) || misaligned(b1_codes) ||
+      misaligned(b1_scales) || misaligned(b2_codes) || misaligned(b2_scales) || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return FFNK_ERR_ALIGN;
+  const MxBackwardSpace w = mx_backward_space(M, K, N, 0);
+  if (workspace_bytes < w.total) return FFNK_ERR_CAPACITY;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const void* codes[2] = {b1_codes, b2_codes};
+  const void* scales[2] = {b1_scales, b2_scales};
+  const int64_t rows[2] = {N, N}, cols[2] = {K, K};
+  const int gate[2] = {0, 1};
+  void* wd[2] = {ws + w.w[0], ws + w.w[1]};
+  int r = mx_dequantize_weights(codes, scales, rows, cols, gate, 2, counts, wd, stream);
+  if (r) return r;
+  if ((r = ffnk_permute_rows(g, ldg, perm, counts, ws + w.gr, N, M, N, stream))) return r;
+  return ffnk_ffn_down(ws + w.gr, N, wd[0], wd[1], K, 1, perm, counts, dx, lddx, M, K, N, status, stream);
+}
+
+extern "C" int ffnk_mxfp4_ffn_backward(const void* gy, int64_t ldg, const void* const* codes, const void* const* scales,
+                                       const void* t1, const void* t3, const int32_t* perm, const int32_t* counts,
+                                       void* workspace, int64_t workspace_bytes, void* dx, int64_t lddx, int64_t M, int64_t d,
+                                       int64_t h, int32_t* status, void* stream) {
+  if (M == 0) return 0;
+  if (!gy || !codes || !scales || !t1 || !t3 || !perm || !counts || !workspace || !dx || !status) return FFNK_ERR_NULL;
+  for (int i = 0; i < 6; ++i)
+    if (!codes[i] || !scales[i]) return FFNK_ERR_NULL;
+  if (M < 0 || M >= (1ll << 30) || mx_bad_dim(d) || mx_bad_dim(h)) return FFNK_ERR_SHAPE;
+  if ((ldg & 7) || (lddx & 7) || ldg < d || lddx < d || misaligned(gy) || misaligned(dx) || misaligned(t1) || misaligned(t3) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return FFNK_ERR_ALIGN;
+  for (int i = 0; i < 6; ++i)
+    if (misaligned(codes[i]) || misaligned(scales[i])) return FFNK_ERR_ALIGN;
+  const MxBackwardSpace w = mx_backward_space(M, d, d, h);
+  if (workspace_bytes < w.total) return FFNK_ERR_CAPACITY;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  int64_t rows[6], cols[6];
+  const int gate[6] = {0, 0, 0, 1, 1, 1};
+  void* wd[6];
+  for (int i = 0; i < 6; ++i) {
+    rows[i] = i % 3 == 1 ? d : h;
+    cols[i] = i % 3 == 1 ? h : d;
+    wd[i] = ws + w.w[i];
+  }
+  const int r = mx_dequantize_weights(codes, scales, rows, cols, gate, 6, counts, wd, stream);
+  if (r) return r;
+  return ffn_backward_dx(gy, ldg, t1, t3, wd[0], wd[1], wd[2], wd[3], wd[4], wd[5], perm, counts, ws + w.gr, ws + w.dt1,
+                         ws + w.dt3, dx, lddx, M, d, h, status, stream);
+}

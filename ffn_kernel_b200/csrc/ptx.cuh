@@ -46,6 +46,13 @@ __device__ __forceinline__ bool mask_is_scattered(const int* counts, int run_thr
   return static_cast<long long>(counts[4]) * run_threshold > counts[3];
 }
 
+// Pre-activations kept in fp32 between the forward and the backward pass of the FFN on 4-bit weights: element (routed
+// row, column) of a matrix `h` columns wide in tiles of 128 rows x 4 columns, so that the 32 rows of a warp are 512
+// contiguous bytes (columns in fours).
+__device__ __forceinline__ int64_t pre_tile_offset(int64_t row, int col, int h) {
+  return (((row >> 7) * (h >> 2) + (col >> 2)) * 128 + (row & 127)) * 4 + (col & 3);
+}
+
 __device__ __forceinline__ uint32_t lane_id() { return threadIdx.x & 31; }
 
 // ---------------------------------------------------------------------------------------------

@@ -63,7 +63,9 @@ enum { A_GATHER = 0, A_ROUTED = 1 };
 // EPI_DSWIGLU     : acc = dH; with t1 = aux0, t3 = aux1 at the same position:
 //                   out = dH * t3 * s * (1 + t1 * (1 - s)),  aux2 = dH * t1 * s,  s = sigmoid(t1)
 //                   (the element-wise terms of the FFN backward, reference README.md:159-172)
-enum { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_SWIGLU_SAVE = 2, EPI_DSWIGLU = 3 };
+// EPI_DSWIGLU_F32 : the same with t1, t3 in fp32, in the tiled order of pre_tile_offset (the forward pass on 4-bit
+//                   weights leaves them so)
+enum { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_SWIGLU_SAVE = 2, EPI_DSWIGLU = 3, EPI_DSWIGLU_F32 = 4 };
 __host__ __device__ constexpr bool epi_glu(int e) { return e == EPI_SWIGLU || e == EPI_SWIGLU_SAVE; }
 // OUT_SCATTER : row of token t -> out[t]            OUT_ROUTED : row i of the routed order -> out[i]
 // OUT_PEER    : row of token t -> row block `peer_rank` of the buffer of the rank that owns token t
@@ -307,7 +309,10 @@ __device__ __forceinline__ void epilogue_glu_staged(uint32_t taddr, const GemmPa
 // dSwiGLU epilogue (FFN backward) with the same shared-memory transposition, for the two loads of
 // the saved pre-activations as well as for the two stores: four accesses per element, each of which
 // would otherwise touch 32 rows per instruction.
-template <int BN_T>
+//
+// F32: t1 and t3 come in fp32 in the tiled order instead, a lane's own row at a time: the 32 lanes of a warp read 512
+// contiguous bytes an access and nothing is transposed.
+template <int BN_T, bool F32 = false>
 __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const GemmParams& p, long long row_off,
                                                         int n_base, int part, int parts, uint8_t* stg, int lane) {
   constexpr int CH = BN_T / 32;
@@ -361,19 +366,43 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
   };
   const int c_begin = part * CH / parts, c_end = (part + 1) * CH / parts;
   uint4 l1[4], l3[4];
-  load4(l1, p.aux0, n_base + c_begin * 32);
-  load4(l3, p.aux1, n_base + c_begin * 32);
+  if constexpr (!F32) {
+    load4(l1, p.aux0, n_base + c_begin * 32);
+    load4(l3, p.aux1, n_base + c_begin * 32);
+  }
+  const int my_row = row_off >= 0 ? static_cast<int>(row_off / p.ldo) : -1;
+  float4 f1[8], f3[8];
+  auto load_tiled = [&](float4 (&l)[8], const __nv_bfloat16* base, int n0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      l[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (my_row >= 0 && n0 + 4 * j < p.n_out)
+        l[j] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + pre_tile_offset(my_row, n0 + 4 * j, p.n_out));
+    }
+  };
+  if constexpr (F32) {
+    load_tiled(f1, p.aux0, n_base + c_begin * 32);
+    load_tiled(f3, p.aux1, n_base + c_begin * 32);
+  }
 #pragma unroll 1
   for (int c = c_begin; c < c_end; ++c) {
     uint32_t acc[32];
     tmem_ld_32x32(taddr + c * 32, acc);
     const int n0 = n_base + c * 32;
     float t1[32], t3[32];
-    spread(t1, l1);
-    spread(t3, l3);
-    if (c + 1 < c_end) {             // the next chunk's loads fly while this one is computed and stored
-      load4(l1, p.aux0, n0 + 32);
-      load4(l3, p.aux1, n0 + 32);
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        t1[4 * j] = f1[j].x; t1[4 * j + 1] = f1[j].y; t1[4 * j + 2] = f1[j].z; t1[4 * j + 3] = f1[j].w;
+        t3[4 * j] = f3[j].x; t3[4 * j + 1] = f3[j].y; t3[4 * j + 2] = f3[j].z; t3[4 * j + 3] = f3[j].w;
+      }
+    } else {
+      spread(t1, l1);
+      spread(t3, l3);
+      if (c + 1 < c_end) {           // the next chunk's loads fly while this one is computed and stored
+        load4(l1, p.aux0, n0 + 32);
+        load4(l3, p.aux1, n0 + 32);
+      }
     }
     tmem_ld_wait();
     if (n0 >= p.n_out) continue;   // warp-uniform
@@ -384,6 +413,10 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
       const float d1 = dh * t3[e] * sg * (1.0f + t1[e] * (1.0f - sg));
       t3[e] = dh * t1[e] * sg;     // d3
       t1[e] = d1;
+    }
+    if (F32 && c + 1 < c_end) {      // the accumulator's registers are free now: the next chunk's loads fly under the stores
+      load_tiled(f1, p.aux0, n0 + 32);
+      load_tiled(f3, p.aux1, n0 + 32);
     }
     flush(t1, p.out, n0);
     flush(t3, p.aux2, n0);
@@ -811,8 +844,8 @@ routed_gemm_kernel(const __grid_constant__ AMaps am, const __grid_constant__ CUt
       if constexpr (epi_glu(EPI))
         epilogue_glu_staged<EPI, BN_T>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * (BN_T / 2), part,
                                        epilogue_parts(), smem + TSTAGES * TSTAGE_BYTES + 256 + (warp - 2) * 2048, lane);
-      else if constexpr (EPI == EPI_DSWIGLU)
-        epilogue_dswiglu_staged<BN_T>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * BN_T, part, epilogue_parts(),
+      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_F32)
+        epilogue_dswiglu_staged<BN_T, EPI == EPI_DSWIGLU_F32>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * BN_T, part, epilogue_parts(),
                                       smem + TSTAGES * TSTAGE_BYTES + 256 + (warp - 2) * 2048, lane);
       else
         epilogue_rows_staged<BN_T>(taddr, p, OUT_MODE == OUT_PEER ? peer_dst : (valid ? p.out + dst_row * p.ldo : nullptr),
@@ -1094,8 +1127,8 @@ routed_gemm_pair_kernel(const __grid_constant__ AMaps am, const __grid_constant_
       if constexpr (epi_glu(EPI))
         epilogue_glu_staged<EPI, BN>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * N_PER_TILE, part,
                                      epilogue_parts(), smem + PAIR_STAGES * PAIR_STAGE_BYTES + 256 + (warp - 2) * 2048, lane);
-      else if constexpr (EPI == EPI_DSWIGLU)
-        epilogue_dswiglu_staged<BN>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * N_PER_TILE, part, epilogue_parts(),
+      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_F32)
+        epilogue_dswiglu_staged<BN, EPI == EPI_DSWIGLU_F32>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * N_PER_TILE, part, epilogue_parts(),
                                     smem + PAIR_STAGES * PAIR_STAGE_BYTES + 256 + (warp - 2) * 2048, lane);
       else
         epilogue_rows_staged<BN>(taddr, p, OUT_MODE == OUT_PEER ? peer_dst : (valid ? p.out + dst_row * p.ldo : nullptr),
@@ -1726,6 +1759,7 @@ static int usable_sms(const DeviceInfo& dev) {
   int n = dev.sm_count - g_sm_margin;
   return n < 2 ? 2 : n;
 }
+int usable_sms() { return usable_sms(device_info()); }
 
 // Row tiles per super-tile.  One super-tile of A rows should stay in L2 while the weights stream past
 // it: about 32 MiB of A for single CTAs (128-row tiles), about 16 MiB for CTA pairs (256-row tiles).
@@ -2343,6 +2377,59 @@ extern "C" int ffnk_ffn_forward_train(const void* x, int64_t ldx, const void* w1
   return ffnk_ffn_down(hid, h, w2, u2, w2_stride_k, w2_stride_n, perm, counts, y, ldy, M, d, h, status, stream);
 }
 
+namespace ffnk {
+// (dt1, dt3) = dswiglu(gr @ W2^T): contraction over d, output columns over h
+template <int EPI>
+static int dswiglu_gemm(const void* gr, const void* w2, const void* u2, int64_t w2_stride_k, int64_t w2_stride_n, const void* t1,
+                        const void* t3, const int32_t* perm, const int32_t* counts, void* dt1, void* dt3, int64_t M, int64_t d,
+                        int64_t h, int32_t* status, cudaStream_t s) {
+  const int64_t rows = ffnk_route_capacity(M) + 512;
+  AMaps tmA;
+  CUtensorMap tmB[4];
+  int r = make_tensor_map_2d(&tmA.m[RUN_LEVELS], gr, d, rows, d, BK, BM);
+  if (r) return r;
+  for (int i = 0; i <= COPY_MAP; ++i)
+    if (i != RUN_LEVELS) tmA.m[i] = tmA.m[RUN_LEVELS];
+  bool mn1 = false, mn2 = false;
+  const TileChoice tile = pick_tile(M, h, A_ROUTED, EPI, weights_k_major(w2_stride_n, w2_stride_k, d));
+  if ((r = weight_map(&tmB[0], WeightView{w2, w2_stride_n, w2_stride_k, d, h}, &mn1, tile.bn / 2))) return r;
+  if ((r = weight_map(&tmB[2], WeightView{u2, w2_stride_n, w2_stride_k, d, h}, &mn2, tile.bn / 2))) return r;
+  tmB[1] = tmB[0];
+  tmB[3] = tmB[2];
+  GemmParams p{perm, counts, static_cast<__nv_bfloat16*>(dt1), h, static_cast<int>(h), static_cast<int>(d),
+               static_cast<int>(rows), pick_group_m(d), max_run_rows(), status, g_prof_buffer};
+  p.aux0 = static_cast<__nv_bfloat16*>(const_cast<void*>(t1));
+  p.aux1 = static_cast<__nv_bfloat16*>(const_cast<void*>(t3));
+  p.aux2 = static_cast<__nv_bfloat16*>(dt3);
+  return launch_gemm<A_ROUTED, EPI, OUT_ROUTED>(tmA, tmB, mn1, p, M, tile, s);
+}
+
+// dx[token] = dt1 @ W1^T + dt3 @ W3^T: two contraction segments of length h into one accumulator
+static int ffn_dx_gemm(const void* dt1, const void* dt3, const void* w1, const void* w3, const void* u1, const void* u3,
+                       int64_t w13_stride_k, int64_t w13_stride_n, const int32_t* perm, const int32_t* counts, void* dx,
+                       int64_t lddx, int64_t M, int64_t d, int64_t h, int32_t* status, cudaStream_t s) {
+  const int64_t rows = ffnk_route_capacity(M) + 512;
+  AMaps tmA;
+  CUtensorMap tmB[4];
+  int r = make_tensor_map_2d(&tmA.m[RUN_LEVELS], dt1, h, rows, h, BK, BM);
+  if (r) return r;
+  for (int i = 0; i <= COPY_MAP; ++i)
+    if (i != RUN_LEVELS) tmA.m[i] = tmA.m[RUN_LEVELS];
+  if ((r = make_tensor_map_2d(&tmA.m[RUN_LEVELS - 1], dt3, h, rows, h, BK, BM))) return r;
+  bool mn = false, mn_i = false;
+  const void* ws[4] = {w1, w3, u1, u3};
+  const TileChoice tile = pick_tile(M, d, A_ROUTED, EPI_STORE, weights_k_major(w13_stride_n, w13_stride_k, h));
+  for (int i = 0; i < 4; ++i) {
+    if ((r = weight_map(&tmB[i], WeightView{ws[i], w13_stride_n, w13_stride_k, h, d}, &mn_i, tile.bn / 2))) return r;
+    mn = mn_i;
+  }
+  GemmParams p{perm, counts, static_cast<__nv_bfloat16*>(dx), lddx, static_cast<int>(d), static_cast<int>(h),
+               static_cast<int>(rows), pick_group_m(2 * h), max_run_rows(), status, g_prof_buffer};
+  p.k_len1 = static_cast<int>(h);
+  return launch_gemm<A_ROUTED, EPI_STORE, OUT_SCATTER>(tmA, tmB, mn, p, M, tile, s);
+}
+}  // namespace ffnk
+
 extern "C" int ffnk_ffn_backward(const void* gy, int64_t ldg, const void* xr, const void* t1, const void* t3,
                                  const void* hid, const void* w1, const void* w2, const void* w3, const void* u1,
                                  const void* u2, const void* u3, int64_t w13_stride_k, int64_t w13_stride_n,
@@ -2366,26 +2453,8 @@ extern "C" int ffnk_ffn_backward(const void* gy, int64_t ldg, const void* xr, co
   int r = ffnk_permute_rows(gy, ldg, perm, counts, gr, d, M, d, stream);
   if (r) return r;
 
-  // (dt1, dt3) = dswiglu(gr @ W2^T): contraction over d, output columns over h
-  {
-    AMaps tmA;
-    CUtensorMap tmB[4];
-    if ((r = make_tensor_map_2d(&tmA.m[RUN_LEVELS], gr, d, rows, d, BK, BM))) return r;
-    for (int i = 0; i <= COPY_MAP; ++i)
-      if (i != RUN_LEVELS) tmA.m[i] = tmA.m[RUN_LEVELS];
-    bool mn1 = false, mn2 = false;
-    const TileChoice tile = pick_tile(M, h, A_ROUTED, EPI_DSWIGLU, weights_k_major(w2_stride_n, w2_stride_k, d));
-    if ((r = weight_map(&tmB[0], WeightView{w2, w2_stride_n, w2_stride_k, d, h}, &mn1, tile.bn / 2))) return r;
-    if ((r = weight_map(&tmB[2], WeightView{u2, w2_stride_n, w2_stride_k, d, h}, &mn2, tile.bn / 2))) return r;
-    tmB[1] = tmB[0];
-    tmB[3] = tmB[2];
-    GemmParams p{perm, counts, static_cast<__nv_bfloat16*>(dt1), h, static_cast<int>(h), static_cast<int>(d),
-                 static_cast<int>(rows), pick_group_m(d), max_run_rows(), status, g_prof_buffer};
-    p.aux0 = static_cast<__nv_bfloat16*>(const_cast<void*>(t1));
-    p.aux1 = static_cast<__nv_bfloat16*>(const_cast<void*>(t3));
-    p.aux2 = static_cast<__nv_bfloat16*>(dt3);
-    if ((r = launch_gemm<A_ROUTED, EPI_DSWIGLU, OUT_ROUTED>(tmA, tmB, mn1, p, M, tile, s))) return r;
-  }
+  if ((r = dswiglu_gemm<EPI_DSWIGLU>(gr, w2, u2, w2_stride_k, w2_stride_n, t1, t3, perm, counts, dt1, dt3, M, d, h, status, s)))
+    return r;
   // weight gradients, written in each weight's storage order
   if (w2_k) r = launch_wgrad(gr, d, d, hid, h, h, rows, dw2, du2, w2_stride_n, 1, perm, counts, status, s);   // [d][h]
   else r = launch_wgrad(hid, h, h, gr, d, d, rows, dw2, du2, w2_stride_k, 1, perm, counts, status, s);       // [h][d]
@@ -2397,26 +2466,18 @@ extern "C" int ffnk_ffn_backward(const void* gy, int64_t ldg, const void* xr, co
     if ((r = launch_wgrad(xr, d, d, dt1, h, h, rows, dw1, du1, w13_stride_k, 1, perm, counts, status, s))) return r;
     if ((r = launch_wgrad(xr, d, d, dt3, h, h, rows, dw3, du3, w13_stride_k, 1, perm, counts, status, s))) return r;
   }
-  // dx[token] = dt1 @ W1^T + dt3 @ W3^T: two contraction segments of length h into one accumulator
-  {
-    AMaps tmA;
-    CUtensorMap tmB[4];
-    if ((r = make_tensor_map_2d(&tmA.m[RUN_LEVELS], dt1, h, rows, h, BK, BM))) return r;
-    for (int i = 0; i <= COPY_MAP; ++i)
-      if (i != RUN_LEVELS) tmA.m[i] = tmA.m[RUN_LEVELS];
-    if ((r = make_tensor_map_2d(&tmA.m[RUN_LEVELS - 1], dt3, h, rows, h, BK, BM))) return r;
-    bool mn = false, mn_i = false;
-    const void* ws[4] = {w1, w3, u1, u3};
-    const TileChoice tile = pick_tile(M, d, A_ROUTED, EPI_STORE, weights_k_major(w13_stride_n, w13_stride_k, h));
-    for (int i = 0; i < 4; ++i) {
-      if ((r = weight_map(&tmB[i], WeightView{ws[i], w13_stride_n, w13_stride_k, h, d}, &mn_i, tile.bn / 2))) return r;
-      mn = mn_i;
-    }
-    GemmParams p{perm, counts, static_cast<__nv_bfloat16*>(dx), lddx, static_cast<int>(d), static_cast<int>(h),
-                 static_cast<int>(rows), pick_group_m(2 * h), max_run_rows(), status, g_prof_buffer};
-    p.k_len1 = static_cast<int>(h);
-    return launch_gemm<A_ROUTED, EPI_STORE, OUT_SCATTER>(tmA, tmB, mn, p, M, tile, s);
-  }
+  return ffn_dx_gemm(dt1, dt3, w1, w3, u1, u3, w13_stride_k, w13_stride_n, perm, counts, dx, lddx, M, d, h, status, s);
+}
+
+int ffnk::ffn_backward_dx(const void* gy, int64_t ldg, const void* t1, const void* t3, const void* w1, const void* w2,
+                          const void* w3, const void* u1, const void* u2, const void* u3, const int32_t* perm,
+                          const int32_t* counts, void* gr, void* dt1, void* dt3, void* dx, int64_t lddx, int64_t M, int64_t d,
+                          int64_t h, int32_t* status, void* stream) {
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int r = ffnk_permute_rows(gy, ldg, perm, counts, gr, d, M, d, stream);
+  if (r) return r;
+  if ((r = dswiglu_gemm<EPI_DSWIGLU_F32>(gr, w2, u2, 1, h, t1, t3, perm, counts, dt1, dt3, M, d, h, status, s))) return r;
+  return ffn_dx_gemm(dt1, dt3, w1, w3, u1, u3, 1, d, perm, counts, dx, lddx, M, d, h, status, s);
 }
 
 extern "C" int ffnk_debug_profile_buffer(void* buffer) {

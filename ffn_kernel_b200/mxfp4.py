@@ -1,0 +1,285 @@
+"""MXFP4: 4-bit floating point with one power-of-two scale per 32 values, and the routed operators on it.
+
+The reference computes in bf16 only; this module adds the same two layers with weights held in 4 bits (4.25
+bits a value with its share of the scales) and multiplied on the 4-bit tensor-core path:
+
+``quantize_mxfp4(x, dim)`` / ``dequantize_mxfp4(q, dtype)``  a matrix into the format and back,
+``MXFP4MaskedLinear.apply(a, q1, q2, mask)``                 ``MaskedLinear`` on 4-bit weights,
+``MXFP4MaskedFFN.apply(a, q_w1, ..., q_u3, mask)``           ``MaskedFFN`` on 4-bit weights.
+
+Activations come and go in bf16 and are quantised inside the call, row by row in blocks of 32 along the
+contraction, so a token's result depends on that token alone.  Gradients reach the activations (the rounding to 4 bits counts as
+the identity); the weights are frozen.  A block that holds an infinity or a NaN reads back as NaN.
+"""
+from __future__ import annotations
+
+import ctypes
+from contextlib import nullcontext
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from ._lib import check, lib
+from .linear import _activation, _check_dims
+from .route import _require_cuda, maybe_check, status_word, stream_ptr
+
+__all__ = ["MXFP4Tensor", "quantize_mxfp4", "dequantize_mxfp4", "MXFP4MaskedLinear", "MXFP4MaskedFFN"]
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_Six = ctypes.c_void_p * 6
+
+
+def _on(dev):
+    """Makes ``dev`` the current device for the block (nothing to do where it is already)."""
+    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+class MXFP4Tensor:
+    """A matrix [rows, cols] in MXFP4, blocks of 32 along the columns (the contraction: a weight is [out, in]).
+
+    codes   uint8 [rows, 16 * ceil(cols / 32)], two values a byte, the lower column in the low half
+    scales  uint8 [ceil(rows / 128), ceil(cols / 128), 32, 4, 4]; 2^(byte - 127) of (row r, block b) sits at
+            [r // 128, b // 4, r % 32, r % 128 // 32, b % 4]; entries without a row or block are 0
+    """
+    __slots__ = ("codes", "scales", "rows", "cols")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
+        want_c, want_s = (rows, -(-cols // 32) * 16), (-(-rows // 128), -(-cols // 128), 32, 4, 4)
+        for t, want, name in ((codes, want_c, "codes"), (scales, want_s, "scales")):
+            _require_cuda(t, name)
+            if t.dtype != torch.uint8 or tuple(t.shape) != want:
+                raise RuntimeError(f"{name} of a [{rows}, {cols}] MXFP4 matrix must be torch.uint8 {list(want)}, "
+                                   f"got {t.dtype} {list(t.shape)}")
+            if not t.is_contiguous() or t.data_ptr() % 16:
+                raise RuntimeError(f"{name} must be contiguous and 16-byte aligned")
+        if codes.device != scales.device:
+            raise RuntimeError("codes and scales must be on the same device")
+        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def __repr__(self):
+        return f"MXFP4Tensor([{self.rows}, {self.cols}], device={self.codes.device})"
+
+
+def quantize_mxfp4(x: torch.Tensor, dim: int = 1) -> MXFP4Tensor:
+    """``x`` (2-D; bf16, fp16 or fp32) with blocks along ``dim``.  The result's columns are ``x``'s dimension
+    ``dim``: an ``nn.Linear`` weight [out, in] is quantised along 1, its ``.T`` view or an [in, out] weight along 0."""
+    _require_cuda(x, "x")
+    if x.dim() != 2:
+        raise RuntimeError(f"x must be 2-D, got shape {tuple(x.shape)}")
+    if x.dtype not in _DTYPES:
+        raise RuntimeError(f"x must be torch.bfloat16, torch.float16 or torch.float32, got {x.dtype}")
+    if dim not in (0, 1, -1, -2):
+        raise RuntimeError(f"dim must be 0 or 1, got {dim}")
+    if dim in (0, -2):
+        x = x.T
+    x = x.detach()
+    rows, cols = x.shape
+    if max(rows, cols) >= 1 << 30:
+        raise RuntimeError(f"x is too large: {tuple(x.shape)}")
+    if not (x.stride(1) == 1 or cols == 1 or x.stride(0) == 1 or rows == 1) or min(x.stride()) < 0:
+        x = x.contiguous()
+    dev = x.device
+    with _on(dev):
+        codes = torch.empty((rows, -(-cols // 32) * 16), dtype=torch.uint8, device=dev)
+        scales = torch.empty((-(-rows // 128), -(-cols // 128), 32, 4, 4), dtype=torch.uint8, device=dev)
+        check("ffnk_mxfp4_quantize", lib().ffnk_mxfp4_quantize(
+            x.data_ptr(), _DTYPES[x.dtype], x.stride(0), x.stride(1), rows, cols, codes.data_ptr(), scales.data_ptr(),
+            stream_ptr(dev)))
+    return MXFP4Tensor(codes, scales, rows, cols)
+
+
+def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The matrix [rows, cols] that ``q`` stands for: exact in bf16 and fp32, rounded to nearest in fp16."""
+    if not isinstance(q, MXFP4Tensor):
+        raise RuntimeError(f"q must be an MXFP4Tensor, got {type(q).__name__}")
+    if dtype not in _DTYPES:
+        raise RuntimeError(f"dtype must be torch.bfloat16, torch.float16 or torch.float32, got {dtype}")
+    dev = q.codes.device
+    with _on(dev):
+        out = torch.empty((q.rows, q.cols), dtype=dtype, device=dev)
+        check("ffnk_mxfp4_dequantize", lib().ffnk_mxfp4_dequantize(
+            q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols, out.data_ptr(), _DTYPES[dtype], q.cols, stream_ptr(dev)))
+    return out
+
+
+def _check_weights(ws, names, shapes, dev):
+    for w, n, s in zip(ws, names, shapes):
+        if not isinstance(w, MXFP4Tensor):
+            raise RuntimeError(f"{n} must be an MXFP4Tensor, got {type(w).__name__}")
+        if (w.rows, w.cols) != s:
+            raise RuntimeError(f"{n} must have shape {list(s)} ([out, in]), got [{w.rows}, {w.cols}]")
+        if w.codes.device != dev:
+            raise RuntimeError(f"{n} must be on the same device as the activations")
+
+
+def _check_mask(mask, M, dev):
+    if not isinstance(mask, torch.Tensor) or mask.dim() != 1 or mask.shape[0] != M or mask.device != dev:
+        raise RuntimeError(f"mask must have shape [{M}] on {dev}")
+    if mask.dtype not in (torch.bool, torch.uint8):
+        raise RuntimeError(f"mask must be torch.bool (or uint8), got {mask.dtype}")
+    return mask.contiguous()
+
+
+def _lists(M, dev):
+    """Routing lists of one call: perm int32 [2 * cap], counts int32 [8], in one allocation."""
+    cap = (M + 127) // 128 * 128
+    t = torch.empty(2 * cap + 8, dtype=torch.int32, device=dev)
+    return t, t.data_ptr(), t.data_ptr() + 8 * cap
+
+
+def _mxfp4_linear_forward(a, b1, b2, mask):
+    """y[m] = Q(a[m]) @ (b1 if mask[m] else b2).T -> (y [M, N] bf16, routing lists)."""
+    a = _activation(a, "a")
+    M, K = a.shape
+    dev = a.device
+    N = b1.rows if isinstance(b1, MXFP4Tensor) else -1
+    _check_weights((b1, b2), ("b1", "b2"), ((N, K),) * 2, dev)
+    _check_dims(K=K, N=N)
+    mask = _check_mask(mask, M, dev)
+    L = lib()
+    with _on(dev):
+        y = torch.empty((M, N), device=dev, dtype=torch.bfloat16)
+        if M == 0:
+            return y, None
+        lists, perm, counts = _lists(M, dev)
+        nbytes = L.ffnk_mxfp4_workspace_bytes(M, K, 0)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        check("ffnk_mxfp4_linear_forward", L.ffnk_mxfp4_linear_forward(
+            a.data_ptr(), a.stride(0), b1.codes.data_ptr(), b1.scales.data_ptr(), b2.codes.data_ptr(), b2.scales.data_ptr(),
+            mask.data_ptr(), perm, counts, ws.data_ptr(), nbytes, y.data_ptr(), N, M, N, K, status_word(dev).data_ptr(),
+            stream_ptr(dev)))
+    maybe_check(dev)
+    return y, lists
+
+
+def _mxfp4_linear_backward(g, b1, b2, lists):
+    """dx[m] = g[m] @ (b1 if mask[m] else b2)."""
+    M, (N, K) = g.shape[0], b1.shape
+    g = _activation(g, "grad")
+    dev = g.device
+    L = lib()
+    with _on(dev):
+        dx = torch.empty((M, K), device=dev, dtype=torch.bfloat16)
+        if M == 0:
+            return dx
+        nbytes = L.ffnk_mxfp4_backward_workspace_bytes(M, K, N, 0)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        perm = lists.data_ptr()
+        check("ffnk_mxfp4_linear_backward", L.ffnk_mxfp4_linear_backward(
+            g.data_ptr(), g.stride(0), b1.codes.data_ptr(), b1.scales.data_ptr(), b2.codes.data_ptr(), b2.scales.data_ptr(),
+            perm, perm + 4 * (lists.numel() - 8), ws.data_ptr(), nbytes, dx.data_ptr(), K, M, N, K,
+            status_word(dev).data_ptr(), stream_ptr(dev)))
+    maybe_check(dev)
+    return dx
+
+
+_FFN_NAMES = ("w1", "w2", "w3", "u1", "u2", "u3")
+
+
+def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
+    """The whole FFN forward -> (y [M, d] bf16, what the backward pass needs or None)."""
+    x = _activation(x, "x")
+    M, d = x.shape
+    dev = x.device
+    h = ws6[0].rows if isinstance(ws6[0], MXFP4Tensor) else -1
+    _check_weights(ws6, _FFN_NAMES, ((h, d), (d, h), (h, d)) * 2, dev)
+    _check_dims(d=d, h=h)
+    mask = _check_mask(mask, M, dev)
+    L = lib()
+    with _on(dev):
+        y = torch.empty((M, d), device=dev, dtype=torch.bfloat16)
+        if M == 0:
+            return y, (None, None, None)
+        lists, perm, counts = _lists(M, dev)
+        nbytes = L.ffnk_mxfp4_workspace_bytes(M, d, h)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        t1 = t3 = None
+        if keep:
+            t1, t3 = (torch.empty(((M + 127) // 128 * 128 + 512) * h, device=dev, dtype=torch.float32) for _ in range(2))
+        check("ffnk_mxfp4_ffn_forward", L.ffnk_mxfp4_ffn_forward(
+            x.data_ptr(), x.stride(0), _Six(*[w.codes.data_ptr() for w in ws6]), _Six(*[w.scales.data_ptr() for w in ws6]),
+            mask.data_ptr(), perm, counts, ws.data_ptr(), nbytes, t1.data_ptr() if keep else None,
+            t3.data_ptr() if keep else None, y.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
+    maybe_check(dev)
+    return y, (lists, t1, t3)
+
+
+def _mxfp4_ffn_backward(gy, ws6, saved):
+    """Gradient of the activations."""
+    lists, t1, t3 = saved
+    M, (h, d) = gy.shape[0], ws6[0].shape
+    gy = _activation(gy, "grad")
+    dev = gy.device
+    L = lib()
+    with _on(dev):
+        dx = torch.empty((M, d), device=dev, dtype=torch.bfloat16)
+        if M == 0:
+            return dx
+        nbytes = L.ffnk_mxfp4_backward_workspace_bytes(M, d, d, h)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        perm = lists.data_ptr()
+        check("ffnk_mxfp4_ffn_backward", L.ffnk_mxfp4_ffn_backward(
+            gy.data_ptr(), gy.stride(0), _Six(*[w.codes.data_ptr() for w in ws6]),
+            _Six(*[w.scales.data_ptr() for w in ws6]), t1.data_ptr(), t3.data_ptr(), perm, perm + 4 * (lists.numel() - 8),
+            ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
+    maybe_check(dev)
+    return dx
+
+
+def _wants_grad(a) -> bool:
+    return isinstance(a, torch.Tensor) and a.requires_grad and torch.is_grad_enabled()
+
+
+class MXFP4MaskedLinear(Function):
+    """``MXFP4MaskedLinear.apply(a, b1, b2, mask)``: ``Q(a[m]) @ b1.T`` where ``mask[m]`` else ``Q(a[m]) @ b2.T``.
+
+    a [M, K] bf16; b1 (visual), b2 (text): ``MXFP4Tensor`` [N, K], the ``nn.Linear`` weights quantised.  Gradient
+    of ``a`` only."""
+
+    @classmethod
+    def apply(cls, a, b1, b2, mask):
+        return super().apply(a, b1, b2, mask) if _wants_grad(a) else _mxfp4_linear_forward(a, b1, b2, mask)[0]
+
+    @staticmethod
+    def forward(ctx, a, b1, b2, mask):
+        y, ctx.lists = _mxfp4_linear_forward(a, b1, b2, mask)
+        ctx.weights = (b1, b2)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        return _mxfp4_linear_backward(grad, *ctx.weights, ctx.lists), None, None, None
+
+
+class MXFP4MaskedFFN(Function):
+    """``MXFP4MaskedFFN.apply(a, w1, w2, w3, u1, u2, u3, mask)``: the routed SwiGLU FFN on 4-bit weights.
+
+    y = Q(silu(Q(a) w1.T) * (Q(a) w3.T)) w2.T for visual tokens, u* for text tokens; the weights are ``MXFP4Tensor``
+    in ``nn.Linear`` order (w1, w3, u1, u3 [h, d]; w2, u2 [d, h]).  Gradient of ``a`` only."""
+
+    @classmethod
+    def apply(cls, a, w1, w2, w3, u1, u2, u3, mask):
+        if _wants_grad(a):
+            return super().apply(a, w1, w2, w3, u1, u2, u3, mask)
+        return _mxfp4_ffn_forward(a, (w1, w2, w3, u1, u2, u3), mask, keep=False)[0]
+
+    @staticmethod
+    def forward(ctx, a, w1, w2, w3, u1, u2, u3, mask):
+        ctx.weights = (w1, w2, w3, u1, u2, u3)
+        y, ctx.kept = _mxfp4_ffn_forward(a, ctx.weights, mask, keep=True)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        return (_mxfp4_ffn_backward(grad, ctx.weights, ctx.kept), *([None] * 7))

@@ -312,6 +312,73 @@ int ffnk_ffn_backward(const void* gy, int64_t ldg, const void* xr, const void* t
                       int64_t lddx, void* dw1, void* dw2, void* dw3, void* du1, void* du2, void* du3, int64_t M,
                       int64_t d, int64_t h, int32_t* status, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * MXFP4: 4-bit floating point with one power-of-two scale per 32 values (the OCP microscaling format).
+ * No counterpart in the reference, which is bf16 only.
+ *
+ * A matrix [rows, cols], blocks of 32 along the columns (the contraction):
+ *   codes   uint8 [rows, 16 * ceil(cols / 32)]   two values a byte, the lower column in the low half; a value is
+ *           sign, two exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6; columns past `cols` are 0
+ *   scales  uint8 [ceil(rows / 128)][ceil(cols / 128)][32][4][4]: the scale 2^(byte - 127) of row r, block b is
+ *           [r / 128][b / 4][r % 32][r % 128 / 32][b % 4]; entries of rows and blocks that do not exist are 0
+ * both 16-byte aligned.  For a block with largest magnitude m: E = clamp(floor(log2 m) - 2, -127, 127), every
+ * value is x / 2^E rounded to nearest even and limited to 6; a block holding an infinity or a NaN has the scale
+ * byte 255 and codes 0 (it reads back as NaN).  A weight is stored [out, in], the nn.Linear order.
+ * ------------------------------------------------------------------------------------- */
+#define FFNK_BF16 0
+#define FFNK_FP16 1
+#define FFNK_FP32 2
+int64_t ffnk_mxfp4_code_bytes(int64_t rows, int64_t cols);
+int64_t ffnk_mxfp4_scale_bytes(int64_t rows, int64_t cols);
+
+/* x(r, c) at x[r * row_stride + c * col_stride] (elements of `dtype`; one of the strides is 1) -> codes, scales, every
+ * byte of both written.  Any sizes. */
+int ffnk_mxfp4_quantize(const void* x, int dtype, int64_t row_stride, int64_t col_stride, int64_t rows, int64_t cols,
+                        void* codes, void* scales, void* stream);
+/* The inverse: out [rows, ldo] of `dtype`.  Exact in bf16 and fp32; rounded to nearest in fp16. */
+int ffnk_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype,
+                          int64_t ldo, void* stream);
+
+/* Routed linear layer on MXFP4 weights (compare ffnk_linear_fwd):
+ *     y[m, :] = Q(x[m, :]) @ (mask[m] ? b1 : b2)^T       x [M, K] bf16; b* [N, K] in MXFP4; y [M, N] bf16
+ * Q quantises the token's row to MXFP4 inside the call; products are exact, sums fp32.  The call routes the mask
+ * itself: perm int32 [2 * cap] and counts int32 [8] are outputs, as from ffnk_route.  workspace:
+ * ffnk_mxfp4_workspace_bytes(M, K, 0) bytes, 256-byte aligned, free again when the stream has passed the call. */
+int64_t ffnk_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t h);
+int ffnk_mxfp4_linear_forward(const void* x, int64_t ldx, const void* b1_codes, const void* b1_scales,
+                              const void* b2_codes, const void* b2_scales, const void* mask, int32_t* perm, int32_t* counts,
+                              void* workspace, int64_t workspace_bytes, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                              int32_t* status, void* stream);
+
+/* Routed SwiGLU FFN on MXFP4 weights (compare ffnk_ffn_forward):
+ *     y = Q(silu(Q(x) w1^T) * (Q(x) w3^T)) w2^T for visual tokens, u1, u3, u2 for text tokens
+ * codes, scales: HOST arrays of six device pointers each, in the order w1, w2, w3, u1, u2, u3; w1, w3, u1, u3 are
+ * [h, d], w2, u2 [d, h].  The hidden activation is quantised from fp32.  t1, t3: both null, or fp32 of
+ * (cap + 512) * h elements each, where the pre-activations are kept for the backward pass, in an order of the
+ * library's own.  workspace: ffnk_mxfp4_workspace_bytes(M, d, h). */
+int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* const* codes, const void* const* scales,
+                           const void* mask, int32_t* perm, int32_t* counts, void* workspace, int64_t workspace_bytes,
+                           void* t1, void* t3, void* y, int64_t ldy, int64_t M, int64_t d, int64_t h, int32_t* status,
+                           void* stream);
+
+/* Gradients of the activations of the two forward passes above, the weights being frozen and the rounding of
+ * activations to 4 bits counting as the identity:
+ *     linear: dx[m, :] = g[m, :] @ (mask[m] ? b1 : b2)
+ *     ffn:    dh = gy w2, dt1 = dh * t3 * s * (1 + t1 * (1 - s)), dt3 = dh * t1 * s, s = sigmoid(t1),
+ *             dx = dt1 w1 + dt3 w3      (per modality)
+ * perm, counts (and t1, t3) as the forward call left them.  The weights of the modalities present are read back
+ * to bf16, exactly, in the workspace; the products are bf16 with fp32 sums.  workspace:
+ * ffnk_mxfp4_backward_workspace_bytes(M, K, N, 0) for the linear layer, (M, d, d, h) for the FFN, 256-byte aligned. */
+int64_t ffnk_mxfp4_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t h);
+int ffnk_mxfp4_linear_backward(const void* g, int64_t ldg, const void* b1_codes, const void* b1_scales,
+                               const void* b2_codes, const void* b2_scales, const int32_t* perm, const int32_t* counts,
+                               void* workspace, int64_t workspace_bytes, void* dx, int64_t lddx, int64_t M, int64_t N,
+                               int64_t K, int32_t* status, void* stream);
+int ffnk_mxfp4_ffn_backward(const void* gy, int64_t ldg, const void* const* codes, const void* const* scales,
+                            const void* t1, const void* t3, const int32_t* perm, const int32_t* counts, void* workspace,
+                            int64_t workspace_bytes, void* dx, int64_t lddx, int64_t M, int64_t d, int64_t h,
+                            int32_t* status, void* stream);
+
 /* Synchronises `stream`, copies the status word to the host and returns it (0 = ok, >0 one of
  * the device status codes, <0 an error as above).  If `clear` is non-zero the word is reset to 0. */
 int ffnk_read_status(int32_t* status, int clear, void* stream);

@@ -1,0 +1,360 @@
+"""MXFP4 quantisation and the routed operators on 4-bit weights against the 64-bit oracle.
+
+Quantisation is compared bit for bit.  Products are compared element by element with bounds that the oracle derives
+from the roundings on the way (``oracle/mxfp4_ref.py``)."""
+import pytest
+import torch
+
+from ffn_kernel_b200 import (GraphedMaskedFFN, MaskedFFNModule, MaskedLinearModule, MXFP4MaskedFFN, MXFP4MaskedFFNModule,
+                             MXFP4MaskedLinear, MXFP4MaskedLinearModule, MXFP4Tensor, check_status, dequantize_mxfp4,
+                             quantize_mxfp4)
+from ffn_kernel_b200.synth import edge_mask
+from oracle import mxfp4_ref as R
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def spread(rows, cols, seed, dtype=torch.bfloat16):
+    """Magnitudes that differ by row and column."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp2(torch.randn(rows, 1, generator=g))
+    return (x * torch.exp2(2 * torch.randn(1, cols, generator=g))).to(dtype)
+
+
+def poison(dev):
+    """Freed blocks full of NaN, for the allocator to hand out again as outputs and workspaces."""
+    junk = [torch.full((n,), float("nan"), device=dev) for n in (1 << 10, 1 << 14, 1 << 18, 1 << 22)]
+    del junk
+
+
+def same_matrix(q: MXFP4Tensor, x: torch.Tensor):
+    codes, scales = R.quantize(x.cpu().double())
+    assert torch.equal(q.codes.cpu(), codes)
+    assert torch.equal(q.scales.cpu(), scales)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 8), (3, 31), (37, 200), (64, 32), (130, 72), (129, 257), (5, 2049)])
+def test_quantize_bit_for_bit(dev, name, rows, cols):
+    x = spread(rows, cols, rows * 1000 + cols, DTYPES[name])
+    poison(dev)
+    same_matrix(quantize_mxfp4(x.to(dev)), x)
+    poison(dev)
+    same_matrix(quantize_mxfp4(x.T.contiguous().to(dev), dim=0), x)      # blocks along the strided dimension
+    same_matrix(quantize_mxfp4(x.to(dev).T, dim=0), x)                   # the nn.Linear weight seen as [in, out]
+
+
+def test_quantize_strided_and_offset_views(dev):
+    base = spread(70, 300, 1).to(dev)
+    for v in (base[:, 3:203], base[::2, :128], base[1:, 1:], base[:, ::3], base[5:6], base[:, 7:8]):
+        same_matrix(quantize_mxfp4(v), v)
+        same_matrix(quantize_mxfp4(v, dim=0), v.T)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_quantize_every_tie_and_special_value(dev, name):
+    dt = DTYPES[name]
+    ties = torch.tensor([6, .25, .75, 1.25, 1.75, 2.5, 3.5, 5, -.25, -.75, -1.25, -1.75, -2.5, -3.5, -5, 7.5, 7, -7.5, 0, -0.0])
+    x = torch.zeros(12, 64)
+    x[0, :20], x[1, 32:52], x[2, :20] = ties, ties * 2 ** -10, ties * 2 ** 8
+    x[3, 5], x[4, 5], x[5, 5] = float("inf"), float("-inf"), float("nan")
+    x[3, 6] = x[4, 40] = 3.0
+    x[6, :4] = torch.tensor([torch.finfo(dt).max, -torch.finfo(dt).max, 1.0, torch.finfo(dt).tiny])
+    x[7, :4] = torch.tensor([torch.finfo(dt).smallest_normal, -torch.finfo(dt).smallest_normal / 2, 0.0, 0.0])
+    x = x.to(dt)
+    x[8, 0] = torch.finfo(dt).smallest_normal * torch.finfo(dt).eps      # the smallest subnormal alone
+    x[9, 33] = -torch.finfo(dt).smallest_normal
+    q = quantize_mxfp4(x.to(dev))
+    same_matrix(q, x)
+    back = dequantize_mxfp4(q, torch.float32).cpu().double()
+    want = R.values(q.codes, q.scales, 12, 64)
+    assert torch.equal(torch.isnan(back), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(back), torch.nan_to_num(want))
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 31), (130, 72), (257, 300), (9, 1031)])
+def test_dequantize_any_codes_and_scales(dev, rows, cols):
+    g = torch.Generator().manual_seed(rows)
+    q = MXFP4Tensor(torch.randint(0, 256, (rows, -(-cols // 32) * 16), generator=g, dtype=torch.uint8).to(dev),
+                    torch.randint(0, 256, (-(-rows // 128), -(-cols // 128), 32, 4, 4), generator=g, dtype=torch.uint8).to(dev),
+                    rows, cols)
+    want = R.values(q.codes, q.scales, rows, cols)
+    for dt in (torch.float32, torch.bfloat16, torch.float16):
+        got = dequantize_mxfp4(q, dt).cpu()
+        # 6 * 2^127 is beyond bf16 and fp32: infinity, as the rounding of the value gives
+        ref = want.to(torch.float32).to(dt)
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        assert torch.equal(torch.nan_to_num(got.float()), torch.nan_to_num(ref.float()))
+
+
+def test_empty_matrices(dev):
+    for shape in ((0, 64), (5, 0)):
+        q = quantize_mxfp4(torch.empty(shape, dtype=torch.bfloat16, device=dev))
+        assert q.shape == shape and tuple(dequantize_mxfp4(q).shape) == shape
+
+
+# ------------------------------------------------------------------------------------------------ products
+def weights(shapes, seed, dev):
+    qs = [quantize_mxfp4((spread(r, c, seed + i) * (0.5 * c ** -0.5)).to(dev)) for i, (r, c) in enumerate(shapes)]
+    return qs, [R.values(q.codes, q.scales, q.rows, q.cols) for q in qs]
+
+
+def inside(got, want_and_bound):
+    want, bound = want_and_bound
+    off = (got.cpu().double() - want).abs()
+    assert torch.isfinite(got).all()
+    assert (off <= bound).all(), f"worst: {(off / bound).max().item():.3f} of the bound"
+
+
+MASKS = ["all_visual", "all_text", "alternating", "bernoulli", "span"]
+LINEAR_SIZES = [(1, 64, 64), (1, 4096, 264), (2, 8, 8), (7, 40, 136), (33, 1000, 72), (127, 264, 520), (128, 256, 256),
+                (129, 128, 1032), (300, 2056, 328), (515, 96, 2048), (1030, 520, 264), (8200, 72, 64)]
+
+
+@pytest.mark.parametrize("M,K,N", LINEAR_SIZES)
+@pytest.mark.parametrize("kind", MASKS)
+def test_linear_forward_and_gradient(dev, M, K, N, kind):
+    x, mask, g = spread(M, K, M + K), edge_mask(M, kind, seed=M), spread(M, N, M + N + 1)
+    (b1, b2), (v1, v2) = weights([(N, K)] * 2, K, dev)
+    poison(dev)
+    with torch.no_grad():
+        y0 = MXFP4MaskedLinear.apply(x.to(dev), b1, b2, mask.to(dev))
+    xg = x.to(dev).requires_grad_(True)
+    y = MXFP4MaskedLinear.apply(xg, b1, b2, mask.to(dev))
+    poison(dev)
+    y.backward(g.to(dev))
+    check_status()
+    assert torch.equal(y0, y.detach())
+    inside(y.detach(), R.linear(x, v1, v2, mask))
+    inside(xg.grad, R.linear_dx(g, v1, v2, mask))
+
+
+FFN_SIZES = [(1, 64, 64), (1, 1024, 1416), (2, 8, 8), (7, 40, 136), (33, 1000, 72), (127, 264, 520), (128, 256, 256),
+             (130, 128, 1032), (300, 512, 328), (515, 96, 1000), (1030, 264, 136), (8200, 64, 72)]
+
+
+def ffn_weights(d, h, seed, dev):
+    return weights([(h, d), (d, h), (h, d)] * 2, seed, dev)
+
+
+@pytest.mark.parametrize("M,d,h", FFN_SIZES)
+@pytest.mark.parametrize("kind", MASKS)
+def test_ffn_forward_and_gradient(dev, M, d, h, kind):
+    x, mask, g = spread(M, d, M + d), edge_mask(M, kind, seed=M), spread(M, d, M + h)
+    qs, vs = ffn_weights(d, h, d + h, dev)
+    poison(dev)
+    with torch.no_grad():
+        y0 = MXFP4MaskedFFN.apply(x.to(dev), *qs, mask.to(dev))
+    xg = x.to(dev).requires_grad_(True)
+    y = MXFP4MaskedFFN.apply(xg, *qs, mask.to(dev))
+    poison(dev)
+    y.backward(g.to(dev))
+    check_status()
+    assert torch.equal(y0, y.detach())
+    inside(y.detach(), R.ffn(x, vs, mask))
+    inside(xg.grad, R.ffn_dx(g, x, vs, mask))
+
+
+def test_linear_gradient_is_a_difference_of_outputs(dev):
+    # activations that the format holds exactly, moved to others that it holds exactly: y moves by d @ W^T
+    M, K, N = 40, 96, 128
+    g = torch.Generator().manual_seed(5)
+    grid = torch.tensor([1.0, 1.5, 2.0, 3.0, 4.0])
+    x, x2 = (grid[torch.randint(0, 5, (M, K), generator=g)].to(torch.bfloat16) for _ in range(2))
+    x[:, ::32] = x2[:, ::32] = 4.0                  # every block's largest value, so that its exponent is 0
+    mask = edge_mask(M, "bernoulli", 3).to(dev)
+    (b1, b2), _ = weights([(N, K)] * 2, 9, dev)
+    up = spread(M, N, 2).to(dev)
+    xg = x.to(dev).requires_grad_(True)
+    y = MXFP4MaskedLinear.apply(xg, b1, b2, mask)
+    y.backward(up)
+    y2 = MXFP4MaskedLinear.apply(x2.to(dev), b1, b2, mask)
+    moved = ((y2.double() - y.detach().double()) * up.double()).sum()
+    told = (xg.grad.double() * (x2 - x).double().to(dev)).sum()
+    # y, y2 and dx are each rounded to bf16 once (half a step, 2^-8 relative)
+    bound = R.U16 * (((y.detach().abs() + y2.abs()).double() * up.abs().double()).sum()
+                     + (xg.grad.abs().double() * (x2 - x).abs().double().to(dev)).sum()) * 1.01
+    assert (moved - told).abs() <= bound
+
+
+def test_ffn_gradient_is_a_difference_of_the_formula(dev):
+    # the layer without its roundings to 4 bits, at the activations that the 4 bits hold
+    M, d, h = 24, 64, 96
+    x, mask, g = spread(M, d, 3), edge_mask(M, "bernoulli", 1), spread(M, d, 4)
+    qs, vs = ffn_weights(d, h, 7, dev)
+    xg = x.to(dev).requires_grad_(True)
+    MXFP4MaskedFFN.apply(xg, *qs, mask.to(dev)).backward(g.to(dev))
+    w1, w2, w3, u1, u2, u3 = vs
+
+    def value(a):
+        t1, t3 = R.by_rows(a, mask, w1.T, u1.T), R.by_rows(a, mask, w3.T, u3.T)
+        return (R.by_rows(t1 * torch.sigmoid(t1) * t3, mask, w2.T, u2.T) * g.double()).sum()
+
+    q, bound = R.rounded(x.double()), R.ffn_dx(g, x, vs, mask)[1]
+    for i in range(6):
+        way = torch.randn(M, d, generator=torch.Generator().manual_seed(i), dtype=torch.float64)
+        eps = 1e-5
+        diff = (value(q + eps * way) - value(q - eps * way)) / (2 * eps)
+        told = (xg.grad.cpu().double() * way).sum()
+        # central difference: its own error is of the order eps^2 times third derivatives, far below 1e-4 relative here
+        assert (diff - told).abs() <= (bound * way.abs()).sum() + 1e-4 * diff.abs()
+
+
+def test_rows_do_not_depend_on_one_another(dev):
+    M, d, h = 700, 136, 264
+    x, mask = spread(M, d, 1).to(dev), edge_mask(M, "span", 2).to(dev)
+    qs, _ = ffn_weights(d, h, 3, dev)
+    y = MXFP4MaskedFFN.apply(x, *qs, mask)
+    for n in (1, 5, 130):
+        assert torch.equal(MXFP4MaskedFFN.apply(x[:n], *qs, mask[:n]), y[:n])
+    bad = x.clone()
+    bad[::7] = float("nan")
+    y2 = MXFP4MaskedFFN.apply(bad, *qs, mask)
+    keep = torch.ones(M, dtype=torch.bool, device=dev)
+    keep[::7] = False
+    assert torch.equal(y2[keep], y[keep]) and torch.isnan(y2[::7]).all()
+
+
+def test_infinite_activations_and_weights_give_nan_where_they_are_used(dev):
+    M, K, N = 9, 96, 136
+    x, mask = spread(M, K, 1), edge_mask(M, "alternating")
+    x[4, 33] = float("inf")
+    w = [spread(N, K, i) for i in (2, 3)]
+    w[0][17, 5] = float("-inf")                # a visual weight row
+    y = MXFP4MaskedLinear.apply(x.to(dev), *[quantize_mxfp4(t.to(dev)) for t in w], mask.to(dev)).cpu()
+    want = torch.zeros(M, N, dtype=torch.bool)
+    want[4] = True
+    want[mask, 17] = True
+    assert torch.equal(torch.isnan(y), want)
+
+
+def test_strided_activations_gradients_and_uint8_mask(dev):
+    M, K, N = 200, 72, 136
+    wide = spread(M, K + 40, 1).to(dev)
+    mask = edge_mask(M, "bernoulli", 1).to(dev)
+    (b1, b2), _ = weights([(N, K)] * 2, 2, dev)
+    want = MXFP4MaskedLinear.apply(wide[:, 8:8 + K].contiguous(), b1, b2, mask)
+    for v in (wide[:, 8:8 + K], wide[:, 8:8 + K].T.contiguous().T):
+        assert torch.equal(MXFP4MaskedLinear.apply(v, b1, b2, mask.to(torch.uint8) * 3), want)
+    xg = wide[:, 8:8 + K].clone().requires_grad_(True)
+    y = MXFP4MaskedLinear.apply(xg, b1, b2, mask)
+    g = spread(M, N, 5).to(dev)
+    a = torch.autograd.grad(y, xg, g, retain_graph=True)[0]
+    b = torch.autograd.grad(y, xg, torch.cat([g, g], 1)[:, :N], retain_graph=True)[0]      # strided upstream gradient
+    c = torch.autograd.grad(y.sum(), xg)[0]                                                # an expanded one
+    assert torch.equal(a, b) and torch.isfinite(c).all()
+
+
+def test_no_tokens(dev):
+    mask = torch.zeros(0, dtype=torch.bool, device=dev)
+    (b1, b2), _ = weights([(64, 32)] * 2, 1, dev)
+    qs, _ = ffn_weights(32, 64, 1, dev)
+    x = torch.empty(0, 32, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    y, z = MXFP4MaskedLinear.apply(x, b1, b2, mask), MXFP4MaskedFFN.apply(x, *qs, mask)
+    assert tuple(y.shape) == (0, 64) and tuple(z.shape) == (0, 32)
+    (y.sum() + z.sum()).backward()
+    assert tuple(x.grad.shape) == (0, 32)
+
+
+def test_refusals(dev):
+    M, K, N = 16, 64, 96
+    x, mask = spread(M, K, 1).to(dev), edge_mask(M, "alternating").to(dev)
+    (b1, b2), _ = weights([(N, K)] * 2, 1, dev)
+    qs, _ = ffn_weights(K, N, 1, dev)
+    lin, ffn = MXFP4MaskedLinear.apply, MXFP4MaskedFFN.apply
+    refused = [
+        lambda: lin(x.float(), b1, b2, mask), lambda: lin(x[0], b1, b2, mask), lambda: lin(x, b1, b2, mask[1:]),
+        lambda: lin(x, b1, b2, mask.float()), lambda: lin(x, b1, b2, mask.cpu()), lambda: lin(x, b1, b1.codes, mask),
+        lambda: lin(x[:, :56], b1, b2, mask), lambda: lin(x, b1, qs[1], mask), lambda: ffn(x, *qs[:5], b1, mask[:4]),
+        lambda: ffn(x, qs[1], *qs[1:], mask), lambda: ffn(x, *qs[:5], x, mask),
+        lambda: quantize_mxfp4(x.double()), lambda: quantize_mxfp4(x[0]), lambda: quantize_mxfp4(x, dim=2),
+        lambda: dequantize_mxfp4(b1, torch.float64), lambda: dequantize_mxfp4(b1.codes),
+        lambda: MXFP4Tensor(b1.codes, b1.scales, N, K + 64), lambda: MXFP4Tensor(b1.codes.int(), b1.scales, N, K),
+        lambda: MXFP4Tensor(b1.codes, b1.scales.permute(0, 1, 3, 2, 4).permute(0, 1, 3, 2, 4)[:, :, :, :, :2], N, K),
+        lambda: MXFP4Tensor(b1.codes.cpu(), b1.scales, N, K),
+        lambda: MXFP4Tensor(torch.cat([b1.codes] * 2, 1)[:, :32], b1.scales, N, K),
+    ]
+    for call in refused:
+        with pytest.raises((RuntimeError, TypeError)):
+            call()
+    q36 = quantize_mxfp4(spread(96, 36, 1).to(dev))           # the format holds 36 columns, the product does not
+    with pytest.raises(RuntimeError):
+        lin(spread(M, 36, 1).to(dev), q36, q36, mask)
+    check_status()
+
+
+# ------------------------------------------------------------------------------------------------ as they are used together
+def test_modules_and_graph_replay(dev):
+    torch.manual_seed(3)
+    d, h, T = 136, 264, 50
+    ffn, lin = MaskedFFNModule(d, h, device=dev), MaskedLinearModule(d, d, device=dev)
+    f4, l4 = MXFP4MaskedFFNModule.from_module(ffn), MXFP4MaskedLinearModule.from_module(lin)
+    x = torch.randn(2, T // 2, d, device=dev, dtype=torch.bfloat16)
+    mask = torch.rand(2, T // 2, device=dev) < 0.5
+    xg = x.clone().requires_grad_(True)
+    y = f4(l4(xg, mask), mask)                                # the two layers one after the other, trained through
+    y.sum().backward()
+    assert y.shape == x.shape and xg.grad.shape == x.shape and torch.isfinite(xg.grad).all()
+    # what the layers hold is what the operators compute on
+    mid = MXFP4MaskedLinear.apply(x.view(-1, d), quantize_mxfp4(lin.linear_v.weight), quantize_mxfp4(lin.linear_t.weight.T, dim=0),
+                                  mask.view(-1))
+    want = MXFP4MaskedFFN.apply(mid, *[quantize_mxfp4(getattr(ffn, n).weight) for n in f4.NAMES], mask.view(-1))
+    assert torch.equal(want.view_as(x), y.detach())
+    again = MXFP4MaskedFFNModule(d, h, device=dev)
+    again.load_state_dict(f4.state_dict())
+    graphed = GraphedMaskedFFN(again, T)
+    for seed in range(3):
+        xi = spread(T, d, seed).to(dev)
+        mi = edge_mask(T, MASKS[seed], seed).to(dev)
+        assert torch.equal(graphed(xi, mi), f4(xi, mi))
+    check_status()
+
+
+def test_two_streams_at_once_and_captured_training(dev):
+    M, d, h = 600, 128, 264
+    qs, _ = ffn_weights(d, h, 1, dev)
+    (b1, b2), _ = weights([(d, d)] * 2, 2, dev)
+    xs = [spread(M, d, s).to(dev) for s in range(4)]
+    mask = edge_mask(M, "span", 1).to(dev)
+
+    def step(x):
+        x = x.detach().requires_grad_(True)
+        y = MXFP4MaskedFFN.apply(MXFP4MaskedLinear.apply(x, b1, b2, mask), *qs, mask)
+        return y.detach(), torch.autograd.grad(y, x, x.detach())[0]
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device=dev) for _ in range(2)]
+    got = [None] * 4
+    for rep in range(3):
+        for i, x in enumerate(xs):
+            with torch.cuda.stream(streams[i % 2]):
+                got[i] = step(x)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    static = xs[0].clone()
+    streams[0].wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(streams[0]):
+        step(static)
+    torch.cuda.current_stream(dev).wait_stream(streams[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for i in (2, 1):
+        static.copy_(xs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[i][0]) and torch.equal(out[1], want[i][1])
+    check_status()
+
+
+def test_repeated_calls_give_the_same_bits(dev):
+    M, d, h = 3000, 264, 520
+    x, mask = spread(M, d, 1).to(dev), edge_mask(M, "span", 1).to(dev)
+    qs, _ = ffn_weights(d, h, 2, dev)
+    y = MXFP4MaskedFFN.apply(x, *qs, mask)
+    for _ in range(5):
+        assert torch.equal(MXFP4MaskedFFN.apply(x, *qs, mask), y)
