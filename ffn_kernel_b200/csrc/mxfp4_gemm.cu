@@ -63,7 +63,6 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t tmem, uint32_t smem) {
 // ---------------------------------------------------------------------------------------------
 constexpr int MX_BM = 128;                    // rows of a CTA's tile
 constexpr int MX_BN = 256;                    // accumulator columns (gate/up tiles: 128 gate | 128 up)
-constexpr int MX_BK = 256;                    // values of a k-step: 128 bytes, one swizzle row; two scale atoms
 constexpr int MX_A_BYTES = MX_BM * 128;       // 16 KiB of codes
 constexpr int MX_SF_BYTES = 2 * kMxAtomBytes; // scales of 128 rows x one k-step
 constexpr int MX_THREADS = 320;               // producer, MMA, eight epilogue warps
@@ -90,7 +89,7 @@ struct MxParams {
   uint8_t* scales;
   int64_t code_ld;
   int k_atoms_out;
-  int pdl;
+  long long* prof;         // optional per-CTA wait-cycle counters (ffnk_debug_profile_buffer)
 };
 
 struct MxMaps {
@@ -174,6 +173,20 @@ __device__ __forceinline__ uint32_t mx_quantize_block(const float (&v)[32], uint
   }
   codes = make_uint4(w[0], w[1], w[2], w[3]);
   return byte;
+}
+
+// One lane of a converged warp.  The producer and MMA warps run their loops with all lanes and let this one issue: the
+// operands of TMA and tcgen05 instructions live in uniform registers, and in a branch that the compiler takes for
+// divergent each of them is moved there one by one (about 20 cycles a register: an MMA cost 183 cycles to issue
+// whatever its N, a scale copy 60).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// the same bounded wait for all lanes of a warp
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag));
 }
 
 __device__ __forceinline__ void mx_report(int* status, int code) {
@@ -273,37 +286,49 @@ __device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, c
 }
 
 // ---------------------------------------------------------------------------------------------
-// One CTA per tile of 128 rows x 256 accumulator columns, persistent, warp specialised: warp 0 producer (TMA),
-// warp 1 scale copies and MMAs, warps 2..9 epilogue.
+// CTAS = 1: one CTA per tile of 128 rows x 256 accumulator columns.  CTAS = 2: a cluster of two CTAs (one TPC) shares
+// tcgen05.mma.cta_group::2 of 256 rows x 256 columns: each CTA fetches its own 128 rows of A and half of the weight
+// rows (gate/up: the leader the gate rows, the partner the up rows), 35 KiB a k-step instead of 51; the scales of all
+// 256 weight rows are needed in both.  The leader (rank 0) issues everything; its `full` barriers count both CTAs'
+// bytes, its commits free the stage and publish the accumulator in both, both epilogues report to its `tempty`.
+// Persistent, warp specialised: warp 0 producer (TMA), warp 1 scale copies and MMAs, warps 2..9 epilogue.
 // ---------------------------------------------------------------------------------------------
-constexpr int MX_B_BYTES = MX_BN * 128;
-constexpr int MX_STAGE_BYTES = MX_A_BYTES + MX_B_BYTES + 3 * MX_SF_BYTES;   // 51 KiB
-constexpr int MX_STAGES = 4;
-constexpr int MX_SMEM = MX_STAGES * MX_STAGE_BYTES + MX_STAGING + 256 + 1024;
+template <int CTAS> struct MxGeom {
+  static constexpr int b_bytes = MX_BN / CTAS * 128;
+  static constexpr int stage_bytes = MX_A_BYTES + b_bytes + 3 * MX_SF_BYTES;
+  static constexpr int stages = CTAS == 2 ? 5 : 4;
+  static constexpr int smem = stages * stage_bytes + MX_STAGING + 256 + 1024;
+};
 
-template <int EPI>
+template <int CTAS>
+__device__ __forceinline__ void mx_load(void* dst, const CUtensorMap* m, uint64_t* bar, uint32_t lead_bar, int x, int y) {
+  if constexpr (CTAS == 1) tma_load_2d(dst, m, bar, x, y);
+  else tma_load_2d_pair(dst, m, lead_bar, x, y);
+}
+
+template <int EPI, int CTAS>
 __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
+  using G = MxGeom<CTAS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* staging = smem + MX_STAGES * MX_STAGE_BYTES;
+  uint8_t* staging = smem + G::stages * G::stage_bytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(staging + MX_STAGING);
-  uint64_t* empty = full + MX_STAGES;
-  uint64_t* tfull = empty + MX_STAGES;     // accumulator ready for the epilogue [2]
+  uint64_t* empty = full + G::stages;
+  uint64_t* tfull = empty + G::stages;     // accumulator ready for the epilogue [2]
   uint64_t* tempty = tfull + 2;            // the epilogue has read the first chunk of a tile
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);   // warp-uniform for the compiler too
   const int lane = threadIdx.x & 31;
+  const int rank = CTAS == 2 ? static_cast<int>(cluster_ctarank()) : 0;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < MX_STAGES; ++s) {
-      mbar_init(&full[s], 1);
+    for (int s = 0; s < G::stages; ++s) {
+      mbar_init(&full[s], CTAS);           // one arrive.expect_tx per CTA
       mbar_init(&empty[s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&tfull[i], 1);
-    }
-    mbar_init(tempty, 8);
+    for (int i = 0; i < 2; ++i) mbar_init(&tfull[i], 1);
+    mbar_init(tempty, 8 * CTAS);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&maps.a);
@@ -314,120 +339,156 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
     }
   }
   if (warp == 1) {
-    tmem_alloc<1>(tmem_slot, 512);
-    tmem_relinquish<1>();
+    tmem_alloc<CTAS>(tmem_slot, 512);
+    tmem_relinquish<CTAS>();
   }
   griddep_launch_dependents();
   tc_fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync_all();   // both CTAs' barriers exist before anybody signals across
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   griddep_wait();
 
   const int Mv = p.counts[0], Mt = p.counts[1], cap = p.counts[2];
-  const int tiles_v = (Mv + MX_BM - 1) / MX_BM;
-  const int m_tiles = tiles_v + (Mt + MX_BM - 1) / MX_BM;
+  constexpr int TILE_M = MX_BM * CTAS;
+  const int tiles_v = (Mv + TILE_M - 1) / TILE_M;
+  const int m_tiles = tiles_v + (Mt + TILE_M - 1) / TILE_M;
   constexpr int N_PER_TILE = mx_glu(EPI) ? MX_BN / 2 : MX_BN;
   const int n_tiles = (p.n_out + N_PER_TILE - 1) / N_PER_TILE;
   const int total = m_tiles * n_tiles;
   const int k_steps = (p.k_bytes + 127) / 128;
+  const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0, issued = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      const uint32_t bytes = p.a_rows * 128 + MX_B_BYTES + MX_SF_BYTES + 2 * MX_SF_BYTES;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        const MxTile tc = mx_tile(t, MX_BM, 0, tiles_v, m_tiles, n_tiles, p.group_m, Mv, Mt, cap);
-        const CUtensorMap* b0 = &maps.b[tc.text ? 2 : 0];
-        const CUtensorMap* sb0 = &maps.sb[tc.text ? 2 : 0];
-        for (int ks = 0; ks < k_steps; ++ks) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag)) {
-            mx_report(p.status, ST_TIMEOUT_PRODUCER);
-            ok = false;
-            break;
-          }
-          uint8_t* a = smem + stage * MX_STAGE_BYTES;
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const bool lead = elect_one();
+    const uint32_t bytes = p.a_rows * 128 + G::b_bytes + 3 * MX_SF_BYTES;
+    for (int t = first; t < total && ok; t += step) {
+      const MxTile tc = mx_tile(t, TILE_M, rank * MX_BM, tiles_v, m_tiles, n_tiles, p.group_m, Mv, Mt, cap);
+      const CUtensorMap* b0 = &maps.b[tc.text ? 2 : 0];
+      const CUtensorMap* sb0 = &maps.sb[tc.text ? 2 : 0];
+      const int n0 = tc.nt * N_PER_TILE;
+      for (int ks = 0; ks < k_steps; ++ks) {
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag)) {
+          if (lead) mx_report(p.status, ST_TIMEOUT_PRODUCER);
+          ok = false;
+          break;
+        }
+        if (lead) {
+          uint8_t* a = smem + stage * G::stage_bytes;
           uint8_t* b = a + MX_A_BYTES;
-          uint8_t* sa = b + MX_B_BYTES;
+          uint8_t* sa = b + G::b_bytes;
           uint8_t* sb = sa + MX_SF_BYTES;
-          mbar_arrive_expect_tx(&full[stage], bytes);
-          if constexpr (mx_glu(EPI)) {
-            const int n0 = tc.nt * N_PER_TILE;
-            tma_load_2d(b, b0, &full[stage], ks * 128, n0);
-            tma_load_2d(b + MX_B_BYTES / 2, b0 + 1, &full[stage], ks * 128, n0);
-            tma_load_2d(sb, sb0, &full[stage], ks * 256, n0 / 128);
-            tma_load_2d(sb + MX_SF_BYTES, sb0 + 1, &full[stage], ks * 256, n0 / 128);
+          uint64_t* bar = &full[stage];
+          uint32_t lead_bar = 0;
+          if constexpr (CTAS == 2) {
+            lead_bar = mapa_shared(smem_u32(bar), 0);
+            mbar_arrive_expect_tx_cluster(lead_bar, bytes);
           } else {
-            tma_load_2d(b, b0, &full[stage], ks * 128, tc.nt * MX_BN);
-            tma_load_2d(sb, sb0, &full[stage], ks * 256, tc.nt * (MX_BN / 128));
+            mbar_arrive_expect_tx(bar, bytes);
           }
-          tma_load_2d(a, &maps.a, &full[stage], ks * 128, static_cast<int>(tc.routed0));
-          tma_load_2d(sa, &maps.sa, &full[stage], ks * 256, static_cast<int>(tc.routed0 >> 7));
-          ++issued;
-          if (++stage == MX_STAGES) { stage = 0; phase ^= 1; }
+          if constexpr (CTAS == 2) {
+            if constexpr (mx_glu(EPI)) mx_load<CTAS>(b, b0 + rank, bar, lead_bar, ks * 128, n0);
+            else mx_load<CTAS>(b, b0, bar, lead_bar, ks * 128, n0 + rank * (MX_BN / 2));
+          } else {
+            mx_load<CTAS>(b, b0, bar, lead_bar, ks * 128, n0);
+            if constexpr (mx_glu(EPI)) mx_load<CTAS>(b + G::b_bytes / 2, b0 + 1, bar, lead_bar, ks * 128, n0);
+          }
+          mx_load<CTAS>(sb, sb0, bar, lead_bar, ks * 256, n0 / 128);
+          if constexpr (mx_glu(EPI)) mx_load<CTAS>(sb + MX_SF_BYTES, sb0 + 1, bar, lead_bar, ks * 256, n0 / 128);
+          mx_load<CTAS>(a, &maps.a, bar, lead_bar, ks * 128, static_cast<int>(tc.routed0));
+          mx_load<CTAS>(sa, &maps.sa, bar, lead_bar, ks * 256, static_cast<int>(tc.routed0 >> 7));
         }
+        __syncwarp();
+        ++issued;
+        if (++stage == G::stages) { stage = 0; phase ^= 1; }
       }
-      if (*abort_flag) {
-        // let the copies already issued land before the CTA gives its shared memory back
-        for (int i = 0; i < (issued < MX_STAGES ? issued : MX_STAGES); ++i) {
-          if (--stage < 0) { stage = MX_STAGES - 1; phase ^= 1; }
-          int dummy = 0;
-          mbar_wait(&full[stage], phase, &dummy, 1000000ull);
-        }
+    }
+    if (CTAS == 1 && *abort_flag && lead) {
+      // let the copies already issued land before the CTA gives its shared memory back
+      for (int i = 0; i < (issued < G::stages ? issued : G::stages); ++i) {
+        if (--stage < 0) { stage = G::stages - 1; phase ^= 1; }
+        int dummy = 0;
+        mbar_wait(&full[stage], phase, &dummy, 1000000ull);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (rank == 0) {
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++it) {
+      const bool lead = elect_one();
+      const long long t_begin = clock64();
+      long long t_full = 0, t_tmem = 0;
+      for (int t = first; t < total && ok; t += step, ++it) {
         const int acc = it & 1;
-        const bool free = it == 0 || mbar_wait(tempty, (it - 1) & 1, abort_flag);
-        if (!free) {
-          mx_report(p.status, ST_TIMEOUT_MMA_TMEM);
+        long long tw = clock64();
+        if (it != 0 && !mbar_wait_warp(tempty, (it - 1) & 1, abort_flag)) {
+          if (lead) mx_report(p.status, ST_TIMEOUT_MMA_TMEM);
           break;
         }
+        t_tmem += clock64() - tw;
         tc_fence_after();
         const uint32_t d = tmem + (acc ? MX_ACC1 : 0);
         for (int ks = 0; ks < k_steps; ++ks) {
-          if (!mbar_wait(&full[stage], phase, abort_flag)) {
-            mx_report(p.status, ST_TIMEOUT_MMA_FULL);
+          tw = clock64();
+          if (!mbar_wait_warp(&full[stage], phase, abort_flag)) {
+            if (lead) mx_report(p.status, ST_TIMEOUT_MMA_FULL);
             ok = false;
             break;
           }
+          t_full += clock64() - tw;
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + stage * MX_STAGE_BYTES);
+          const uint32_t a = smem_u32(smem + stage * G::stage_bytes);
           const uint32_t b = a + MX_A_BYTES;
-          const uint32_t sa = b + MX_B_BYTES;
+          const uint32_t sa = b + G::b_bytes;
           const int left = p.k_bytes - ks * 128;                       // the contraction may end inside a k-step:
           const int mmas = left >= 128 ? 4 : (left + 31) / 32;         // no MMA past its last scale atom
-          mx_copy_step_scales<1>(tmem, sa, sa + MX_SF_BYTES, (mmas + 1) / 2);
+          if (lead) {
+            mx_copy_step_scales<CTAS>(tmem, sa, sa + MX_SF_BYTES, (mmas + 1) / 2);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            if (kk < mmas)
-              umma_mxf4<1>(d, umma_smem_desc(a + kk * 32, 16, 1024), umma_smem_desc(b + kk * 32, 16, 1024),
-                           mx_idesc(MX_BM, MX_BN, (kk & 1) * 2), tmem + MX_SFA + 4 * (kk >> 1), tmem + MX_SFB + 8 * (kk >> 1),
-                           (ks | kk) != 0 ? 1u : 0u);
+            for (int kk = 0; kk < 4; ++kk) {
+              if (kk < mmas)
+                umma_mxf4<CTAS>(d, umma_smem_desc(a + kk * 32, 16, 1024), umma_smem_desc(b + kk * 32, 16, 1024),
+                                mx_idesc(TILE_M, MX_BN, (kk & 1) * 2), tmem + MX_SFA + 4 * (kk >> 1),
+                                tmem + MX_SFB + 8 * (kk >> 1), (ks | kk) != 0 ? 1u : 0u);
+            }
+            if constexpr (CTAS == 2) umma_commit_pair(&empty[stage], 3);
+            else umma_commit(&empty[stage]);
           }
-          umma_commit(&empty[stage]);
-          if (++stage == MX_STAGES) { stage = 0; phase ^= 1; }
+          __syncwarp();
+          if (++stage == G::stages) { stage = 0; phase ^= 1; }
         }
-        if (ok) umma_commit(&tfull[acc]);
+        if (ok && lead) {
+          if constexpr (CTAS == 2) umma_commit_pair(&tfull[acc], 3);
+          else umma_commit(&tfull[acc]);
+        }
+        __syncwarp();
+      }
+      if (p.prof && lead) {
+        p.prof[blockIdx.x * 8 + 0] = clock64() - t_begin;
+        p.prof[blockIdx.x * 8 + 1] = t_full;
+        p.prof[blockIdx.x * 8 + 2] = t_tmem;
+        p.prof[blockIdx.x * 8 + 7] = it;
       }
     }
     __syncwarp();
   } else {
     const int q = warp & 3, part = (warp - 2) >> 2, row = q * 32 + lane;
     int it = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x, ++it) {
-      const MxTile tc = mx_tile(t, MX_BM, 0, tiles_v, m_tiles, n_tiles, p.group_m, Mv, Mt, cap);
+    const long long t_begin = clock64();
+    long long t_wait = 0;
+    for (int t = first; t < total; t += step, ++it) {
+      const MxTile tc = mx_tile(t, TILE_M, rank * MX_BM, tiles_v, m_tiles, n_tiles, p.group_m, Mv, Mt, cap);
       const int acc = it & 1;
       int w = 1;
+      const long long tw = clock64();
       if (lane == 0) w = mbar_wait(&tfull[acc], (it >> 1) & 1, abort_flag) ? 1 : 0;
+      t_wait += clock64() - tw;
       if (!__shfl_sync(0xFFFFFFFFu, w, 0)) {
         if (lane == 0) mx_report(p.status, ST_TIMEOUT_EPILOGUE);
         break;
@@ -437,16 +498,24 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
       mx_epilogue<EPI>(taddr, p, tc, acc, row, part, staging + (warp - 2) * 2048, lane, [&] {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty);
+        if (lane == 0) {
+          if constexpr (CTAS == 2) mbar_arrive_cluster(mapa_shared(smem_u32(tempty), 0));
+          else mbar_arrive(tempty);
+        }
       });
+    }
+    if (p.prof && warp == 2 && lane == 0) {
+      p.prof[blockIdx.x * 8 + 5] = t_wait;
+      p.prof[blockIdx.x * 8 + 6] = clock64() - t_begin;
     }
   }
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync_all();   // the partner's shared memory and barriers stay alive until both are done
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc<1>(tmem, 512);
+    tmem_dealloc<CTAS>(tmem, 512);
   }
 }
 
@@ -475,19 +544,40 @@ static int mx_group_m(int64_t k, int64_t rows_per_tile) {
   return static_cast<int>(g < 4 ? 4 : (g > 64 ? 64 : g));
 }
 
-static int mx_a_box_rows(int64_t M) { return M >= MX_BM ? MX_BM : static_cast<int>((M + 7) / 8 * 8); }
+static int mx_a_box_rows(int64_t M) { return M >= MX_BM || tune_overrides().pair > 0 ? MX_BM : static_cast<int>((M + 7) / 8 * 8); }
+
+// CTA pairs or single CTAs.
+static bool mx_pairs(int64_t M) {
+  const int forced = tune_overrides().pair;
+  return forced >= 0 ? forced != 0 : M >= 2048;
+}
+
+template <int EPI, int CTAS>
+static int mx_launch_as(const MxMaps& maps, const MxParams& p, int64_t M, cudaStream_t stream) {
+  const int n_per_tile = mx_glu(EPI) ? MX_BN / 2 : MX_BN;
+  int64_t units = ((M + MX_BM * CTAS - 1) / (MX_BM * CTAS) + 1) * ((p.n_out + n_per_tile - 1) / n_per_tile);
+  if (units > usable_sms() / CTAS) units = usable_sms() / CTAS;
+  const cudaError_t e = cudaFuncSetAttribute(mx_gemm_kernel<EPI, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, MxGeom<CTAS>::smem);
+  if (e != cudaSuccess) return cuda_status(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * CTAS));
+  cfg.blockDim = dim3(MX_THREADS);
+  cfg.dynamicSmemBytes = MxGeom<CTAS>::smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CTAS;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CTAS == 2 ? 1 : 0;
+  return cuda_status(cudaLaunchKernelEx(&cfg, mx_gemm_kernel<EPI, CTAS>, maps, p));
+}
 
 template <int EPI>
-static int mx_launch(const MxMaps& maps, const MxParams& p, int64_t M, cudaStream_t stream) {
-  const DeviceInfo& dev = device_info();
-  if (dev.cc_major != 10) return FFNK_ERR_DEVICE;
-  const int n_per_tile = mx_glu(EPI) ? MX_BN / 2 : MX_BN;
-  int64_t grid = ((M + MX_BM - 1) / MX_BM + 1) * ((p.n_out + n_per_tile - 1) / n_per_tile);
-  if (grid > usable_sms()) grid = usable_sms();
-  const cudaError_t e = cudaFuncSetAttribute(mx_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, MX_SMEM);
-  if (e != cudaSuccess) return cuda_status(e);
-  mx_gemm_kernel<EPI><<<static_cast<unsigned>(grid), MX_THREADS, MX_SMEM, stream>>>(maps, p);
-  return cuda_status(cudaGetLastError());
+static int mx_launch(const MxMaps& maps, const MxParams& p, int64_t M, bool pairs, cudaStream_t stream) {
+  if (device_info().cc_major != 10) return FFNK_ERR_DEVICE;
+  return pairs ? mx_launch_as<EPI, 2>(maps, p, M, stream) : mx_launch_as<EPI, 1>(maps, p, M, stream);
 }
 
 // y[token] = routed rows of (codes, scales) by the modality's weight [N, K]
@@ -497,18 +587,20 @@ static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt,
   int r;
   const int64_t rows = ffnk_route_capacity(M) + 512;
   if ((r = mx_maps(&m.a, &m.sa, a, rows, K, mx_a_box_rows(M), 1))) return r;
-  if ((r = mx_maps(&m.b[0], &m.sb[0], wv, N, K, MX_BN, 2))) return r;
-  if ((r = mx_maps(&m.b[2], &m.sb[2], wt, N, K, MX_BN, 2))) return r;
+  const bool pairs = mx_pairs(M);
+  const int box = pairs ? MX_BN / 2 : MX_BN;
+  if ((r = mx_maps(&m.b[0], &m.sb[0], wv, N, K, box, 2))) return r;
+  if ((r = mx_maps(&m.b[2], &m.sb[2], wt, N, K, box, 2))) return r;
   m.b[1] = m.b[0]; m.b[3] = m.b[2]; m.sb[1] = m.sb[0]; m.sb[3] = m.sb[2];
   MxParams p{};
-  p.perm = perm; p.counts = counts; p.status = status;
+  p.perm = perm; p.counts = counts; p.status = status; p.prof = debug_profile_buffer();
   p.n_out = static_cast<int>(N);
   p.k_bytes = static_cast<int>(mx_code_ld(K));
   p.a_rows = mx_a_box_rows(M);
-  p.group_m = mx_group_m(K, MX_BM);
+  p.group_m = mx_group_m(K, pairs ? 2 * MX_BM : MX_BM);
   p.out = static_cast<__nv_bfloat16*>(y);
   p.ldo = ldy;
-  return mx_launch<MX_EPI_STORE>(m, p, M, s);
+  return mx_launch<MX_EPI_STORE>(m, p, M, pairs, s);
 }
 
 // quantised silu(gate) * up of the routed rows, optionally with the pre-activations kept (t1, t3 both or neither)
@@ -521,18 +613,19 @@ static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* p
   for (int i = 0; i < 4; ++i)
     if ((r = mx_maps(&m.b[i], &m.sb[i], w[i], h, d, MX_BN / 2, 1))) return r;
   MxParams p{};
-  p.perm = perm; p.counts = counts; p.status = status;
+  p.perm = perm; p.counts = counts; p.status = status; p.prof = debug_profile_buffer();
   p.n_out = static_cast<int>(h);
   p.k_bytes = static_cast<int>(mx_code_ld(d));
   p.a_rows = mx_a_box_rows(M);
-  p.group_m = mx_group_m(d, MX_BM);
+  const bool pairs = mx_pairs(M);
+  p.group_m = mx_group_m(d, pairs ? 2 * MX_BM : MX_BM);
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = static_cast<uint8_t*>(scales);
   p.code_ld = mx_code_ld(h);
   p.k_atoms_out = static_cast<int>(mx_k_atoms(h));
   p.t1 = static_cast<float*>(t1);
   p.t3 = static_cast<float*>(t3);
-  return t1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, s) : mx_launch<MX_EPI_GLU>(m, p, M, s);
+  return t1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, pairs, s) : mx_launch<MX_EPI_GLU>(m, p, M, pairs, s);
 }
 
 static int64_t mx_align(int64_t v) { return (v + 255) & ~int64_t(255); }
