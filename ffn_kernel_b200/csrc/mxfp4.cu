@@ -14,6 +14,8 @@
 #include "ptx.cuh"
 #include "route.cuh"
 
+#include <type_traits>
+
 namespace ffnk {
 
 template <int T> struct MxType;
@@ -26,125 +28,193 @@ __device__ __forceinline__ float mx_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float mx_float(float v) { return v; }
 
 constexpr int kQuantThreads = 256;
-constexpr int kChunk = 256;          // columns of one warp step: a lane holds 8 consecutive values, 4 lanes a block
-constexpr int kChunksPerItem = 4;    // warp steps whose loads are in flight together
+constexpr int kQuantPerSm = 4;        // resident CTAs the row kernels are compiled for
+constexpr int kChunksMax = 2;         // warp steps of a row in flight together (for few rows one, on more warps)
 
-// Eight consecutive values of a row as floats; beyond `cols` zeros.  `vec`: the row is 16-byte aligned.
+// A lane holds 32 bytes of a row, one 256-bit load: 16 values of a 16-bit type (two lanes a block) or 8 of fp32 (four).
+template <typename T> struct MxLane {
+  static constexpr int values = 32 / sizeof(T);
+  static constexpr int chunk = 32 * values;          // columns of one warp step
+  static constexpr int lanes_per_block = 32 / values;
+};
+struct MxRaw {
+  uint32_t w[8];
+};
+
+// Values c ... of a row; beyond `cols` zeros.  align: bytes the rows are aligned to (32, 16, or less).
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t cols, bool vec, float (&v)[8]) {
-  if (vec && c + 8 <= cols) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + c));
-      __align__(16) T e[8];
-      *reinterpret_cast<uint4*>(e) = w;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = mx_float(e[i]);
+__device__ __forceinline__ MxRaw load_lane(const T* row, int c, int cols, int align) {
+  MxRaw r;
+  if (align >= 16 && c + MxLane<T>::values <= cols) {
+    if (align >= 32) {
+      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+                   : "l"(row + c));
     } else {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(row + c)), b = __ldg(reinterpret_cast<const float4*>(row + c) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c)), b = __ldg(reinterpret_cast<const uint4*>(row + c) + 1);
+      r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+      r.w[4] = b.x; r.w[5] = b.y; r.w[6] = b.z; r.w[7] = b.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? mx_float(row[c + i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const int k = c + 2 * i;
+        const uint32_t lo = k < cols ? reinterpret_cast<const unsigned short*>(row)[k] : 0u;
+        const uint32_t hi = k + 1 < cols ? reinterpret_cast<const unsigned short*>(row)[k + 1] : 0u;
+        r.w[i] = lo | hi << 16;
+      } else {
+        r.w[i] = c + i < cols ? reinterpret_cast<const uint32_t*>(row)[c + i] : 0u;
+      }
+    }
   }
+  return r;
 }
 
-// One warp, one row, up to kChunksPerItem chunks of 256 columns from chunk `first` on.  Every lane of a block's
-// four gets the block's maximum by two shuffles; the eight scale bytes of a chunk are two words of two atoms.
+// bits of the lane's max |x| as fp32 (16-bit types: packed integer maxima of two values at a time, converted once)
 template <typename T>
-__device__ __forceinline__ void quantize_row(const T* row, bool vec, int64_t cols, int first, int chunks, uint8_t* codes_row,
-                                             uint8_t* scales, int64_t dst, int64_t k_atoms, int lane) {
-  float v[kChunksPerItem][8];
+__device__ __forceinline__ uint32_t absmax_bits(const MxRaw& r) {
+  constexpr uint32_t mask = sizeof(T) == 2 ? 0x7FFF7FFFu : 0x7FFFFFFFu;
+  uint32_t m = 0;
 #pragma unroll
-  for (int u = 0; u < kChunksPerItem; ++u)
-    if (first + u < chunks) load8(row, static_cast<int64_t>(first + u) * kChunk + lane * 8, cols, vec, v[u]);
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 2) m = __vmaxu2(m, r.w[i] & mask);
+    else m = max(m, r.w[i] & mask);
+  }
+  if constexpr (sizeof(T) == 2) m = max(m & 0xFFFFu, m >> 16);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return m << 16;
+  else if constexpr (sizeof(T) == 2) return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+  else return m;
+}
+
+template <typename T>
+__device__ __forceinline__ float raw_value(const MxRaw& r, int i) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? r.w[i >> 1] & 0xFFFF0000u : r.w[i >> 1] << 16);
+  else if constexpr (sizeof(T) == 2) return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? r.w[i >> 1] >> 16 : r.w[i >> 1])));
+  else return __uint_as_float(r.w[i]);
+}
+
+// One chunk of a row: the lanes of a block share its maximum by shuffles, each rounds its own values.
+template <typename T>
+__device__ __forceinline__ void quantize_chunk(const MxRaw& raw, int chunk, int cols, uint8_t* codes_row, uint8_t* scale_row,
+                                               int k_atoms, int lane) {
+  using L = MxLane<T>;
+  uint32_t m = absmax_bits<T>(raw);
 #pragma unroll
-  for (int u = 0; u < kChunksPerItem; ++u) {
-    if (first + u >= chunks) break;                    // warp-uniform
-    uint32_t m = 0;
+  for (int o = 1; o < L::lanes_per_block; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  const uint32_t byte = mx_scale_byte(m);
+  const float inv = mx_inverse_scale(byte);
+  uint32_t code[L::values / 8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[u][i]) & 0x7FFFFFFFu);
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-    const uint32_t byte = mx_scale_byte(m);
-    const float inv = mx_inverse_scale(byte);
+  for (int j = 0; j < L::values / 8; ++j) {
+    float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[u][i] = mul_keep_subnormals(v[u][i], inv);
-    uint32_t code = byte == 255u ? 0u : mx_pack8(v[u]);
-    const int64_t c = static_cast<int64_t>(first + u) * kChunk + lane * 8;
-    if (c < (cols + 31) / 32 * 32) *reinterpret_cast<uint32_t*>(codes_row + c / 2) = code;
-    uint32_t word = byte << (8 * ((lane >> 2) & 3));
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
-    const int64_t atom = static_cast<int64_t>(first + u) * 2 + (lane >> 4);
-    if ((lane & 15) == 0 && atom < k_atoms) *reinterpret_cast<uint32_t*>(scales + mx_scale_word(dst, atom, k_atoms)) = word;
+    for (int i = 0; i < 8; ++i) v[i] = mul_keep_subnormals(raw_value<T>(raw, 8 * j + i), inv);
+    code[j] = byte == 255u ? 0u : mx_pack8(v);
+  }
+  const int c = chunk * L::chunk + lane * L::values;
+  if (c < ((cols + 31) & ~31)) {
+    if constexpr (L::values == 16) *reinterpret_cast<uint2*>(codes_row + c / 2) = make_uint2(code[0], code[1]);
+    else *reinterpret_cast<uint32_t*>(codes_row + c / 2) = code[0];
+  }
+  const int block = c >> 5;
+  if (lane % L::lanes_per_block == 0 && (block >> 2) < k_atoms)
+    scale_row[static_cast<int64_t>(block >> 2) * kMxAtomBytes + (block & 3)] = static_cast<uint8_t>(byte);
+}
+
+// The rows of one warp, `n` <= kChunksMax chunks from chunk `first` on; the next row's loads are in flight while one
+// is rounded.  `row(i)` names the i-th row's source and destination (source < 0: no further row).
+struct MxRowRef {
+  int src, dst;
+};
+template <typename T, class Rows>
+__device__ __forceinline__ void quantize_rows(const T* x, int64_t ldx, int align, int cols, int first, int n, uint8_t* codes,
+                                              uint8_t* scales, int lane, Rows&& row) {
+  const int64_t ld = mx_code_ld(cols);
+  const int k_atoms = static_cast<int>(mx_k_atoms(cols));
+  MxRowRef now = row(0), next = row(1);
+  MxRaw raw[kChunksMax];
+  auto load = [&](const MxRowRef& r) {
+#pragma unroll
+    for (int u = 0; u < kChunksMax; ++u)
+      if (u < n && r.src >= 0) raw[u] = load_lane(x + r.src * ldx, (first + u) * MxLane<T>::chunk + lane * MxLane<T>::values, cols, align);
+  };
+  load(now);
+  for (int i = 2; now.src >= 0; ++i) {
+    MxRaw cur[kChunksMax];
+#pragma unroll
+    for (int u = 0; u < kChunksMax; ++u) cur[u] = raw[u];
+    load(next);
+    const MxRowRef after = row(i);
+#pragma unroll
+    for (int u = 0; u < kChunksMax; ++u)
+      if (u < n)                                       // warp-uniform
+        quantize_chunk<T>(cur[u], first + u, cols, codes + now.dst * ld, scales + mx_scale_word(now.dst, 0, k_atoms), k_atoms, lane);
+    now = next;
+    next = after;
   }
 }
 
+// blockIdx.y: which group of `per_warp` chunks of every row.
 // Plain (perm == nullptr): row r of x -> row r; the scale bytes of the rows that fill the last atom are zeroed.
 // Routed: rows in routed order (visual rows first, text rows from the next multiple of 256), none beyond them.
+// Measured: 32768 x 4096 bf16 52.6 us = 6.46 TB/s, 0.99 of a plain copy; 11008 x 4096 fp32 32.3 us = 6.32 TB/s.  (Loads of
+// one row at a time, without the next row in flight, and 16-byte loads: 78 us; with 64-bit index divisions 118 us.)
 template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) mx_quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
-                                                                         int64_t cols, const int* __restrict__ perm,
-                                                                         const int* __restrict__ counts,
-                                                                         uint8_t* __restrict__ codes,
-                                                                         uint8_t* __restrict__ scales, bool vec) {
+__global__ void __launch_bounds__(kQuantThreads, kQuantPerSm) mx_quantize_rows_kernel(
+    const T* __restrict__ x, int64_t ldx, int rows, int cols, const int* __restrict__ perm, const int* __restrict__ counts,
+    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int align, int per_warp) {
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int chunks = static_cast<int>((cols + kChunk - 1) / kChunk);
-  const int groups = (chunks + kChunksPerItem - 1) / kChunksPerItem;
-  const int64_t ld = mx_code_ld(cols), k_atoms = mx_k_atoms(cols);
-  const int64_t all_rows = perm ? rows : mx_row_atoms(rows) * 128;
-  const int64_t items = all_rows * groups;
-  int Mv = 0, cap = 0;
+  const int chunks = (cols + MxLane<T>::chunk - 1) / MxLane<T>::chunk;
+  const int first = blockIdx.y * per_warp, n = min(per_warp, chunks - first);
+  const int step = gridDim.x * (kQuantThreads / 32);
+  const int r0 = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   if (perm) {
-    Mv = counts[0];
-    cap = counts[2];
+    const int Mv = counts[0], cap = counts[2], text_base = ((Mv + 255) >> 8) << 8;
+    quantize_rows(x, ldx, align, cols, first, n, codes, scales, lane, [&](int i) {
+      const int64_t r = r0 + static_cast<int64_t>(i) * step;
+      if (r >= rows) return MxRowRef{-1, 0};
+      const int k = static_cast<int>(r);
+      return k < Mv ? MxRowRef{perm[k], k} : MxRowRef{perm[cap + (k - Mv)], text_base + (k - Mv)};
+    });
+    return;
   }
-  const int64_t text_base = ((Mv + 255) >> 8) << 8;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5); it < items;
-       it += static_cast<int64_t>(gridDim.x) * (kQuantThreads / 32)) {
-    const int64_t r = it / groups;
-    const int first = static_cast<int>(it - r * groups) * kChunksPerItem;
-    if (r >= rows) {
-      for (int64_t a = first * 2 + lane; a < k_atoms && a < (first + kChunksPerItem) * 2; a += 32)
-        *reinterpret_cast<uint32_t*>(scales + mx_scale_word(r, a, k_atoms)) = 0u;
-      continue;
-    }
-    int64_t src = r, dst = r;
-    if (perm) {
-      src = r < Mv ? perm[r] : perm[cap + (r - Mv)];
-      dst = r < Mv ? r : text_base + (r - Mv);
-    }
-    quantize_row(x + src * ldx, vec, cols, first, chunks, codes + dst * ld, scales, dst, k_atoms, lane);
-  }
+  quantize_rows(x, ldx, align, cols, first, n, codes, scales, lane, [&](int i) {
+    const int64_t r = r0 + static_cast<int64_t>(i) * step;
+    return r < rows ? MxRowRef{static_cast<int>(r), static_cast<int>(r)} : MxRowRef{-1, 0};
+  });
+  // rows that only fill the last atom
+  const int k_atoms = static_cast<int>(mx_k_atoms(cols));
+  const int a0 = first * (MxLane<T>::chunk / 128), a1 = min(k_atoms, (first + n) * (MxLane<T>::chunk / 128));
+  for (int64_t r = rows + r0; r < mx_row_atoms(rows) * 128; r += step)
+    for (int a = a0 + lane; a < a1; a += 32) *reinterpret_cast<uint32_t*>(scales + mx_scale_word(r, a, k_atoms)) = 0u;
 }
 
 // Routing and quantisation of the activations in one launch (M <= 8192): every CTA routes the whole mask for
-// itself in shared memory, CTA 0 also writes perm and counts, then every warp quantises its share of the rows.
-__global__ void __launch_bounds__(kRouteThreads) mx_route_quantize_kernel(const uint8_t* __restrict__ mask, int M, int cap,
-                                                                          int* __restrict__ perm, int* __restrict__ counts,
-                                                                          const __nv_bfloat16* __restrict__ x, int64_t ldx,
-                                                                          int64_t cols, uint8_t* __restrict__ codes,
-                                                                          uint8_t* __restrict__ scales) {
+// itself in shared memory, CTA (0, 0) also writes perm and counts, then every warp quantises its share of the rows.
+__global__ void __launch_bounds__(kRouteThreads, kQuantPerSm) mx_route_quantize_kernel(
+    const uint8_t* __restrict__ mask, int M, int cap, int* __restrict__ perm, int* __restrict__ counts,
+    const __nv_bfloat16* __restrict__ x, int64_t ldx, int cols, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+    int align, int per_warp) {
   __shared__ int s_list[kRouteTile];   // visual tokens ascending, then text tokens ascending
   __shared__ int s_warp[kRouteThreads / 32];
   __shared__ int s_runs;
   const int tid = threadIdx.x, lane = tid & 31;
+  const bool writer = blockIdx.x == 0 && blockIdx.y == 0;
   griddep_launch_dependents();
   const ThreadTokens tt = load_thread_tokens(mask, M, tid * kRoutePerThread);
   if (tid == 0) s_runs = 0;
   int Mv = 0;
   const int ev = block_exclusive_scan(__popc(tt.bits), s_warp, &Mv);
-  if (blockIdx.x == 0) {
+  if (writer) {
     const int wr = __reduce_add_sync(0xFFFFFFFFu, tt.nruns);
     if (lane == 0 && wr) atomicAdd(&s_runs, wr);
   }
   compact_tile(s_list, s_list + Mv, 0, tt.bits, ev, tt.valid);
   __syncthreads();
   const int Mt = M - Mv;
-  if (blockIdx.x == 0) {
+  if (writer) {
     for (int i = tid; i < Mv; i += kRouteThreads) perm[i] = s_list[i];
     for (int i = tid; i < Mt; i += kRouteThreads) perm[cap + i] = s_list[Mv + i];
     if (tid == 0) {
@@ -155,63 +225,85 @@ __global__ void __launch_bounds__(kRouteThreads) mx_route_quantize_kernel(const 
       counts[4] = s_runs;
     }
   }
-  const int64_t text_base = ((Mv + 255) >> 8) << 8;
-  const int chunks = static_cast<int>((cols + kChunk - 1) / kChunk);
-  const int groups = (chunks + kChunksPerItem - 1) / kChunksPerItem;
-  const int64_t ld = mx_code_ld(cols), k_atoms = mx_k_atoms(cols);
-  const int64_t items = static_cast<int64_t>(M) * groups;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * (kRouteThreads / 32) + (tid >> 5); it < items;
-       it += static_cast<int64_t>(gridDim.x) * (kRouteThreads / 32)) {
-    const int i = static_cast<int>(it / groups);
-    const int first = static_cast<int>(it - static_cast<int64_t>(i) * groups) * kChunksPerItem;
-    const int64_t dst = i >= Mv ? text_base + (i - Mv) : i;
-    quantize_row(x + static_cast<int64_t>(s_list[i]) * ldx, true, cols, first, chunks, codes + dst * ld, scales, dst,
-                 k_atoms, lane);
-  }
+  const int text_base = ((Mv + 255) >> 8) << 8;
+  const int chunks = (cols + MxLane<__nv_bfloat16>::chunk - 1) / MxLane<__nv_bfloat16>::chunk;
+  const int first = blockIdx.y * per_warp, n = min(per_warp, chunks - first);
+  const int step = gridDim.x * (kRouteThreads / 32), r0 = blockIdx.x * (kRouteThreads / 32) + (tid >> 5);
+  quantize_rows(x, ldx, align, cols, first, n, codes, scales, lane, [&](int i) {
+    const int r = r0 + i * step;
+    return r < M ? MxRowRef{s_list[r], r >= Mv ? text_base + (r - Mv) : r} : MxRowRef{-1, 0};
+  });
 }
 
-// x(r, c) at x[c * ldc + r]: blocks run across the contiguous dimension.  A CTA takes 64 rows x one atom of
-// blocks; a thread reads the 32 values of one block (neighbouring lanes neighbouring rows), and the codes go
-// through shared memory so that a row leaves as 64 contiguous bytes.
-constexpr int kColRows = 64;
+// x(r, c) at x[c * ldc + r]: blocks run across the contiguous dimension.  A CTA takes 64 (fp32) or 128 (16-bit types)
+// rows x one atom of four blocks; a thread reads the 32 values of one block of one row, or of two neighbouring rows at
+// once, so that a warp reads 128 contiguous bytes a column; the codes go through shared memory so that a row leaves as
+// 64 contiguous bytes.  `pairs`: the 16-bit columns are 4-byte aligned.
+template <typename T> struct MxCols {
+  static constexpr int per_thread = 4 / sizeof(T);
+  static constexpr int rows = 64 * per_thread;
+};
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) mx_quantize_cols_kernel(const T* __restrict__ x, int64_t ldc, int64_t rows,
                                                                          int64_t cols, uint8_t* __restrict__ codes,
-                                                                         uint8_t* __restrict__ scales) {
-  __shared__ uint4 s_code[kColRows][5];      // four blocks a row, one piece of padding against bank conflicts
-  __shared__ uint8_t s_scale[kColRows][4];
+                                                                         uint8_t* __restrict__ scales, bool pairs) {
+  constexpr int P = MxCols<T>::per_thread, R = MxCols<T>::rows;
+  __shared__ uint4 s_code[R][5];             // four blocks a row, one piece of padding against bank conflicts
+  __shared__ __align__(4) uint8_t s_scale[R][4];
   const int tid = threadIdx.x;
   const int64_t ld = mx_code_ld(cols), k_atoms = mx_k_atoms(cols);
-  const int64_t row_tiles = mx_row_atoms(rows) * 2;
+  const int64_t row_tiles = mx_row_atoms(rows) * (128 / R);
   const int64_t tiles = row_tiles * k_atoms;
-  const int lr = tid & (kColRows - 1), b = tid >> 6;
+  const int lr = (tid & 63) * P, b = tid >> 6;
   for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int64_t atom = t / row_tiles, r0 = (t - atom * row_tiles) * kColRows;
+    const int64_t atom = t / row_tiles, r0 = (t - atom * row_tiles) * R;
     const int64_t r = r0 + lr, c0 = atom * 128 + b * 32;
-    float v[32];
+    uint32_t w[32];                          // one fp32, or two 16-bit values of neighbouring rows
+    const T* src = x + c0 * ldc + r;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = r < rows && c0 + i < cols ? mx_float(x[(c0 + i) * ldc + r]) : 0.0f;
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    const uint32_t byte = mx_scale_byte(m);
-    const float inv = mx_inverse_scale(byte);
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float a[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = mul_keep_subnormals(v[8 * j + i], inv);
-      w[j] = byte == 255u ? 0u : mx_pack8(a);
+    for (int i = 0; i < 32; ++i) {
+      w[i] = 0;
+      if (c0 + i < cols) {
+        if constexpr (P == 1) {
+          if (r < rows) w[i] = reinterpret_cast<const uint32_t*>(src)[i * ldc];
+        } else {
+          const unsigned short* q = reinterpret_cast<const unsigned short*>(src) + i * ldc;
+          if (pairs && r + 1 < rows) w[i] = __ldg(reinterpret_cast<const uint32_t*>(q));
+          else if (r < rows) w[i] = q[0] | (r + 1 < rows ? static_cast<uint32_t>(q[1]) << 16 : 0u);
+        }
+      }
     }
-    s_code[lr][b] = make_uint4(w[0], w[1], w[2], w[3]);
-    s_scale[lr][b] = static_cast<uint8_t>(byte);
+#pragma unroll
+    for (int h = 0; h < P; ++h) {
+      float v[32];
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        MxRaw one;
+        one.w[0] = w[i];
+        v[i] = raw_value<T>(one, h);
+        m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+      }
+      const uint32_t byte = mx_scale_byte(m);
+      const float inv = mx_inverse_scale(byte);
+      uint32_t c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float a[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = mul_keep_subnormals(v[8 * j + i], inv);
+        c[j] = byte == 255u ? 0u : mx_pack8(a);
+      }
+      s_code[lr + h][b] = make_uint4(c[0], c[1], c[2], c[3]);
+      s_scale[lr + h][b] = static_cast<uint8_t>(byte);
+    }
     __syncthreads();
-    const int64_t wr = r0 + (tid >> 2), block = atom * 4 + (tid & 3);
-    if (wr < rows && block * 16 < ld) *reinterpret_cast<uint4*>(codes + wr * ld + block * 16) = s_code[tid >> 2][tid & 3];
-    if (tid < kColRows)
-      *reinterpret_cast<uint32_t*>(scales + mx_scale_word(r0 + tid, atom, k_atoms)) =
-          *reinterpret_cast<const uint32_t*>(s_scale[tid]);
+    for (int i = tid; i < R * 4; i += kQuantThreads) {
+      const int64_t wr = r0 + (i >> 2), block = atom * 4 + (i & 3);
+      if (wr < rows && block * 16 < ld) *reinterpret_cast<uint4*>(codes + wr * ld + block * 16) = s_code[i >> 2][i & 3];
+    }
+    if (tid < R)
+      *reinterpret_cast<uint32_t*>(scales + mx_scale_word(r0 + tid, atom, k_atoms)) = *reinterpret_cast<const uint32_t*>(s_scale[tid]);
     __syncthreads();
   }
 }
@@ -231,37 +323,37 @@ struct MxDequantJob {
   const int* counts;
 };
 
+constexpr int kDqChunk = 256;         // columns of one warp step: a lane makes eight values
+constexpr int kDqChunksMax = 4;
 template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) mx_dequantize_kernel(const __grid_constant__ MxDequantJob job) {
-  const int w = blockIdx.y;
+__global__ void __launch_bounds__(kQuantThreads, 6) mx_dequantize_kernel(const __grid_constant__ MxDequantJob job, int per_warp) {
+  const int w = blockIdx.z;
   if (job.gate[w] >= 0 && job.counts[job.gate[w]] == 0) return;
   const uint8_t* __restrict__ codes = job.codes[w];
   const uint8_t* __restrict__ scales = job.scales[w];
   T* __restrict__ out = static_cast<T*>(job.out[w]);
-  const int64_t rows = job.rows[w], cols = job.cols[w], ldo = job.ldo[w];
-  const bool vec = ((reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(ldo * sizeof(T))) & 15) == 0;
+  const int rows = static_cast<int>(job.rows[w]), cols = static_cast<int>(job.cols[w]);
+  const int64_t ldo = job.ldo[w];
+  const bool vec = ((reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(ldo * sizeof(T))) & (8 * sizeof(T) - 1)) == 0;
   const int lane = threadIdx.x & 31;
-  const int chunks = static_cast<int>((cols + kChunk - 1) / kChunk);
-  const int groups = (chunks + kChunksPerItem - 1) / kChunksPerItem;
-  const int64_t ld = mx_code_ld(cols), k_atoms = mx_k_atoms(cols);
-  const int64_t items = rows * groups;
-  for (int64_t it = static_cast<int64_t>(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5); it < items;
-       it += static_cast<int64_t>(gridDim.x) * (kQuantThreads / 32)) {
-    const int64_t r = it / groups;
-    const int first = static_cast<int>(it - r * groups) * kChunksPerItem;
-    uint32_t code[kChunksPerItem] = {}, word[kChunksPerItem] = {};
+  const int first = blockIdx.y * per_warp;
+  const int64_t ld = mx_code_ld(cols);
+  const int k_atoms = static_cast<int>(mx_k_atoms(cols));
+  for (int r = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); r < rows; r += gridDim.x * (kQuantThreads / 32)) {
+    uint32_t code[kDqChunksMax] = {}, word[kDqChunksMax] = {};
+    const uint8_t* scale_row = scales + mx_scale_word(r, 0, k_atoms);
 #pragma unroll
-    for (int u = 0; u < kChunksPerItem; ++u) {
-      const int64_t c = static_cast<int64_t>(first + u) * kChunk + lane * 8;
-      if (c < cols) {
+    for (int u = 0; u < kDqChunksMax; ++u) {
+      const int c = (first + u) * kDqChunk + lane * 8;
+      if (u < per_warp && c < cols) {
         code[u] = __ldg(reinterpret_cast<const uint32_t*>(codes + r * ld + c / 2));
-        word[u] = __ldg(reinterpret_cast<const uint32_t*>(scales + mx_scale_word(r, c / 128, k_atoms)));
+        word[u] = __ldg(reinterpret_cast<const uint32_t*>(scale_row + static_cast<int64_t>(c / 128) * kMxAtomBytes));
       }
     }
 #pragma unroll
-    for (int u = 0; u < kChunksPerItem; ++u) {
-      const int64_t c = static_cast<int64_t>(first + u) * kChunk + lane * 8;
-      if (c >= cols) break;
+    for (int u = 0; u < kDqChunksMax; ++u) {
+      const int c = (first + u) * kDqChunk + lane * 8;
+      if (u >= per_warp || c >= cols) break;
       const float s = mx_scale_value((word[u] >> (8 * ((lane >> 2) & 3))) & 255u);
       float v[8];
       mx_unpack8(code[u], v);
@@ -270,9 +362,13 @@ __global__ void __launch_bounds__(kQuantThreads) mx_dequantize_kernel(const __gr
       for (int i = 0; i < 8; ++i) mx_put(&e[i], mul_keep_subnormals(v[i], s));
       T* o = out + r * ldo + c;
       if (vec && c + 8 <= cols) {
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-          reinterpret_cast<uint4*>(o)[i] = reinterpret_cast<const uint4*>(e)[i];
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(e);
+        } else {
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o), "f"(e[0]), "f"(e[1]), "f"(e[2]), "f"(e[3]),
+                       "f"(e[4]), "f"(e[5]), "f"(e[6]), "f"(e[7])
+                       : "memory");
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -282,13 +378,31 @@ __global__ void __launch_bounds__(kQuantThreads) mx_dequantize_kernel(const __gr
   }
 }
 
-static unsigned quant_grid(int64_t warps_of_work, int per_sm) {
-  int64_t blocks = (warps_of_work + kQuantThreads / 32 - 1) / (kQuantThreads / 32);
-  const int64_t most = static_cast<int64_t>(device_info().sm_count) * per_sm;
-  if (blocks > most) blocks = most;
-  return static_cast<unsigned>(blocks < 1 ? 1 : blocks);
+// Rows over blockIdx.x, groups of chunks over blockIdx.y.  With many rows a warp takes as many chunks of a row as it
+// can hold in flight; with few, every chunk gets a warp of its own.
+constexpr int64_t kMaxGroups = 65535;                                    // blockIdx.y
+constexpr int64_t kMaxCols = kMaxGroups * 512;                           // 33553920: two chunks of 256 fp32 columns a group
+struct QuantShape {
+  dim3 grid;
+  int per_warp;
+};
+static QuantShape quant_shape(int64_t rows, int64_t cols, int chunk, int chunks_max, int per_sm) {
+  const int64_t chunks = (cols + chunk - 1) / chunk;
+  const int64_t blocks = static_cast<int64_t>(device_info().sm_count) * per_sm;
+  int per = chunks_max;
+  while (per > 1 && rows * ((chunks + per - 1) / per) < blocks * (kQuantThreads / 32) &&
+         (chunks + per / 2 - 1) / (per / 2) <= kMaxGroups)
+    per /= 2;
+  const int64_t groups = (chunks + per - 1) / per;
+  int64_t x = (rows + kQuantThreads / 32 - 1) / (kQuantThreads / 32);
+  const int64_t most = (blocks + groups - 1) / groups;
+  if (x > most) x = most;
+  return QuantShape{dim3(static_cast<unsigned>(x < 1 ? 1 : x), static_cast<unsigned>(groups)), per};
 }
-static int64_t row_groups(int64_t cols) { return (cols + kChunk * kChunksPerItem - 1) / (kChunk * kChunksPerItem); }
+static int row_alignment(const void* x, int64_t row_bytes) {
+  const uintptr_t v = reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(row_bytes);
+  return v & 15 ? 1 : (v & 31 ? 16 : 32);
+}
 
 template <int T>
 static int quantize_typed(const void* x_, int64_t row_stride, int64_t col_stride, int64_t rows, int64_t cols, void* codes,
@@ -298,14 +412,16 @@ static int quantize_typed(const void* x_, int64_t row_stride, int64_t col_stride
   uint8_t* c = static_cast<uint8_t*>(codes);
   uint8_t* sc = static_cast<uint8_t*>(scales);
   if (col_stride == 1 || cols == 1) {
-    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (row_stride * static_cast<int64_t>(sizeof(E))) % 16 == 0;
-    mx_quantize_rows_kernel<E><<<quant_grid(mx_row_atoms(rows) * 128 * row_groups(cols), 8), kQuantThreads, 0, s>>>(
-        x, row_stride, rows, cols, nullptr, nullptr, c, sc, vec);
+    const QuantShape q = quant_shape(rows, cols, MxLane<E>::chunk, kChunksMax, kQuantPerSm);
+    mx_quantize_rows_kernel<E><<<q.grid, kQuantThreads, 0, s>>>(
+        x, row_stride, static_cast<int>(rows), static_cast<int>(cols), nullptr, nullptr, c, sc,
+        row_alignment(x, row_stride * static_cast<int64_t>(sizeof(E))), q.per_warp);
   } else {
-    int64_t tiles = mx_row_atoms(rows) * 2 * mx_k_atoms(cols);
+    int64_t tiles = mx_row_atoms(rows) * (128 / MxCols<E>::rows) * mx_k_atoms(cols);
     const int64_t most = static_cast<int64_t>(device_info().sm_count) * 8;
     if (tiles > most) tiles = most;
-    mx_quantize_cols_kernel<E><<<static_cast<unsigned>(tiles), kQuantThreads, 0, s>>>(x, col_stride, rows, cols, c, sc);
+    mx_quantize_cols_kernel<E><<<static_cast<unsigned>(tiles), kQuantThreads, 0, s>>>(
+        x, col_stride, rows, cols, c, sc, ((reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(col_stride * sizeof(E))) & 3) == 0);
   }
   return cuda_status(cudaGetLastError());
 }
@@ -317,22 +433,24 @@ int mx_route_quantize(const void* mask, int64_t M, const void* x, int64_t ldx, i
   uint8_t* c = static_cast<uint8_t*>(codes);
   uint8_t* sc = static_cast<uint8_t*>(scales);
   if (M <= kRouteTile) {
-    mx_route_quantize_kernel<<<quant_grid(M * row_groups(d), 4), kRouteThreads, 0, s>>>(
-        static_cast<const uint8_t*>(mask), static_cast<int>(M), static_cast<int>(ffnk_route_capacity(M)), perm, counts, xb,
-        ldx, d, c, sc);
+    const QuantShape q = quant_shape(M, d, MxLane<__nv_bfloat16>::chunk, kChunksMax, kQuantPerSm);
+    mx_route_quantize_kernel<<<q.grid, kRouteThreads, 0, s>>>(static_cast<const uint8_t*>(mask), static_cast<int>(M),
+                                                              static_cast<int>(ffnk_route_capacity(M)), perm, counts, xb, ldx,
+                                                              static_cast<int>(d), c, sc, row_alignment(x, 2 * ldx), q.per_warp);
     return cuda_status(cudaGetLastError());
   }
   const int r = ffnk_route(mask, M, perm, counts, scan, status, stream);
   if (r) return r;
-  mx_quantize_rows_kernel<__nv_bfloat16><<<quant_grid(M * row_groups(d), 8), kQuantThreads, 0, s>>>(
-      xb, ldx, M, d, perm, counts, c, sc, true);
+  const QuantShape q = quant_shape(M, d, MxLane<__nv_bfloat16>::chunk, kChunksMax, kQuantPerSm);
+  mx_quantize_rows_kernel<__nv_bfloat16><<<q.grid, kQuantThreads, 0, s>>>(xb, ldx, static_cast<int>(M), static_cast<int>(d), perm,
+                                                                          counts, c, sc, row_alignment(x, 2 * ldx), q.per_warp);
   return cuda_status(cudaGetLastError());
 }
 
 int mx_dequantize_weights(const void* const* codes, const void* const* scales, const int64_t* rows, const int64_t* cols,
                           const int* gate, int n, const int32_t* counts, void* const* out, void* stream) {
   MxDequantJob job{};
-  int64_t items = 0;
+  int64_t most_rows = 0, most_cols = 0;
   for (int i = 0; i < n; ++i) {
     job.codes[i] = static_cast<const uint8_t*>(codes[i]);
     job.scales[i] = static_cast<const uint8_t*>(scales[i]);
@@ -340,10 +458,13 @@ int mx_dequantize_weights(const void* const* codes, const void* const* scales, c
     job.rows[i] = rows[i];
     job.cols[i] = job.ldo[i] = cols[i];
     job.gate[i] = gate[i];
-    items = rows[i] * row_groups(cols[i]) > items ? rows[i] * row_groups(cols[i]) : items;
+    most_rows = rows[i] > most_rows ? rows[i] : most_rows;
+    most_cols = cols[i] > most_cols ? cols[i] : most_cols;
   }
   job.counts = counts;
-  mx_dequantize_kernel<__nv_bfloat16><<<dim3(quant_grid(items, 8), n), kQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(job);
+  QuantShape q = quant_shape(most_rows, most_cols, kDqChunk, kDqChunksMax, 6);
+  q.grid.z = n;
+  mx_dequantize_kernel<__nv_bfloat16><<<q.grid, kQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(job, q.per_warp);
   return cuda_status(cudaGetLastError());
 }
 
@@ -362,7 +483,7 @@ extern "C" int64_t ffnk_mxfp4_scale_bytes(int64_t rows, int64_t cols) {
 
 extern "C" int ffnk_mxfp4_quantize(const void* x, int dtype, int64_t row_stride, int64_t col_stride, int64_t rows,
                                    int64_t cols, void* codes, void* scales, void* stream) {
-  if (mx_bad_size(rows) || mx_bad_size(cols) || dtype < FFNK_BF16 || dtype > FFNK_FP32) return FFNK_ERR_SHAPE;
+  if (mx_bad_size(rows) || mx_bad_size(cols) || cols > kMaxCols || dtype < FFNK_BF16 || dtype > FFNK_FP32) return FFNK_ERR_SHAPE;
   if (rows == 0 || cols == 0) return 0;
   if (!x || !codes || !scales) return FFNK_ERR_NULL;
   if (!(col_stride == 1 || cols == 1) && !(row_stride == 1 || rows == 1)) return FFNK_ERR_LAYOUT;
@@ -380,14 +501,14 @@ extern "C" int ffnk_mxfp4_quantize(const void* x, int dtype, int64_t row_stride,
 
 extern "C" int ffnk_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype,
                                      int64_t ldo, void* stream) {
-  if (mx_bad_size(rows) || mx_bad_size(cols) || dtype < FFNK_BF16 || dtype > FFNK_FP32) return FFNK_ERR_SHAPE;
+  if (mx_bad_size(rows) || mx_bad_size(cols) || cols > kMaxCols || dtype < FFNK_BF16 || dtype > FFNK_FP32) return FFNK_ERR_SHAPE;
   if (rows == 0 || cols == 0) return 0;
   if (!codes || !scales || !out) return FFNK_ERR_NULL;
   const int size = dtype == FFNK_FP32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(codes) & 15) || (reinterpret_cast<uintptr_t>(scales) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & (size - 1)) || ldo < cols)
     return FFNK_ERR_ALIGN;
-  const unsigned grid = quant_grid(rows * row_groups(cols), 8);
+  const QuantShape q = quant_shape(rows, cols, kDqChunk, kDqChunksMax, 6);
   MxDequantJob job{};
   job.codes[0] = static_cast<const uint8_t*>(codes);
   job.scales[0] = static_cast<const uint8_t*>(scales);
@@ -398,9 +519,9 @@ extern "C" int ffnk_mxfp4_dequantize(const void* codes, const void* scales, int6
   job.gate[0] = -1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case FFNK_BF16: mx_dequantize_kernel<__nv_bfloat16><<<grid, kQuantThreads, 0, s>>>(job); break;
-    case FFNK_FP16: mx_dequantize_kernel<__half><<<grid, kQuantThreads, 0, s>>>(job); break;
-    default: mx_dequantize_kernel<float><<<grid, kQuantThreads, 0, s>>>(job);
+    case FFNK_BF16: mx_dequantize_kernel<__nv_bfloat16><<<q.grid, kQuantThreads, 0, s>>>(job, q.per_warp); break;
+    case FFNK_FP16: mx_dequantize_kernel<__half><<<q.grid, kQuantThreads, 0, s>>>(job, q.per_warp); break;
+    default: mx_dequantize_kernel<float><<<q.grid, kQuantThreads, 0, s>>>(job, q.per_warp);
   }
   return cuda_status(cudaGetLastError());
 }

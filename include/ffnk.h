@@ -332,7 +332,7 @@ int64_t ffnk_mxfp4_code_bytes(int64_t rows, int64_t cols);
 int64_t ffnk_mxfp4_scale_bytes(int64_t rows, int64_t cols);
 
 /* x(r, c) at x[r * row_stride + c * col_stride] (elements of `dtype`; one of the strides is 1) -> codes, scales, every
- * byte of both written.  Any sizes. */
+ * byte of both written.  Any sizes up to 2^30 rows and 33553920 columns. */
 int ffnk_mxfp4_quantize(const void* x, int dtype, int64_t row_stride, int64_t col_stride, int64_t rows, int64_t cols,
                         void* codes, void* scales, void* stream);
 /* The inverse: out [rows, ldo] of `dtype`.  Exact in bf16 and fp32; rounded to nearest in fp16. */
