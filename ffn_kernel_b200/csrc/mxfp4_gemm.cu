@@ -10,6 +10,8 @@
 // Epilogues: bf16 rows scattered to token order; or silu(gate) * up, which leaves as MXFP4 again: the 32
 // accumulator columns a lane reads at a time are one block of its row, so the maximum, the scale and the codes
 // need no other lane.
+#include <atomic>
+
 #include "ffnk_internal.h"
 #include "mxfp4.cuh"
 #include "ptx.cuh"
@@ -520,6 +522,278 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
 }
 
 // ---------------------------------------------------------------------------------------------
+// Few row tiles: bound by the stream of weights, or by latency.  A cluster of up to eight CTAs owns one tile of 128 rows
+// x 128 weight rows of one matrix (gate/up: of both, a CTA takes one of them), the contraction cut into `splits` ranges.
+// Every CTA leaves its fp32 partial tile in its own shared memory; after a cluster-wide barrier each CTA adds up a share
+// of the rows out of its peers' shared memory, range by range in order (the same bits whichever CTA is last), and
+// stores them: bf16 rows in token order, or silu(gate) * up in MXFP4 (a lane holds 4 columns, eight lanes a block).
+// Two CTAs fit on an SM (about 100 KiB and 256 tensor-memory columns each), so that one loads while the other adds up.
+//
+// The weights do not depend on the kernel before this one: launched with programmatic stream serialization, a CTA
+// counts the mask itself, asks for its first stages of weights, and only then waits for the activations.
+// ---------------------------------------------------------------------------------------------
+constexpr int MXS_N = 128;
+constexpr int MXS_THREADS = 192;
+constexpr int MXS_B_BYTES = MXS_N * 128;                    // 16 KiB
+constexpr int MXS_STAGE_FIXED = MXS_B_BYTES + 2 * MX_SF_BYTES;
+constexpr int MXS_MAX_STAGES = 6;
+constexpr int MXS_SMEM_STAGES = 104 * 1024;                 // stages, later the partial tile (at most 64 KiB)
+constexpr int MXS_SMEM = MXS_SMEM_STAGES + 256 + 1024;
+constexpr int MXS_MASK_MAX = 4096;                          // tokens a CTA counts itself
+constexpr uint32_t MXS_SFA = 128, MXS_SFB = 136;            // tensor-memory columns of the scales, behind the accumulator
+
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+struct MxSmall {
+  const uint8_t* mask;    // null: M is larger than a CTA counts
+  int M;
+  int splits;             // ranges of the contraction; the cluster has splits (gate/up: 2 x splits) CTAs
+  int a_slot;             // bytes of a stage's A rows (a multiple of 1 KiB; what the MMA reads past them is B, in rows nobody stores)
+  int stages;
+};
+
+template <bool GLU>
+__global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_constant__ MxMaps maps, const MxParams p, const MxSmall q) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + MXS_SMEM_STAGES);
+  uint64_t* empty = full + MXS_MAX_STAGES;
+  uint64_t* done = empty + MXS_MAX_STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int csize = GLU ? 2 * q.splits : q.splits;
+  const int split = GLU ? rank >> 1 : rank, up = GLU ? rank & 1 : 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < MXS_MAX_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(tmem_slot, 256);
+    tmem_relinquish<1>();
+  }
+  griddep_launch_dependents();
+
+  // rows of each modality: counted here, or read from what the kernel before left
+  int Mv;
+  if (q.mask) {
+    int n = 0;
+    for (int i = threadIdx.x; i < q.M; i += MXS_THREADS) n += q.mask[i] != 0 ? 1 : 0;
+    n = __reduce_add_sync(0xFFFFFFFFu, n);
+    int* s_count = reinterpret_cast<int*>(const_cast<int*>(abort_flag) + 1);
+    if (lane == 0) s_count[warp] = n;
+    tc_fence_before();
+    __syncthreads();
+    Mv = 0;
+    for (int i = 0; i < MXS_THREADS / 32; ++i) Mv += s_count[i];
+  } else {
+    tc_fence_before();
+    __syncthreads();
+    griddep_wait();
+    Mv = p.counts[0];
+  }
+  tc_fence_after();
+  const int Mt = q.M - Mv;
+  const uint32_t tmem = *tmem_slot;
+  const int tiles_v = (Mv + MX_BM - 1) / MX_BM;
+  const int m_tiles = tiles_v + (Mt + MX_BM - 1) / MX_BM;
+  const int n_tiles = (p.n_out + MXS_N - 1) / MXS_N;
+  const int t = blockIdx.x / csize;                       // the same in the whole cluster
+  const bool work = t < m_tiles * n_tiles;
+  const int nt = work ? t / m_tiles : 0;
+  const int mt = work ? t - nt * m_tiles : 0;
+  const bool text = mt >= tiles_v;
+  const int row0 = (text ? mt - tiles_v : mt) * MX_BM;
+  const int rows = work ? min(MX_BM, (text ? Mt : Mv) - row0) : 0;
+  const int routed0 = (text ? mx_text_base(Mv) : 0) + row0;
+  const int k_steps = (p.k_bytes + 127) / 128;
+  const int ks0 = split * k_steps / q.splits, ks1 = work ? (split + 1) * k_steps / q.splits : ks0;
+  const int stage_bytes = q.a_slot + MXS_STAGE_FIXED;
+
+  if (warp == 0) {
+    const bool lead = elect_one();
+    const CUtensorMap* mb = &maps.b[(text ? 2 : 0) + up];
+    const CUtensorMap* msb = &maps.sb[(text ? 2 : 0) + up];
+    const uint32_t bytes = p.a_rows * 128 + MXS_STAGE_FIXED;
+    int issued = 0;
+    auto load_b = [&](int ks, int stage) {
+      uint8_t* b = smem + stage * stage_bytes + q.a_slot;
+      mbar_arrive_expect_tx(&full[stage], bytes);
+      tma_load_2d(b, mb, &full[stage], ks * 128, nt * MXS_N);
+      tma_load_2d(b + MXS_B_BYTES + MX_SF_BYTES, msb, &full[stage], ks * 256, nt);
+    };
+    auto load_a = [&](int ks, int stage) {
+      uint8_t* a = smem + stage * stage_bytes;
+      tma_load_2d(a, &maps.a, &full[stage], ks * 128, routed0);
+      tma_load_2d(a + q.a_slot + MXS_B_BYTES, &maps.sa, &full[stage], ks * 256, routed0 >> 7);
+    };
+    const int ahead = min(q.stages, ks1 - ks0);
+    if (lead)
+      for (int i = 0; i < ahead; ++i) load_b(ks0 + i, i);
+    griddep_wait();                                       // the activations are there from here on
+    if (lead)
+      for (int i = 0; i < ahead; ++i) load_a(ks0 + i, i);
+    __syncwarp();
+    issued = ahead;
+    int stage = 0;
+    uint32_t phase = 0;
+    if (ahead == q.stages) phase = 1;
+    else stage = ahead;
+    for (int ks = ks0 + ahead; ks < ks1; ++ks) {
+      if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag)) {
+        if (lead) mx_report(p.status, ST_TIMEOUT_PRODUCER);
+        break;
+      }
+      if (lead) {
+        load_b(ks, stage);
+        load_a(ks, stage);
+      }
+      __syncwarp();
+      ++issued;
+      if (++stage == q.stages) { stage = 0; phase ^= 1; }
+    }
+    if (*abort_flag && lead) {
+      for (int i = 0; i < (issued < q.stages ? issued : q.stages); ++i) {
+        if (--stage < 0) { stage = q.stages - 1; phase ^= 1; }
+        int dummy = 0;
+        mbar_wait(&full[stage], phase, &dummy, 1000000ull);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    const bool lead = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int ks = ks0; ks < ks1; ++ks) {
+      if (!mbar_wait_warp(&full[stage], phase, abort_flag)) {
+        if (lead) mx_report(p.status, ST_TIMEOUT_MMA_FULL);
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t a = smem_u32(smem + stage * stage_bytes);
+      const uint32_t b = a + q.a_slot;
+      const uint32_t sa = b + MXS_B_BYTES;
+      const int left = p.k_bytes - ks * 128;
+      const int mmas = left >= 128 ? 4 : (left + 31) / 32;
+      if (lead) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (2 * j < mmas) {
+            tmem_copy_scales<1>(tmem + MXS_SFA + 4 * j, sa + j * kMxAtomBytes);
+            tmem_copy_scales<1>(tmem + MXS_SFB + 4 * j, sa + MX_SF_BYTES + j * kMxAtomBytes);
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if (kk < mmas)
+            umma_mxf4<1>(tmem, umma_smem_desc(a + kk * 32, 16, 1024), umma_smem_desc(b + kk * 32, 16, 1024),
+                         mx_idesc(MX_BM, MXS_N, (kk & 1) * 2), tmem + MXS_SFA + 4 * (kk >> 1), tmem + MXS_SFB + 4 * (kk >> 1),
+                         ks > ks0 || kk != 0 ? 1u : 0u);
+        }
+        umma_commit(&empty[stage]);
+      }
+      __syncwarp();
+      if (++stage == q.stages) { stage = 0; phase ^= 1; }
+    }
+    if (lead && ok) umma_commit(done);
+    __syncwarp();
+  } else {
+    // the partial tile to shared memory, [row][32 pieces of four columns], pieces XOR-swizzled by the row
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    if (quarter * 32 < rows) {
+      if (!mbar_wait_warp(done, 0, abort_flag)) {
+        if (lane == 0) mx_report(p.status, ST_TIMEOUT_EPILOGUE);
+      } else {
+        tc_fence_after();
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld_32x32(taddr + c * 32, v);
+          tmem_ld_wait();
+          if (row < rows) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(smem + row * 512 + (((c * 8 + j) ^ (row & 31)) << 4)) =
+                  make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+        }
+      }
+    }
+  }
+  griddep_wait();                                         // every thread: perm is read below
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                     // every partial tile of the cluster is in place
+
+  for (int row = rank + csize * warp; row < rows; row += csize * (MXS_THREADS / 32)) {
+    const uint32_t mine = smem_u32(smem + row * 512 + ((lane ^ (row & 31)) << 4));
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < csize) {
+        const float4 v = ld_cluster(mapa_shared(mine, i));
+        float4& d = GLU && (i & 1) ? u : g;
+        d.x += v.x; d.y += v.y; d.z += v.z; d.w += v.w;
+      }
+    }
+    const int n0 = nt * MXS_N + lane * 4;
+    if constexpr (!GLU) {
+      if (n0 < p.n_out) {
+        const int64_t token = p.perm[(text ? p.counts[2] : 0) + row0 + row];
+        *reinterpret_cast<uint2*>(p.out + token * p.ldo + n0) = make_uint2(mx_pack_bf16(g.x, g.y), mx_pack_bf16(g.z, g.w));
+      }
+    } else {
+      const int64_t drow = routed0 + row;
+      if (p.t1 && n0 < p.n_out) {
+        const int64_t o = pre_tile_offset(drow, n0, p.n_out);
+        *reinterpret_cast<float4*>(p.t1 + o) = g;
+        *reinterpret_cast<float4*>(p.t3 + o) = u;
+      }
+      float v[8] = {};
+      if (n0 < p.n_out) {
+        v[0] = mx_silu_mul(g.x, u.x);
+        v[1] = mx_silu_mul(g.y, u.y);
+        v[2] = mx_silu_mul(g.z, u.z);
+        v[3] = mx_silu_mul(g.w, u.w);
+      }
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      const uint32_t byte = mx_scale_byte(m);
+      const float inv = mx_inverse_scale(byte);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] *= inv;
+      const uint32_t code = byte == 255u ? 0u : mx_pack8(v);
+      const int block = nt * 4 + (lane >> 3);
+      if (block * 32 < p.n_out) *reinterpret_cast<uint16_t*>(p.codes + drow * p.code_ld + block * 16 + (lane & 7) * 2) = static_cast<uint16_t>(code);
+      if ((lane & 7) == 0) p.scales[mx_scale_word(drow, nt, p.k_atoms_out) + (lane >> 3)] = static_cast<uint8_t>(byte);
+    }
+  }
+  cluster_sync_all();                                     // nobody leaves while a peer still reads its shared memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, 256);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
 struct MxWeight {
@@ -552,13 +826,26 @@ static bool mx_pairs(int64_t M) {
   return forced >= 0 ? forced != 0 : M >= 2048;
 }
 
+// Dynamic shared memory of a kernel, allowed once per device (the driver keeps the attribute).
+template <class K>
+static int mx_allow_smem(K kernel, int bytes, std::atomic<uint64_t>& allowed) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (allowed.load(std::memory_order_relaxed) & bit)) return 0;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) allowed.fetch_or(bit, std::memory_order_relaxed);
+  return cuda_status(e);
+}
+
 template <int EPI, int CTAS>
 static int mx_launch_as(const MxMaps& maps, const MxParams& p, int64_t M, cudaStream_t stream) {
   const int n_per_tile = mx_glu(EPI) ? MX_BN / 2 : MX_BN;
   int64_t units = ((M + MX_BM * CTAS - 1) / (MX_BM * CTAS) + 1) * ((p.n_out + n_per_tile - 1) / n_per_tile);
   if (units > usable_sms() / CTAS) units = usable_sms() / CTAS;
-  const cudaError_t e = cudaFuncSetAttribute(mx_gemm_kernel<EPI, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, MxGeom<CTAS>::smem);
-  if (e != cudaSuccess) return cuda_status(e);
+  static std::atomic<uint64_t> allowed{0};
+  if (const int r = mx_allow_smem(mx_gemm_kernel<EPI, CTAS>, MxGeom<CTAS>::smem, allowed)) return r;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(units * CTAS));
   cfg.blockDim = dim3(MX_THREADS);
@@ -580,17 +867,65 @@ static int mx_launch(const MxMaps& maps, const MxParams& p, int64_t M, bool pair
   return pairs ? mx_launch_as<EPI, 2>(maps, p, M, stream) : mx_launch_as<EPI, 1>(maps, p, M, stream);
 }
 
+// The small kernel takes a problem whose 128 x 128 tiles (both matrices of a gate/up pair counted) leave it to be split
+// over two CTAs an SM; the number of ranges is the largest power of two that fits, with at least `kMxMinSteps` k-steps each.
+constexpr int kMxMinSteps = 2;
+static int mx_small_splits(int64_t M, int64_t n_out, int64_t k, bool glu) {
+  const int forced = tune_overrides().narrow;
+  if (forced == 0) return 0;
+  const int64_t m_tiles = M <= 1 ? 1 : (M + MX_BM - 1) / MX_BM + (M <= MX_BM ? 1 : 0);
+  const int64_t tiles = m_tiles * ((n_out + MXS_N - 1) / MXS_N) * (glu ? 2 : 1);
+  const int64_t slots = 2 * usable_sms();
+  const int64_t steps = (mx_code_ld(k) + 127) / 128;
+  if (M > 512 && forced < 0) return 0;
+  int splits = 1;
+  while (2 * splits * (glu ? 2 : 1) <= 8 && tiles * splits * 2 <= slots && steps / (splits * 2) >= kMxMinSteps) splits *= 2;
+  return splits;
+}
+
+template <bool GLU>
+static int mx_launch_small(const MxMaps& maps, const MxParams& p, int64_t M, const void* mask, int splits, cudaStream_t stream) {
+  if (device_info().cc_major != 10) return FFNK_ERR_DEVICE;
+  MxSmall q{};
+  q.mask = M <= MXS_MASK_MAX ? static_cast<const uint8_t*>(mask) : nullptr;
+  q.M = static_cast<int>(M);
+  q.splits = splits;
+  q.a_slot = (p.a_rows * 128 + 1023) & ~1023;
+  q.stages = MXS_SMEM_STAGES / (q.a_slot + MXS_STAGE_FIXED);
+  if (q.stages > MXS_MAX_STAGES) q.stages = MXS_MAX_STAGES;
+  const int csize = GLU ? 2 * splits : splits;
+  const int64_t tiles = ((M + MX_BM - 1) / MX_BM + (M > 1 ? 1 : 0)) * ((p.n_out + MXS_N - 1) / MXS_N);
+  static std::atomic<uint64_t> allowed{0};
+  if (const int r = mx_allow_smem(mx_small_kernel<GLU>, MXS_SMEM, allowed)) return r;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * csize));
+  cfg.blockDim = dim3(MXS_THREADS);
+  cfg.dynamicSmemBytes = MXS_SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = csize;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cuda_status(cudaLaunchKernelEx(&cfg, mx_small_kernel<GLU>, maps, p, q));
+}
+
 // y[token] = routed rows of (codes, scales) by the modality's weight [N, K]
 static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt, const int32_t* perm, const int32_t* counts,
-                      void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int32_t* status, cudaStream_t s) {
+                      const void* mask, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int32_t* status, cudaStream_t s) {
   MxMaps m;
   int r;
   const int64_t rows = ffnk_route_capacity(M) + 512;
   if ((r = mx_maps(&m.a, &m.sa, a, rows, K, mx_a_box_rows(M), 1))) return r;
   const bool pairs = mx_pairs(M);
-  const int box = pairs ? MX_BN / 2 : MX_BN;
-  if ((r = mx_maps(&m.b[0], &m.sb[0], wv, N, K, box, 2))) return r;
-  if ((r = mx_maps(&m.b[2], &m.sb[2], wt, N, K, box, 2))) return r;
+  const int splits = mx_small_splits(M, N, K, false);
+  const int box = splits ? MXS_N : pairs ? MX_BN / 2 : MX_BN, atoms = splits ? 1 : 2;
+  if ((r = mx_maps(&m.b[0], &m.sb[0], wv, N, K, box, atoms))) return r;
+  if ((r = mx_maps(&m.b[2], &m.sb[2], wt, N, K, box, atoms))) return r;
   m.b[1] = m.b[0]; m.b[3] = m.b[2]; m.sb[1] = m.sb[0]; m.sb[3] = m.sb[2];
   MxParams p{};
   p.perm = perm; p.counts = counts; p.status = status; p.prof = debug_profile_buffer();
@@ -600,12 +935,12 @@ static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt,
   p.group_m = mx_group_m(K, pairs ? 2 * MX_BM : MX_BM);
   p.out = static_cast<__nv_bfloat16*>(y);
   p.ldo = ldy;
-  return mx_launch<MX_EPI_STORE>(m, p, M, pairs, s);
+  return splits ? mx_launch_small<false>(m, p, M, mask, splits, s) : mx_launch<MX_EPI_STORE>(m, p, M, pairs, s);
 }
 
 // quantised silu(gate) * up of the routed rows, optionally with the pre-activations kept (t1, t3 both or neither)
 static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* perm, const int32_t* counts, void* codes,
-                     void* scales, void* t1, void* t3, int64_t M, int64_t d, int64_t h, int32_t* status, cudaStream_t s) {
+                     void* scales, const void* mask, void* t1, void* t3, int64_t M, int64_t d, int64_t h, int32_t* status, cudaStream_t s) {
   MxMaps m;
   int r;
   const int64_t rows = ffnk_route_capacity(M) + 512;
@@ -625,6 +960,7 @@ static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* p
   p.k_atoms_out = static_cast<int>(mx_k_atoms(h));
   p.t1 = static_cast<float*>(t1);
   p.t3 = static_cast<float*>(t3);
+  if (const int splits = mx_small_splits(M, h, d, true)) return mx_launch_small<true>(m, p, M, mask, splits, s);
   return t1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, pairs, s) : mx_launch<MX_EPI_GLU>(m, p, M, pairs, s);
 }
 
@@ -678,7 +1014,7 @@ extern "C" int ffnk_mxfp4_linear_forward(const void* x, int64_t ldx, const void*
   int r = mx_route_quantize(mask, M, x, ldx, K, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
   if (r) return r;
   return mx_product(MxWeight{ws + w.xc, ws + w.xs}, MxWeight{b1_codes, b1_scales}, MxWeight{b2_codes, b2_scales}, perm, counts,
-                    y, ldy, M, N, K, status, static_cast<cudaStream_t>(stream));
+                    mask, y, ldy, M, N, K, status, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* const* codes, const void* const* scales,
@@ -702,9 +1038,9 @@ extern "C" int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* co
   int r = mx_route_quantize(mask, M, x, ldx, d, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
   if (r) return r;
   const MxWeight gu[4] = {{codes[0], scales[0]}, {codes[2], scales[2]}, {codes[3], scales[3]}, {codes[5], scales[5]}};
-  if ((r = mx_gateup(MxWeight{ws + w.xc, ws + w.xs}, gu, perm, counts, ws + w.hc, ws + w.hs, t1, t3, M, d, h, status, s))) return r;
-  return mx_product(MxWeight{ws + w.hc, ws + w.hs}, MxWeight{codes[1], scales[1]}, MxWeight{codes[4], scales[4]}, perm, counts, y,
-                    ldy, M, d, h, status, s);
+  if ((r = mx_gateup(MxWeight{ws + w.xc, ws + w.xs}, gu, perm, counts, ws + w.hc, ws + w.hs, mask, t1, t3, M, d, h, status, s))) return r;
+  return mx_product(MxWeight{ws + w.hc, ws + w.hs}, MxWeight{codes[1], scales[1]}, MxWeight{codes[4], scales[4]}, perm, counts, mask,
+                    y, ldy, M, d, h, status, s);
 }
 
 // ---------------------------------------------------------------------------------------------

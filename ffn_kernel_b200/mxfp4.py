@@ -42,28 +42,29 @@ class MXFP4Tensor:
     scales  uint8 [ceil(rows / 128), ceil(cols / 128), 32, 4, 4]; 2^(byte - 127) of (row r, block b) sits at
             [r // 128, b // 4, r % 32, r % 128 // 32, b % 4]; entries without a row or block are 0
     """
-    __slots__ = ("codes", "scales", "rows", "cols")
+    __slots__ = ("codes", "scales", "rows", "cols", "device", "ptrs")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
         want_c, want_s = (rows, -(-cols // 32) * 16), (-(-rows // 128), -(-cols // 128), 32, 4, 4)
         for t, want, name in ((codes, want_c, "codes"), (scales, want_s, "scales")):
-            _require_cuda(t, name)
-            if t.dtype != torch.uint8 or tuple(t.shape) != want:
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise RuntimeError(f"{name} must be a CUDA tensor; this package has no CPU path")
+            if t.dtype != torch.uint8 or t.shape != want:
                 raise RuntimeError(f"{name} of a [{rows}, {cols}] MXFP4 matrix must be torch.uint8 {list(want)}, "
                                    f"got {t.dtype} {list(t.shape)}")
-            if not t.is_contiguous() or t.data_ptr() % 16:
-                raise RuntimeError(f"{name} must be contiguous and 16-byte aligned")
-        if codes.device != scales.device:
-            raise RuntimeError("codes and scales must be on the same device")
+            if not t.is_contiguous():
+                raise RuntimeError(f"{name} must be contiguous")
         self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+        self.device = codes.device
+        self.ptrs = (codes.data_ptr(), scales.data_ptr())
+        if scales.device != self.device:
+            raise RuntimeError("codes and scales must be on the same device")
+        if (self.ptrs[0] | self.ptrs[1]) & 15:
+            raise RuntimeError("codes and scales must be 16-byte aligned")
 
     @property
     def shape(self):
         return (self.rows, self.cols)
-
-    @property
-    def device(self):
-        return self.codes.device
 
     def __repr__(self):
         return f"MXFP4Tensor([{self.rows}, {self.cols}], device={self.codes.device})"
@@ -79,20 +80,19 @@ def quantize_mxfp4(x: torch.Tensor, dim: int = 1) -> MXFP4Tensor:
         raise RuntimeError(f"x must be torch.bfloat16, torch.float16 or torch.float32, got {x.dtype}")
     if dim not in (0, 1, -1, -2):
         raise RuntimeError(f"dim must be 0 or 1, got {dim}")
-    if dim in (0, -2):
-        x = x.T
-    x = x.detach()
     rows, cols = x.shape
-    if max(rows, cols) >= 1 << 30:
-        raise RuntimeError(f"x is too large: {tuple(x.shape)}")
-    if not (x.stride(1) == 1 or cols == 1 or x.stride(0) == 1 or rows == 1) or min(x.stride()) < 0:
+    rs, cs = x.stride()
+    if not (cs == 1 or cols == 1 or rs == 1 or rows == 1):
         x = x.contiguous()
+        rs, cs = cols, 1
+    if dim in (0, -2):
+        rows, cols, rs, cs = cols, rows, cs, rs
     dev = x.device
     with _on(dev):
         codes = torch.empty((rows, -(-cols // 32) * 16), dtype=torch.uint8, device=dev)
         scales = torch.empty((-(-rows // 128), -(-cols // 128), 32, 4, 4), dtype=torch.uint8, device=dev)
         check("ffnk_mxfp4_quantize", lib().ffnk_mxfp4_quantize(
-            x.data_ptr(), _DTYPES[x.dtype], x.stride(0), x.stride(1), rows, cols, codes.data_ptr(), scales.data_ptr(),
+            x.data_ptr(), _DTYPES[x.dtype], rs, cs, rows, cols, codes.data_ptr(), scales.data_ptr(),
             stream_ptr(dev)))
     return MXFP4Tensor(codes, scales, rows, cols)
 
@@ -103,11 +103,11 @@ def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> tor
         raise RuntimeError(f"q must be an MXFP4Tensor, got {type(q).__name__}")
     if dtype not in _DTYPES:
         raise RuntimeError(f"dtype must be torch.bfloat16, torch.float16 or torch.float32, got {dtype}")
-    dev = q.codes.device
+    dev = q.device
     with _on(dev):
         out = torch.empty((q.rows, q.cols), dtype=dtype, device=dev)
         check("ffnk_mxfp4_dequantize", lib().ffnk_mxfp4_dequantize(
-            q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols, out.data_ptr(), _DTYPES[dtype], q.cols, stream_ptr(dev)))
+            *q.ptrs, q.rows, q.cols, out.data_ptr(), _DTYPES[dtype], q.cols, stream_ptr(dev)))
     return out
 
 
@@ -117,7 +117,7 @@ def _check_weights(ws, names, shapes, dev):
             raise RuntimeError(f"{n} must be an MXFP4Tensor, got {type(w).__name__}")
         if (w.rows, w.cols) != s:
             raise RuntimeError(f"{n} must have shape {list(s)} ([out, in]), got [{w.rows}, {w.cols}]")
-        if w.codes.device != dev:
+        if w.device != dev:
             raise RuntimeError(f"{n} must be on the same device as the activations")
 
 
@@ -129,15 +129,22 @@ def _check_mask(mask, M, dev):
     return mask.contiguous()
 
 
-def _lists(M, dev):
-    """Routing lists of one call: perm int32 [2 * cap], counts int32 [8], in one allocation."""
+def _scratch(nbytes, M, dev, keep: bool):
+    """Workspace and routing lists (perm int32 [2 * cap], counts int32 [8]) of one call -> (tensors to hold, workspace,
+    perm, counts).  Inference takes one allocation for both; a backward pass wants the lists alone."""
     cap = (M + 127) // 128 * 128
-    t = torch.empty(2 * cap + 8, dtype=torch.int32, device=dev)
-    return t, t.data_ptr(), t.data_ptr() + 8 * cap
+    if keep:
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        lists = torch.empty(2 * cap + 8, dtype=torch.int32, device=dev)
+        p = lists.data_ptr()
+        return ws, lists, ws.data_ptr(), p, p + 8 * cap
+    ws = torch.empty(nbytes + 8 * cap + 32, device=dev, dtype=torch.uint8)
+    p = ws.data_ptr()
+    return ws, None, p, p + nbytes, p + nbytes + 8 * cap
 
 
-def _mxfp4_linear_forward(a, b1, b2, mask):
-    """y[m] = Q(a[m]) @ (b1 if mask[m] else b2).T -> (y [M, N] bf16, routing lists)."""
+def _mxfp4_linear_forward(a, b1, b2, mask, keep: bool = False):
+    """y[m] = Q(a[m]) @ (b1 if mask[m] else b2).T -> (y [M, N] bf16, routing lists if ``keep``)."""
     a = _activation(a, "a")
     M, K = a.shape
     dev = a.device
@@ -147,16 +154,14 @@ def _mxfp4_linear_forward(a, b1, b2, mask):
     mask = _check_mask(mask, M, dev)
     L = lib()
     with _on(dev):
-        y = torch.empty((M, N), device=dev, dtype=torch.bfloat16)
+        y = a.new_empty((M, N))
         if M == 0:
             return y, None
-        lists, perm, counts = _lists(M, dev)
         nbytes = L.ffnk_mxfp4_workspace_bytes(M, K, 0)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
         check("ffnk_mxfp4_linear_forward", L.ffnk_mxfp4_linear_forward(
-            a.data_ptr(), a.stride(0), b1.codes.data_ptr(), b1.scales.data_ptr(), b2.codes.data_ptr(), b2.scales.data_ptr(),
-            mask.data_ptr(), perm, counts, ws.data_ptr(), nbytes, y.data_ptr(), N, M, N, K, status_word(dev).data_ptr(),
-            stream_ptr(dev)))
+            a.data_ptr(), a.stride(0), *b1.ptrs, *b2.ptrs, mask.data_ptr(), perm, counts, wp, nbytes, y.data_ptr(), N, M, N, K,
+            status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return y, lists
 
@@ -175,7 +180,7 @@ def _mxfp4_linear_backward(g, b1, b2, lists):
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         perm = lists.data_ptr()
         check("ffnk_mxfp4_linear_backward", L.ffnk_mxfp4_linear_backward(
-            g.data_ptr(), g.stride(0), b1.codes.data_ptr(), b1.scales.data_ptr(), b2.codes.data_ptr(), b2.scales.data_ptr(),
+            g.data_ptr(), g.stride(0), *b1.ptrs, *b2.ptrs,
             perm, perm + 4 * (lists.numel() - 8), ws.data_ptr(), nbytes, dx.data_ptr(), K, M, N, K,
             status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
@@ -196,18 +201,17 @@ def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
     mask = _check_mask(mask, M, dev)
     L = lib()
     with _on(dev):
-        y = torch.empty((M, d), device=dev, dtype=torch.bfloat16)
+        y = x.new_empty((M, d))
         if M == 0:
             return y, (None, None, None)
-        lists, perm, counts = _lists(M, dev)
         nbytes = L.ffnk_mxfp4_workspace_bytes(M, d, h)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
         t1 = t3 = None
         if keep:
             t1, t3 = (torch.empty(((M + 127) // 128 * 128 + 512) * h, device=dev, dtype=torch.float32) for _ in range(2))
         check("ffnk_mxfp4_ffn_forward", L.ffnk_mxfp4_ffn_forward(
-            x.data_ptr(), x.stride(0), _Six(*[w.codes.data_ptr() for w in ws6]), _Six(*[w.scales.data_ptr() for w in ws6]),
-            mask.data_ptr(), perm, counts, ws.data_ptr(), nbytes, t1.data_ptr() if keep else None,
+            x.data_ptr(), x.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]),
+            mask.data_ptr(), perm, counts, wp, nbytes, t1.data_ptr() if keep else None,
             t3.data_ptr() if keep else None, y.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return y, (lists, t1, t3)
@@ -228,8 +232,7 @@ def _mxfp4_ffn_backward(gy, ws6, saved):
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         perm = lists.data_ptr()
         check("ffnk_mxfp4_ffn_backward", L.ffnk_mxfp4_ffn_backward(
-            gy.data_ptr(), gy.stride(0), _Six(*[w.codes.data_ptr() for w in ws6]),
-            _Six(*[w.scales.data_ptr() for w in ws6]), t1.data_ptr(), t3.data_ptr(), perm, perm + 4 * (lists.numel() - 8),
+            gy.data_ptr(), gy.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), t1.data_ptr(), t3.data_ptr(), perm, perm + 4 * (lists.numel() - 8),
             ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return dx
@@ -251,7 +254,7 @@ class MXFP4MaskedLinear(Function):
 
     @staticmethod
     def forward(ctx, a, b1, b2, mask):
-        y, ctx.lists = _mxfp4_linear_forward(a, b1, b2, mask)
+        y, ctx.lists = _mxfp4_linear_forward(a, b1, b2, mask, keep=True)
         ctx.weights = (b1, b2)
         return y
 

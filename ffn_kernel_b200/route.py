@@ -23,7 +23,13 @@ def _require_cuda(t: torch.Tensor, name: str) -> None:
         raise RuntimeError(f"{name} must be a CUDA tensor; this package has no CPU path")
 
 
+# the current stream's handle without building a Stream object (2 us of a call); torch's public form where it is missing
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device) -> int:
+    if _raw_stream is not None and getattr(device, "index", None) is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
