@@ -27,37 +27,45 @@ __host__ __device__ constexpr uint32_t mx_idesc(int m, int n, uint32_t sf) {
   return (sf << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
          (static_cast<uint32_t>(m >> 7) << 27) | (sf << 29);
 }
+// Descriptors are kept as their low word, (address >> 4) | leading offset << 16, and a constant high word, so that a
+// step of the loop is one 32-bit addition; everything an instruction needs is computed outside the branch of the
+// electing lane, where the compiler can use uniform registers.
+constexpr uint32_t MX_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);      // operands: 8-row groups 1 KiB apart, 128-byte swizzle
+constexpr uint32_t MX_SCALE_DESC_HI = (128u >> 4) | (1u << 14);              // scale atoms: 8-row groups 128 bytes apart, no swizzle
+__device__ __forceinline__ uint32_t mx_desc_lo(uint32_t smem) { return ((smem & 0x3FFFFu) >> 4) | (1u << 16); }
+
 template <int CTAS>
-__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t sfa,
-                                          uint32_t sfb, uint32_t accumulate) {
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                          uint32_t accumulate) {
   if constexpr (CTAS == 1)
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %7};\n\tmov.b64 db, {%2, %7};\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
-        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(MX_DESC_HI)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %7};\n\tmov.b64 db, {%2, %7};\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
-        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(MX_DESC_HI)
         : "memory");
 }
 // One scale atom (512 consecutive bytes: 32 rows of 16 bytes) from shared memory to four tensor-memory columns,
 // the same 32 lanes in all four lane quarters.  In issue order with the MMAs of the same thread.
 template <int CTAS>
-__device__ __forceinline__ void tmem_copy_scales(uint32_t tmem, uint32_t smem) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem & 0x3FFFFu) >> 4);
-  d |= 1ull << 16;      // leading offset: unused, one 16-byte column
-  d |= 8ull << 32;      // 128 bytes between groups of eight rows
-  d |= 1ull << 46;      // descriptor version for sm_100; no swizzle
+__device__ __forceinline__ void tmem_copy_scales(uint32_t tmem, uint32_t lo) {
   if constexpr (CTAS == 1)
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+    asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\ttcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n\t}" ::"r"(tmem),
+                 "r"(lo), "r"(MX_SCALE_DESC_HI)
+                 : "memory");
   else
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+    asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\ttcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n\t}" ::"r"(tmem),
+                 "r"(lo), "r"(MX_SCALE_DESC_HI)
+                 : "memory");
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -186,9 +194,24 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
   return r != 0;
 }
+// Has the phase completed?  Never blocks (a try_wait may sleep for microseconds on a stage that is not coming).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
 // the same bounded wait for all lanes of a warp
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag));
+}
+
+// Arrival at another CTA's barrier that hands over tensor memory only (tcgen05 fences order that).  A release at
+// cluster scope would first wait for this thread's global stores, the rows of the tile before: 1800 cycles a tile.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 __device__ __forceinline__ void mx_report(int* status, int code) {
@@ -202,16 +225,26 @@ constexpr uint32_t MX_ACC1 = 224;
 constexpr uint32_t MX_SFA = 480;      // 2 atoms x 4 columns
 constexpr uint32_t MX_SFB = 488;      // 2 atoms x 8 columns (256 weight rows)
 
-// Scales of one k-step from shared memory to tensor memory.  sa: the A atoms [2]; sb: the B atoms [row atom][2].
-template <int CTAS>
-__device__ __forceinline__ void mx_copy_step_scales(uint32_t tmem, uint32_t sa, uint32_t sb, int atoms) {
+// The instructions of one k-step: scales to tensor memory, four MMAs of 64 values.  lo words of the A and B codes, of
+// the A scales [2 atoms] and the B scales [row atom][2 atoms].  `mmas` < 4: the contraction ends inside the step, and
+// nothing is issued past its last scale atom.
+constexpr uint32_t kAtomLo = kMxAtomBytes >> 4;
+template <int CTAS, int TILE_M>
+__device__ __forceinline__ void mx_issue_step(uint32_t d, uint32_t tmem, uint32_t a, uint32_t b, uint32_t sa, uint32_t sb, int mmas,
+                                              uint32_t accumulate) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    if (j < atoms) {
-      tmem_copy_scales<CTAS>(tmem + MX_SFA + 4 * j, sa + j * kMxAtomBytes);
-      tmem_copy_scales<CTAS>(tmem + MX_SFB + 8 * j, sb + j * kMxAtomBytes);
-      tmem_copy_scales<CTAS>(tmem + MX_SFB + 8 * j + 4, sb + MX_SF_BYTES + j * kMxAtomBytes);
+    if (2 * j < mmas) {
+      tmem_copy_scales<CTAS>(tmem + MX_SFA + 4 * j, sa + j * kAtomLo);
+      tmem_copy_scales<CTAS>(tmem + MX_SFB + 8 * j, sb + j * kAtomLo);
+      tmem_copy_scales<CTAS>(tmem + MX_SFB + 8 * j + 4, sb + (2 + j) * kAtomLo);
     }
+  }
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    if (kk < mmas)
+      umma_mxf4<CTAS>(d, a + kk * 2, b + kk * 2, mx_idesc(TILE_M, MX_BN, (kk & 1) * 2), tmem + MX_SFA + 4 * (kk >> 1),
+                      tmem + MX_SFB + 8 * (kk >> 1), kk == 0 ? accumulate : 1u);
   }
 }
 
@@ -219,12 +252,10 @@ __device__ __forceinline__ void mx_copy_step_scales(uint32_t tmem, uint32_t sa, 
 // first chunk has been read (the chunk holding the columns the two accumulators share, for the part that has it).
 template <int EPI, class F>
 __device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, const MxTile& tc, int acc, int row, int part,
-                                            uint8_t* stg, int lane, F&& on_first) {
+                                            unsigned long long dst, uint8_t* stg, int lane, F&& on_first) {
   const bool valid = row < tc.rows;
   if constexpr (!mx_glu(EPI)) {
     constexpr int CH = MX_BN / 64;            // 32-column chunks per part
-    unsigned long long dst = 0;
-    if (valid) dst = reinterpret_cast<unsigned long long>(p.out + static_cast<int64_t>(p.perm[tc.list_off + tc.row0 + row]) * p.ldo);
 #pragma unroll 1
     for (int i = 0; i < CH; ++i) {
       // accumulator 0 shares its last chunk, accumulator 1 its first
@@ -425,10 +456,11 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
       bool ok = true;
       const bool lead = elect_one();
       const long long t_begin = clock64();
-      long long t_full = 0, t_tmem = 0;
+      long long t_tmem = 0;
+      const uint32_t lo0 = mx_desc_lo(smem_u32(smem));
       for (int t = first; t < total && ok; t += step, ++it) {
         const int acc = it & 1;
-        long long tw = clock64();
+        const long long tw = clock64();
         if (it != 0 && !mbar_wait_warp(tempty, (it - 1) & 1, abort_flag)) {
           if (lead) mx_report(p.status, ST_TIMEOUT_MMA_TMEM);
           break;
@@ -436,34 +468,27 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
         t_tmem += clock64() - tw;
         tc_fence_after();
         const uint32_t d = tmem + (acc ? MX_ACC1 : 0);
+        bool ready = mbar_test(&full[stage], phase);
         for (int ks = 0; ks < k_steps; ++ks) {
-          tw = clock64();
-          if (!mbar_wait_warp(&full[stage], phase, abort_flag)) {
+          if (!__all_sync(0xFFFFFFFFu, ready) && !mbar_wait_warp(&full[stage], phase, abort_flag)) {
             if (lead) mx_report(p.status, ST_TIMEOUT_MMA_FULL);
             ok = false;
             break;
           }
-          t_full += clock64() - tw;
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + stage * G::stage_bytes);
-          const uint32_t b = a + MX_A_BYTES;
-          const uint32_t sa = b + G::b_bytes;
-          const int left = p.k_bytes - ks * 128;                       // the contraction may end inside a k-step:
-          const int mmas = left >= 128 ? 4 : (left + 31) / 32;         // no MMA past its last scale atom
+          const uint32_t a = lo0 + stage * (G::stage_bytes >> 4);
+          const uint32_t b = a + (MX_A_BYTES >> 4), sa = b + (G::b_bytes >> 4), sb = sa + (MX_SF_BYTES >> 4);
+          const int left = p.k_bytes - ks * 128;
+          uint64_t* free_bar = &empty[stage];
+          if (++stage == G::stages) { stage = 0; phase ^= 1; }
+          ready = mbar_test(&full[stage], phase);          // asked before the step is issued, looked at after it
           if (lead) {
-            mx_copy_step_scales<CTAS>(tmem, sa, sa + MX_SF_BYTES, (mmas + 1) / 2);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if (kk < mmas)
-                umma_mxf4<CTAS>(d, umma_smem_desc(a + kk * 32, 16, 1024), umma_smem_desc(b + kk * 32, 16, 1024),
-                                mx_idesc(TILE_M, MX_BN, (kk & 1) * 2), tmem + MX_SFA + 4 * (kk >> 1),
-                                tmem + MX_SFB + 8 * (kk >> 1), (ks | kk) != 0 ? 1u : 0u);
-            }
-            if constexpr (CTAS == 2) umma_commit_pair(&empty[stage], 3);
-            else umma_commit(&empty[stage]);
+            if (left >= 128) mx_issue_step<CTAS, TILE_M>(d, tmem, a, b, sa, sb, 4, ks != 0);
+            else mx_issue_step<CTAS, TILE_M>(d, tmem, a, b, sa, sb, (left + 31) / 32, ks != 0);
+            if constexpr (CTAS == 2) umma_commit_pair(free_bar, 3);
+            else umma_commit(free_bar);
           }
           __syncwarp();
-          if (++stage == G::stages) { stage = 0; phase ^= 1; }
         }
         if (ok && lead) {
           if constexpr (CTAS == 2) umma_commit_pair(&tfull[acc], 3);
@@ -473,7 +498,6 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
       }
       if (p.prof && lead) {
         p.prof[blockIdx.x * 8 + 0] = clock64() - t_begin;
-        p.prof[blockIdx.x * 8 + 1] = t_full;
         p.prof[blockIdx.x * 8 + 2] = t_tmem;
         p.prof[blockIdx.x * 8 + 7] = it;
       }
@@ -487,21 +511,25 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
     for (int t = first; t < total; t += step, ++it) {
       const MxTile tc = mx_tile(t, TILE_M, rank * MX_BM, tiles_v, m_tiles, n_tiles, p.group_m, Mv, Mt, cap);
       const int acc = it & 1;
-      int w = 1;
+      // where this lane's row goes, looked up while the tile is still being multiplied: the next tile's MMAs wait for
+      // this epilogue's first chunk
+      unsigned long long dst = 0;
+      if (!mx_glu(EPI) && row < tc.rows)
+        dst = reinterpret_cast<unsigned long long>(p.out + static_cast<int64_t>(p.perm[tc.list_off + tc.row0 + row]) * p.ldo);
       const long long tw = clock64();
-      if (lane == 0) w = mbar_wait(&tfull[acc], (it >> 1) & 1, abort_flag) ? 1 : 0;
+      const bool filled = mbar_wait_warp(&tfull[acc], (it >> 1) & 1, abort_flag);
       t_wait += clock64() - tw;
-      if (!__shfl_sync(0xFFFFFFFFu, w, 0)) {
+      if (!filled) {
         if (lane == 0) mx_report(p.status, ST_TIMEOUT_EPILOGUE);
         break;
       }
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + (acc ? MX_ACC1 : 0);
-      mx_epilogue<EPI>(taddr, p, tc, acc, row, part, staging + (warp - 2) * 2048, lane, [&] {
+      mx_epilogue<EPI>(taddr, p, tc, acc, row, part, dst, staging + (warp - 2) * 2048, lane, [&] {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (CTAS == 2) mbar_arrive_cluster(mapa_shared(smem_u32(tempty), 0));
+          if constexpr (CTAS == 2) mbar_arrive_remote(mapa_shared(smem_u32(tempty), 0));
           else mbar_arrive(tempty);
         }
       });
@@ -674,6 +702,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
     __syncwarp();
   } else if (warp == 1) {
     const bool lead = elect_one();
+    const uint32_t lo0 = mx_desc_lo(smem_u32(smem));
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -684,25 +713,23 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
         break;
       }
       tc_fence_after();
-      const uint32_t a = smem_u32(smem + stage * stage_bytes);
-      const uint32_t b = a + q.a_slot;
-      const uint32_t sa = b + MXS_B_BYTES;
+      const uint32_t a = lo0 + stage * (stage_bytes >> 4);
+      const uint32_t b = a + (q.a_slot >> 4), sa = b + (MXS_B_BYTES >> 4), sb = sa + (MX_SF_BYTES >> 4);
       const int left = p.k_bytes - ks * 128;
       const int mmas = left >= 128 ? 4 : (left + 31) / 32;
       if (lead) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           if (2 * j < mmas) {
-            tmem_copy_scales<1>(tmem + MXS_SFA + 4 * j, sa + j * kMxAtomBytes);
-            tmem_copy_scales<1>(tmem + MXS_SFB + 4 * j, sa + MX_SF_BYTES + j * kMxAtomBytes);
+            tmem_copy_scales<1>(tmem + MXS_SFA + 4 * j, sa + j * kAtomLo);
+            tmem_copy_scales<1>(tmem + MXS_SFB + 4 * j, sb + j * kAtomLo);
           }
         }
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           if (kk < mmas)
-            umma_mxf4<1>(tmem, umma_smem_desc(a + kk * 32, 16, 1024), umma_smem_desc(b + kk * 32, 16, 1024),
-                         mx_idesc(MX_BM, MXS_N, (kk & 1) * 2), tmem + MXS_SFA + 4 * (kk >> 1), tmem + MXS_SFB + 4 * (kk >> 1),
-                         ks > ks0 || kk != 0 ? 1u : 0u);
+            umma_mxf4<1>(tmem, a + kk * 2, b + kk * 2, mx_idesc(MX_BM, MXS_N, (kk & 1) * 2), tmem + MXS_SFA + 4 * (kk >> 1),
+                         tmem + MXS_SFB + 4 * (kk >> 1), ks > ks0 || kk != 0 ? 1u : 0u);
         }
         umma_commit(&empty[stage]);
       }
