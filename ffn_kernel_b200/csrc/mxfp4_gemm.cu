@@ -102,11 +102,30 @@ struct MxParams {
   long long* prof;         // optional per-CTA wait-cycle counters (ffnk_debug_profile_buffer)
 };
 
+// Codes come through tensor maps; scales, whose atoms of a k-step are 1 KiB in a row, by plain bulk copies (each map
+// saved is 0.2 us of host time, which counts where a call takes 10).  CTA pairs need tensor maps for the scales too: only
+// a tensor copy may report to the barrier of another CTA than the one its data goes to.
 struct MxMaps {
-  CUtensorMap a, sa;       // activations: codes, scales
+  CUtensorMap a;           // activation codes
   CUtensorMap b[4];        // weight codes: visual 0/1, text 0/1 (gate, up)
-  CUtensorMap sb[4];       // weight scales
+  CUtensorMap tsa, tsb[4]; // scales, CTA pairs only: [row atom][128 words a k atom], boxes of two k atoms
+  const uint8_t* sa;       // activation scales
+  const uint8_t* sb[4];    // weight scales
+  int k_atoms;             // scale atoms of a row along the contraction
+  int sb_atoms;            // row atoms of a weight
 };
+
+// 16-byte aligned bulk copy to this CTA's shared memory, completion on an mbarrier given by its shared::cluster address
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
+}
+// bytes of one row atom's scales in k-step ks: two atoms of 4 blocks, one where the contraction ends
+__device__ __forceinline__ uint32_t mx_step_scale_bytes(int ks, int k_atoms) { return 2 * ks + 1 < k_atoms ? MX_SF_BYTES : kMxAtomBytes; }
+__device__ __forceinline__ const uint8_t* mx_scale_at(const uint8_t* base, int row_atom, int ks, int k_atoms) {
+  return base + (static_cast<int64_t>(row_atom) * k_atoms + 2 * ks) * kMxAtomBytes;
+}
 
 struct MxTile {
   int nt, row0, rows, list_off;
@@ -365,10 +384,10 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&maps.a);
-    tma_prefetch_desc(&maps.sa);
-    for (int i = 0; i < 4; ++i) {
-      tma_prefetch_desc(&maps.b[i]);
-      tma_prefetch_desc(&maps.sb[i]);
+    for (int i = 0; i < 4; ++i) tma_prefetch_desc(&maps.b[i]);
+    if constexpr (CTAS == 2) {
+      tma_prefetch_desc(&maps.tsa);
+      for (int i = 0; i < 4; ++i) tma_prefetch_desc(&maps.tsb[i]);
     }
   }
   if (warp == 1) {
@@ -398,12 +417,16 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
     uint32_t phase = 0;
     bool ok = true;
     const bool lead = elect_one();
-    const uint32_t bytes = p.a_rows * 128 + G::b_bytes + 3 * MX_SF_BYTES;
+    const uint32_t code_bytes = p.a_rows * 128 + G::b_bytes;
     for (int t = first; t < total && ok; t += step) {
       const MxTile tc = mx_tile(t, TILE_M, rank * MX_BM, tiles_v, m_tiles, n_tiles, p.group_m, Mv, Mt, cap);
       const CUtensorMap* b0 = &maps.b[tc.text ? 2 : 0];
-      const CUtensorMap* sb0 = &maps.sb[tc.text ? 2 : 0];
+      const uint8_t* sb0 = maps.sb[tc.text ? 2 : 0];
+      const uint8_t* sb1 = mx_glu(EPI) ? maps.sb[tc.text ? 3 : 1] : sb0;
+      const CUtensorMap* ts0 = &maps.tsb[tc.text ? 2 : 0];
       const int n0 = tc.nt * N_PER_TILE;
+      const int sb_row0 = n0 / 128, sb_row1 = mx_glu(EPI) ? sb_row0 : sb_row0 + 1;
+      const bool second = sb_row1 < maps.sb_atoms;      // 256 columns may end in their first 128
       for (int ks = 0; ks < k_steps; ++ks) {
         if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag)) {
           if (lead) mx_report(p.status, ST_TIMEOUT_PRODUCER);
@@ -416,12 +439,13 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
           uint8_t* sa = b + G::b_bytes;
           uint8_t* sb = sa + MX_SF_BYTES;
           uint64_t* bar = &full[stage];
-          uint32_t lead_bar = 0;
+          uint32_t lead_bar = smem_u32(bar);
+          const uint32_t sf = mx_step_scale_bytes(ks, maps.k_atoms);
           if constexpr (CTAS == 2) {
-            lead_bar = mapa_shared(smem_u32(bar), 0);
-            mbar_arrive_expect_tx_cluster(lead_bar, bytes);
+            lead_bar = mapa_shared(lead_bar, 0);
+            mbar_arrive_expect_tx_cluster(lead_bar, code_bytes + 3 * MX_SF_BYTES);
           } else {
-            mbar_arrive_expect_tx(bar, bytes);
+            mbar_arrive_expect_tx(bar, code_bytes + (second ? 3 : 2) * sf);
           }
           if constexpr (CTAS == 2) {
             if constexpr (mx_glu(EPI)) mx_load<CTAS>(b, b0 + rank, bar, lead_bar, ks * 128, n0);
@@ -430,10 +454,16 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
             mx_load<CTAS>(b, b0, bar, lead_bar, ks * 128, n0);
             if constexpr (mx_glu(EPI)) mx_load<CTAS>(b + G::b_bytes / 2, b0 + 1, bar, lead_bar, ks * 128, n0);
           }
-          mx_load<CTAS>(sb, sb0, bar, lead_bar, ks * 256, n0 / 128);
-          if constexpr (mx_glu(EPI)) mx_load<CTAS>(sb + MX_SF_BYTES, sb0 + 1, bar, lead_bar, ks * 256, n0 / 128);
           mx_load<CTAS>(a, &maps.a, bar, lead_bar, ks * 128, static_cast<int>(tc.routed0));
-          mx_load<CTAS>(sa, &maps.sa, bar, lead_bar, ks * 256, static_cast<int>(tc.routed0 >> 7));
+          if constexpr (CTAS == 2) {
+            mx_load<CTAS>(sb, ts0, bar, lead_bar, ks * 256, sb_row0);
+            if constexpr (mx_glu(EPI)) mx_load<CTAS>(sb + MX_SF_BYTES, ts0 + 1, bar, lead_bar, ks * 256, sb_row0);
+            mx_load<CTAS>(sa, &maps.tsa, bar, lead_bar, ks * 256, static_cast<int>(tc.routed0 >> 7));
+          } else {
+            bulk_load(sb, mx_scale_at(sb0, sb_row0, ks, maps.k_atoms), sf, lead_bar);
+            if (second) bulk_load(sb + MX_SF_BYTES, mx_scale_at(sb1, sb_row1, ks, maps.k_atoms), sf, lead_bar);
+            bulk_load(sa, mx_scale_at(maps.sa, static_cast<int>(tc.routed0 >> 7), ks, maps.k_atoms), sf, lead_bar);
+          }
         }
         __syncwarp();
         ++issued;
@@ -653,19 +683,21 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
   if (warp == 0) {
     const bool lead = elect_one();
     const CUtensorMap* mb = &maps.b[(text ? 2 : 0) + up];
-    const CUtensorMap* msb = &maps.sb[(text ? 2 : 0) + up];
-    const uint32_t bytes = p.a_rows * 128 + MXS_STAGE_FIXED;
+    const uint8_t* sb = maps.sb[(text ? 2 : 0) + up];
+    const uint32_t code_bytes = p.a_rows * 128 + MXS_B_BYTES;
     int issued = 0;
     auto load_b = [&](int ks, int stage) {
       uint8_t* b = smem + stage * stage_bytes + q.a_slot;
-      mbar_arrive_expect_tx(&full[stage], bytes);
+      const uint32_t sf = mx_step_scale_bytes(ks, maps.k_atoms);
+      mbar_arrive_expect_tx(&full[stage], code_bytes + 2 * sf);
       tma_load_2d(b, mb, &full[stage], ks * 128, nt * MXS_N);
-      tma_load_2d(b + MXS_B_BYTES + MX_SF_BYTES, msb, &full[stage], ks * 256, nt);
+      bulk_load(b + MXS_B_BYTES + MX_SF_BYTES, mx_scale_at(sb, nt, ks, maps.k_atoms), sf, smem_u32(&full[stage]));
     };
     auto load_a = [&](int ks, int stage) {
       uint8_t* a = smem + stage * stage_bytes;
       tma_load_2d(a, &maps.a, &full[stage], ks * 128, routed0);
-      tma_load_2d(a + q.a_slot + MXS_B_BYTES, &maps.sa, &full[stage], ks * 256, routed0 >> 7);
+      bulk_load(a + q.a_slot + MXS_B_BYTES, mx_scale_at(maps.sa, routed0 >> 7, ks, maps.k_atoms),
+                mx_step_scale_bytes(ks, maps.k_atoms), smem_u32(&full[stage]));
     };
     const int ahead = min(q.stages, ks1 - ks0);
     if (lead)
@@ -828,15 +860,33 @@ struct MxWeight {
   const void* scales;
 };
 
-// codes [rows, ld bytes], box of 128 bytes x box_rows; scales as [row atoms][k atoms x 128 words], box of two atoms
-// (1 KiB) x box_atoms.  Boxes past the end read zeros.
-static int mx_maps(CUtensorMap* codes, CUtensorMap* scales, const MxWeight& w, int64_t rows, int64_t cols, int box_rows,
-                   int box_atoms) {
-  int r = make_tensor_map_2d_of(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes, mx_code_ld(cols), rows, mx_code_ld(cols), 128,
-                                box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+// codes [rows, ld bytes], boxes of 128 bytes x box_rows; a box past the end reads zeros
+static int mx_code_map(CUtensorMap* m, const void* codes, int64_t rows, int64_t cols, int box_rows) {
+  return make_tensor_map_2d_of(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, mx_code_ld(cols), rows, mx_code_ld(cols), 128, box_rows,
+                               CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+static int mx_scale_map(CUtensorMap* m, const void* scales, int64_t rows, int64_t cols, int box_atoms) {
+  return make_tensor_map_2d_of(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, mx_k_atoms(cols) * (kMxAtomBytes / 4), mx_row_atoms(rows),
+                               mx_k_atoms(cols) * kMxAtomBytes, 256, box_atoms, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+// `n` weights [n_rows, k] (slot i of maps.b / maps.sb is weight slots[i]) and the routed activations of M tokens
+static int mx_maps(MxMaps& m, const MxWeight& a, int64_t M, const MxWeight* w, const int* slots, int n, int64_t n_rows, int64_t k,
+                   int a_box, int b_box, int pair_sb_box) {
+  const int64_t a_rows = ffnk_route_capacity(M) + 512;
+  int r = mx_code_map(&m.a, a.codes, a_rows, k, a_box);
   if (r) return r;
-  return make_tensor_map_2d_of(scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, w.scales, mx_k_atoms(cols) * (kMxAtomBytes / 4),
-                               mx_row_atoms(rows), mx_k_atoms(cols) * kMxAtomBytes, 256, box_atoms, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (pair_sb_box && (r = mx_scale_map(&m.tsa, a.scales, a_rows, k, 1))) return r;
+  m.sa = static_cast<const uint8_t*>(a.scales);
+  for (int i = 0; i < n; ++i) {
+    if ((r = mx_code_map(&m.b[slots[i]], w[i].codes, n_rows, k, b_box))) return r;
+    if (pair_sb_box && (r = mx_scale_map(&m.tsb[slots[i]], w[i].scales, n_rows, k, pair_sb_box))) return r;
+    m.sb[slots[i]] = static_cast<const uint8_t*>(w[i].scales);
+  }
+  m.k_atoms = static_cast<int>(mx_k_atoms(k));
+  m.sb_atoms = static_cast<int>(mx_row_atoms(n_rows));
+  return 0;
 }
 
 // Row tiles of a super-tile: about 16 MiB of activation codes stay in L2 while the weights pass.
@@ -944,16 +994,18 @@ static int mx_launch_small(const MxMaps& maps, const MxParams& p, int64_t M, con
 // y[token] = routed rows of (codes, scales) by the modality's weight [N, K]
 static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt, const int32_t* perm, const int32_t* counts,
                       const void* mask, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int32_t* status, cudaStream_t s) {
-  MxMaps m;
-  int r;
-  const int64_t rows = ffnk_route_capacity(M) + 512;
-  if ((r = mx_maps(&m.a, &m.sa, a, rows, K, mx_a_box_rows(M), 1))) return r;
   const bool pairs = mx_pairs(M);
   const int splits = mx_small_splits(M, N, K, false);
-  const int box = splits ? MXS_N : pairs ? MX_BN / 2 : MX_BN, atoms = splits ? 1 : 2;
-  if ((r = mx_maps(&m.b[0], &m.sb[0], wv, N, K, box, atoms))) return r;
-  if ((r = mx_maps(&m.b[2], &m.sb[2], wt, N, K, box, atoms))) return r;
-  m.b[1] = m.b[0]; m.b[3] = m.b[2]; m.sb[1] = m.sb[0]; m.sb[3] = m.sb[2];
+  const MxWeight w[2] = {wv, wt};
+  const int slots[2] = {0, 2};
+  MxMaps m{};
+  const int r = mx_maps(m, a, M, w, slots, 2, N, K, mx_a_box_rows(M), splits ? MXS_N : pairs ? MX_BN / 2 : MX_BN,
+                        pairs && !splits ? 2 : 0);
+  if (r) return r;
+  m.b[1] = m.b[0];
+  m.b[3] = m.b[2];
+  m.tsb[1] = m.tsb[0];
+  m.tsb[3] = m.tsb[2];
   MxParams p{};
   p.perm = perm; p.counts = counts; p.status = status; p.prof = debug_profile_buffer();
   p.n_out = static_cast<int>(N);
@@ -968,18 +1020,17 @@ static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt,
 // quantised silu(gate) * up of the routed rows, optionally with the pre-activations kept (t1, t3 both or neither)
 static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* perm, const int32_t* counts, void* codes,
                      void* scales, const void* mask, void* t1, void* t3, int64_t M, int64_t d, int64_t h, int32_t* status, cudaStream_t s) {
-  MxMaps m;
-  int r;
-  const int64_t rows = ffnk_route_capacity(M) + 512;
-  if ((r = mx_maps(&m.a, &m.sa, a, rows, d, mx_a_box_rows(M), 1))) return r;
-  for (int i = 0; i < 4; ++i)
-    if ((r = mx_maps(&m.b[i], &m.sb[i], w[i], h, d, MX_BN / 2, 1))) return r;
+  const int slots[4] = {0, 1, 2, 3};
+  const int splits = mx_small_splits(M, h, d, true);
+  const bool pairs = mx_pairs(M);
+  MxMaps m{};
+  const int r = mx_maps(m, a, M, w, slots, 4, h, d, mx_a_box_rows(M), MX_BN / 2, pairs && !splits ? 1 : 0);
+  if (r) return r;
   MxParams p{};
   p.perm = perm; p.counts = counts; p.status = status; p.prof = debug_profile_buffer();
   p.n_out = static_cast<int>(h);
   p.k_bytes = static_cast<int>(mx_code_ld(d));
   p.a_rows = mx_a_box_rows(M);
-  const bool pairs = mx_pairs(M);
   p.group_m = mx_group_m(d, pairs ? 2 * MX_BM : MX_BM);
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = static_cast<uint8_t*>(scales);
@@ -987,7 +1038,7 @@ static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* p
   p.k_atoms_out = static_cast<int>(mx_k_atoms(h));
   p.t1 = static_cast<float*>(t1);
   p.t3 = static_cast<float*>(t3);
-  if (const int splits = mx_small_splits(M, h, d, true)) return mx_launch_small<true>(m, p, M, mask, splits, s);
+  if (splits) return mx_launch_small<true>(m, p, M, mask, splits, s);
   return t1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, pairs, s) : mx_launch<MX_EPI_GLU>(m, p, M, pairs, s);
 }
 

@@ -45,22 +45,22 @@ class MXFP4Tensor:
     __slots__ = ("codes", "scales", "rows", "cols", "device", "ptrs")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
-        want_c, want_s = (rows, -(-cols // 32) * 16), (-(-rows // 128), -(-cols // 128), 32, 4, 4)
-        for t, want, name in ((codes, want_c, "codes"), (scales, want_s, "scales")):
-            if not isinstance(t, torch.Tensor) or not t.is_cuda:
-                raise RuntimeError(f"{name} must be a CUDA tensor; this package has no CPU path")
-            if t.dtype != torch.uint8 or t.shape != want:
-                raise RuntimeError(f"{name} of a [{rows}, {cols}] MXFP4 matrix must be torch.uint8 {list(want)}, "
-                                   f"got {t.dtype} {list(t.shape)}")
-            if not t.is_contiguous():
-                raise RuntimeError(f"{name} must be contiguous")
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
-        self.device = codes.device
-        self.ptrs = (codes.data_ptr(), scales.data_ptr())
-        if scales.device != self.device:
-            raise RuntimeError("codes and scales must be on the same device")
-        if (self.ptrs[0] | self.ptrs[1]) & 15:
-            raise RuntimeError("codes and scales must be 16-byte aligned")
+        try:
+            ptrs = (codes.data_ptr(), scales.data_ptr())
+            device = codes.device
+            ok = (codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_cuda and scales.device == device
+                  and codes.shape == (rows, (cols + 31) // 32 * 16)
+                  and scales.shape == ((rows + 127) // 128, (cols + 127) // 128, 32, 4, 4)
+                  and codes.is_contiguous() and scales.is_contiguous() and not (ptrs[0] | ptrs[1]) & 15)
+        except AttributeError:
+            ok = False
+        if not ok:
+            raise RuntimeError(
+                f"an MXFP4 matrix [{rows}, {cols}] takes codes torch.uint8 [{rows}, {-(-cols // 32) * 16}] and scales torch.uint8 "
+                f"[{-(-rows // 128)}, {-(-cols // 128)}, 32, 4, 4], both contiguous, 16-byte aligned and on one CUDA device; got "
+                + " and ".join(f"{t.dtype} {list(t.shape)} strides {list(t.stride())} on {t.device}" if isinstance(t, torch.Tensor)
+                               else type(t).__name__ for t in (codes, scales)))
+        self.codes, self.scales, self.rows, self.cols, self.device, self.ptrs = codes, scales, rows, cols, device, ptrs
 
     @property
     def shape(self):
