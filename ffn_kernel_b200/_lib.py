@@ -67,6 +67,7 @@ SIGNATURES = {
     "ffnk_mxfp4_quantize": (c_int, [c_void_p, c_int] + [c_int64] * 4 + [c_void_p] * 3),
     "ffnk_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p]),
     "ffnk_mxfp4_workspace_bytes": (c_int64, [c_int64] * 3),
+    "ffnk_mxfp4_kept_bytes": (c_int64, [c_int64, c_int64]),
     "ffnk_mxfp4_linear_forward": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + [c_int64, c_void_p] + [c_int64] * 4
                                   + [c_void_p, c_void_p]),
     "ffnk_mxfp4_ffn_forward": (c_int, [c_void_p, c_int64, POINTER(c_void_p), POINTER(c_void_p)] + [c_void_p] * 4

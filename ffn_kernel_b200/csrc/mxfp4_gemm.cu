@@ -89,11 +89,12 @@ struct MxParams {
   int k_bytes;             // code bytes of a row along the contraction (a multiple of 16)
   int a_rows;              // rows of an A box (fewer than 128 when no tile has more)
   int group_m;
-  // MX_EPI_STORE: out[token][n]; MX_EPI_GLU_SAVE: t1, t3 fp32 in routed rows, tiled (pre_tile_offset)
+  // MX_EPI_STORE: out[token][n]; MX_EPI_GLU_SAVE: t1, t3 of pre_rows = cap + 512 routed rows (pre_tile_offset)
   __nv_bfloat16* out;
   int64_t ldo;
-  float* t1;
-  float* t3;
+  __half* t1;
+  __half* t3;
+  int64_t pre_rows;
   // MX_EPI_GLU*: codes [routed row][code_ld] and scales of the quantised product
   uint8_t* codes;
   uint8_t* scales;
@@ -267,6 +268,28 @@ __device__ __forceinline__ void mx_issue_step(uint32_t d, uint32_t tmem, uint32_
   }
 }
 
+// One row's 32 pre-activations for the backward pass (pre_tile_offset: fp16 with a shared exponent).
+__device__ __forceinline__ void mx_keep_block(const float (&v)[32], __half* base, int64_t pre_rows, int64_t row, int n0, int h) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  const uint32_t byte = pre_scale_byte(m);
+  const float inv = pre_inverse_scale(byte);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (n0 + 8 * j < h) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2 t = __floats2half2_rn(v[8 * j + 2 * i] * inv, v[8 * j + 2 * i + 1] * inv);
+        w[i] = *reinterpret_cast<const uint32_t*>(&t);
+      }
+      *reinterpret_cast<uint4*>(base + pre_tile_offset(row, n0 + 8 * j, h)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  reinterpret_cast<uint8_t*>(base + pre_rows * h)[pre_scale_offset(row, n0, h)] = static_cast<uint8_t>(byte);
+}
+
 // Epilogue of one warp: TMEM lane quarter q, columns of `part` (0/1 of two).  `on_shared` runs once after the
 // first chunk has been read (the chunk holding the columns the two accumulators share, for the part that has it).
 template <int EPI, class F>
@@ -311,15 +334,9 @@ __device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, c
         b[e] = __uint_as_float(u[e]);
       }
       if constexpr (EPI == MX_EPI_GLU_SAVE) {
-        // kept in fp32: the gradients are taken at these values, and bf16 copies of them would add as much error to dx
-        // as its own rounding does
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (valid && n0 + 4 * j < p.n_out) {
-            const int64_t o = pre_tile_offset(drow, n0 + 4 * j, p.n_out);
-            *reinterpret_cast<float4*>(p.t1 + o) = make_float4(a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
-            *reinterpret_cast<float4*>(p.t3 + o) = make_float4(b[4 * j], b[4 * j + 1], b[4 * j + 2], b[4 * j + 3]);
-          }
+        if (valid && n0 < p.n_out) {
+          mx_keep_block(a, p.t1, p.pre_rows, drow, n0, p.n_out);
+          mx_keep_block(b, p.t3, p.pre_rows, drow, n0, p.n_out);
         }
       }
       // columns past h are weight rows that do not exist: zeros, whatever their scales hold
@@ -818,10 +835,33 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
       }
     } else {
       const int64_t drow = routed0 + row;
-      if (p.t1 && n0 < p.n_out) {
-        const int64_t o = pre_tile_offset(drow, n0, p.n_out);
-        *reinterpret_cast<float4*>(p.t1 + o) = g;
-        *reinterpret_cast<float4*>(p.t3 + o) = u;
+      if (p.t1) {                                         // uniform
+        uint32_t m1 = 0, m3 = 0;
+        if (n0 < p.n_out) {
+          m1 = max(max(__float_as_uint(g.x) & 0x7FFFFFFFu, __float_as_uint(g.y) & 0x7FFFFFFFu),
+                   max(__float_as_uint(g.z) & 0x7FFFFFFFu, __float_as_uint(g.w) & 0x7FFFFFFFu));
+          m3 = max(max(__float_as_uint(u.x) & 0x7FFFFFFFu, __float_as_uint(u.y) & 0x7FFFFFFFu),
+                   max(__float_as_uint(u.z) & 0x7FFFFFFFu, __float_as_uint(u.w) & 0x7FFFFFFFu));
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+          m1 = max(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
+          m3 = max(m3, __shfl_xor_sync(0xFFFFFFFFu, m3, o));
+        }
+        const uint32_t k1 = pre_scale_byte(m1), k3 = pre_scale_byte(m3);
+        if (n0 < p.n_out) {
+          const float i1 = pre_inverse_scale(k1), i3 = pre_inverse_scale(k3);
+          const int64_t o = pre_tile_offset(drow, n0, p.n_out);
+          const __half2 h1[2] = {__floats2half2_rn(g.x * i1, g.y * i1), __floats2half2_rn(g.z * i1, g.w * i1)};
+          const __half2 h3[2] = {__floats2half2_rn(u.x * i3, u.y * i3), __floats2half2_rn(u.z * i3, u.w * i3)};
+          *reinterpret_cast<uint2*>(p.t1 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h1[0]), *reinterpret_cast<const uint32_t*>(&h1[1]));
+          *reinterpret_cast<uint2*>(p.t3 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h3[0]), *reinterpret_cast<const uint32_t*>(&h3[1]));
+          if ((lane & 7) == 0) {
+            const int64_t so = pre_scale_offset(drow, n0, p.n_out);
+            reinterpret_cast<uint8_t*>(p.t1 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k1);
+            reinterpret_cast<uint8_t*>(p.t3 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k3);
+          }
+        }
       }
       float v[8] = {};
       if (n0 < p.n_out) {
@@ -1036,8 +1076,9 @@ static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* p
   p.scales = static_cast<uint8_t*>(scales);
   p.code_ld = mx_code_ld(h);
   p.k_atoms_out = static_cast<int>(mx_k_atoms(h));
-  p.t1 = static_cast<float*>(t1);
-  p.t3 = static_cast<float*>(t3);
+  p.t1 = static_cast<__half*>(t1);
+  p.t3 = static_cast<__half*>(t3);
+  p.pre_rows = ffnk_route_capacity(M) + 512;
   if (splits) return mx_launch_small<true>(m, p, M, mask, splits, s);
   return t1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, pairs, s) : mx_launch<MX_EPI_GLU>(m, p, M, pairs, s);
 }
@@ -1068,6 +1109,12 @@ static bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) &
 }  // namespace ffnk
 
 using namespace ffnk;
+
+extern "C" int64_t ffnk_mxfp4_kept_bytes(int64_t M, int64_t h) {
+  if (M <= 0 || h <= 0) return 256;
+  const int64_t rows = ffnk_route_capacity(M) + 512;
+  return rows * h * 2 + rows * ((h + 31) / 32);
+}
 
 extern "C" int64_t ffnk_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t h) {
   if (M <= 0 || K <= 0 || h < 0) return 256;

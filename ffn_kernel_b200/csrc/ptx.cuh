@@ -46,12 +46,26 @@ __device__ __forceinline__ bool mask_is_scattered(const int* counts, int run_thr
   return static_cast<long long>(counts[4]) * run_threshold > counts[3];
 }
 
-// Pre-activations kept in fp32 between the forward and the backward pass of the FFN on 4-bit weights: element (routed
-// row, column) of a matrix `h` columns wide in tiles of 128 rows x 4 columns, so that the 32 rows of a warp are 512
-// contiguous bytes (columns in fours).
+// Pre-activations kept between the forward and the backward pass of the FFN on 4-bit weights: fp16 with one power of
+// two per row and 32 columns (byte b stands for 2^(b - 127)), chosen so that the largest of the 32 lands in [2^14, 2^15).
+// bf16 copies would add as much error to dx as its own rounding does, fp32 ones are twice the traffic; the shared
+// exponent keeps 11 bits for everything down to 2^-28 of the largest and leaves no value out of range.
+//   values  element (routed row, column) at pre_tile_offset: tiles of 128 rows x 8 columns
+//   scales  byte (routed row, column / 32) at pre_scale_offset, behind the (cap + 512) * h values
+// so that the 32 rows of a warp are 512 (scales: 32) contiguous bytes.
 __device__ __forceinline__ int64_t pre_tile_offset(int64_t row, int col, int h) {
-  return (((row >> 7) * (h >> 2) + (col >> 2)) * 128 + (row & 127)) * 4 + (col & 3);
+  return (((row >> 7) * (h >> 3) + (col >> 3)) * 128 + (row & 127)) * 8 + (col & 7);
 }
+__device__ __forceinline__ int64_t pre_scale_offset(int64_t row, int col, int h) {
+  return ((row >> 7) * ((h + 31) >> 5) + (col >> 5)) * 128 + (row & 127);
+}
+// bits of max |x| over the 32 -> scale byte and the factor 1 / 2^(byte - 127) (infinities and NaN pass through as such)
+__device__ __forceinline__ uint32_t pre_scale_byte(uint32_t absmax_bits) {
+  const int e = static_cast<int>(absmax_bits >> 23);
+  return e == 255 ? 127u : (e > 15 ? static_cast<uint32_t>(e - 14) : 1u);
+}
+__device__ __forceinline__ float pre_inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ float pre_scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 __device__ __forceinline__ uint32_t lane_id() { return threadIdx.x & 31; }
 

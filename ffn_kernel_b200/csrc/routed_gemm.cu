@@ -25,6 +25,7 @@
 // accumulator is double buffered in TMEM (2 x 256 columns) so the epilogue of tile i runs
 // under the main loop of tile i+1.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <mutex>
 
@@ -63,9 +64,8 @@ enum { A_GATHER = 0, A_ROUTED = 1 };
 // EPI_DSWIGLU     : acc = dH; with t1 = aux0, t3 = aux1 at the same position:
 //                   out = dH * t3 * s * (1 + t1 * (1 - s)),  aux2 = dH * t1 * s,  s = sigmoid(t1)
 //                   (the element-wise terms of the FFN backward, reference README.md:159-172)
-// EPI_DSWIGLU_F32 : the same with t1, t3 in fp32, in the tiled order of pre_tile_offset (the forward pass on 4-bit
-//                   weights leaves them so)
-enum { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_SWIGLU_SAVE = 2, EPI_DSWIGLU = 3, EPI_DSWIGLU_F32 = 4 };
+// EPI_DSWIGLU_PRE : the same with t1, t3 as the forward pass on 4-bit weights keeps them (pre_tile_offset, ptx.cuh)
+enum { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_SWIGLU_SAVE = 2, EPI_DSWIGLU = 3, EPI_DSWIGLU_PRE = 4 };
 __host__ __device__ constexpr bool epi_glu(int e) { return e == EPI_SWIGLU || e == EPI_SWIGLU_SAVE; }
 // OUT_SCATTER : row of token t -> out[t]            OUT_ROUTED : row i of the routed order -> out[i]
 // OUT_PEER    : row of token t -> row block `peer_rank` of the buffer of the rank that owns token t
@@ -310,9 +310,9 @@ __device__ __forceinline__ void epilogue_glu_staged(uint32_t taddr, const GemmPa
 // the saved pre-activations as well as for the two stores: four accesses per element, each of which
 // would otherwise touch 32 rows per instruction.
 //
-// F32: t1 and t3 come in fp32 in the tiled order instead, a lane's own row at a time: the 32 lanes of a warp read 512
-// contiguous bytes an access and nothing is transposed.
-template <int BN_T, bool F32 = false>
+// PRE: t1 and t3 come in fp16 with a shared exponent per 32 columns instead, tiled so that a lane reads its own row:
+// the 32 lanes of a warp are 512 contiguous bytes an access and nothing is transposed.
+template <int BN_T, bool PRE = false>
 __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const GemmParams& p, long long row_off,
                                                         int n_base, int part, int parts, uint8_t* stg, int lane) {
   constexpr int CH = BN_T / 32;
@@ -366,23 +366,39 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
   };
   const int c_begin = part * CH / parts, c_end = (part + 1) * CH / parts;
   uint4 l1[4], l3[4];
-  if constexpr (!F32) {
+  if constexpr (!PRE) {
     load4(l1, p.aux0, n_base + c_begin * 32);
     load4(l3, p.aux1, n_base + c_begin * 32);
   }
   const int my_row = row_off >= 0 ? static_cast<int>(row_off / p.ldo) : -1;
-  float4 f1[8], f3[8];
-  auto load_tiled = [&](float4 (&l)[8], const __nv_bfloat16* base, int n0) {
+  uint4 f1[4], f3[4];
+  uint32_t b1 = 0, b3 = 0;
+  auto load_pre = [&](uint4 (&l)[4], uint32_t& scale, const __nv_bfloat16* base, int n0) {
+    const __half* v = reinterpret_cast<const __half*>(base);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      l[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (my_row >= 0 && n0 + 4 * j < p.n_out)
-        l[j] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + pre_tile_offset(my_row, n0 + 4 * j, p.n_out));
+    for (int j = 0; j < 4; ++j) {
+      l[j] = make_uint4(0, 0, 0, 0);
+      if (my_row >= 0 && n0 + 8 * j < p.n_out) l[j] = *reinterpret_cast<const uint4*>(v + pre_tile_offset(my_row, n0 + 8 * j, p.n_out));
+    }
+    if (my_row >= 0 && n0 < p.n_out)
+      scale = reinterpret_cast<const uint8_t*>(v + static_cast<int64_t>(p.pad_row) * p.n_out)[pre_scale_offset(my_row, n0, p.n_out)];
+  };
+  auto spread_pre = [&](float (&v)[32], const uint4 (&l)[4], uint32_t scale) {
+    const float f = pre_scale_value(scale);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w[4] = {l[j].x, l[j].y, l[j].z, l[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[8 * j + 2 * i] = t.x * f;
+        v[8 * j + 2 * i + 1] = t.y * f;
+      }
     }
   };
-  if constexpr (F32) {
-    load_tiled(f1, p.aux0, n_base + c_begin * 32);
-    load_tiled(f3, p.aux1, n_base + c_begin * 32);
+  if constexpr (PRE) {
+    load_pre(f1, b1, p.aux0, n_base + c_begin * 32);
+    load_pre(f3, b3, p.aux1, n_base + c_begin * 32);
   }
 #pragma unroll 1
   for (int c = c_begin; c < c_end; ++c) {
@@ -390,12 +406,9 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
     tmem_ld_32x32(taddr + c * 32, acc);
     const int n0 = n_base + c * 32;
     float t1[32], t3[32];
-    if constexpr (F32) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        t1[4 * j] = f1[j].x; t1[4 * j + 1] = f1[j].y; t1[4 * j + 2] = f1[j].z; t1[4 * j + 3] = f1[j].w;
-        t3[4 * j] = f3[j].x; t3[4 * j + 1] = f3[j].y; t3[4 * j + 2] = f3[j].z; t3[4 * j + 3] = f3[j].w;
-      }
+    if constexpr (PRE) {
+      spread_pre(t1, f1, b1);
+      spread_pre(t3, f3, b3);
     } else {
       spread(t1, l1);
       spread(t3, l3);
@@ -414,9 +427,9 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
       t3[e] = dh * t1[e] * sg;     // d3
       t1[e] = d1;
     }
-    if (F32 && c + 1 < c_end) {      // the accumulator's registers are free now: the next chunk's loads fly under the stores
-      load_tiled(f1, p.aux0, n0 + 32);
-      load_tiled(f3, p.aux1, n0 + 32);
+    if (PRE && c + 1 < c_end) {      // the accumulator's registers are free now: the next chunk's loads fly under the stores
+      load_pre(f1, b1, p.aux0, n0 + 32);
+      load_pre(f3, b3, p.aux1, n0 + 32);
     }
     flush(t1, p.out, n0);
     flush(t3, p.aux2, n0);
@@ -844,8 +857,8 @@ routed_gemm_kernel(const __grid_constant__ AMaps am, const __grid_constant__ CUt
       if constexpr (epi_glu(EPI))
         epilogue_glu_staged<EPI, BN_T>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * (BN_T / 2), part,
                                        epilogue_parts(), smem + TSTAGES * TSTAGE_BYTES + 256 + (warp - 2) * 2048, lane);
-      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_F32)
-        epilogue_dswiglu_staged<BN_T, EPI == EPI_DSWIGLU_F32>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * BN_T, part, epilogue_parts(),
+      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_PRE)
+        epilogue_dswiglu_staged<BN_T, EPI == EPI_DSWIGLU_PRE>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * BN_T, part, epilogue_parts(),
                                       smem + TSTAGES * TSTAGE_BYTES + 256 + (warp - 2) * 2048, lane);
       else
         epilogue_rows_staged<BN_T>(taddr, p, OUT_MODE == OUT_PEER ? peer_dst : (valid ? p.out + dst_row * p.ldo : nullptr),
@@ -1127,8 +1140,8 @@ routed_gemm_pair_kernel(const __grid_constant__ AMaps am, const __grid_constant_
       if constexpr (epi_glu(EPI))
         epilogue_glu_staged<EPI, BN>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * N_PER_TILE, part,
                                      epilogue_parts(), smem + PAIR_STAGES * PAIR_STAGE_BYTES + 256 + (warp - 2) * 2048, lane);
-      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_F32)
-        epilogue_dswiglu_staged<BN, EPI == EPI_DSWIGLU_F32>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * N_PER_TILE, part, epilogue_parts(),
+      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_PRE)
+        epilogue_dswiglu_staged<BN, EPI == EPI_DSWIGLU_PRE>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * N_PER_TILE, part, epilogue_parts(),
                                     smem + PAIR_STAGES * PAIR_STAGE_BYTES + 256 + (warp - 2) * 2048, lane);
       else
         epilogue_rows_staged<BN>(taddr, p, OUT_MODE == OUT_PEER ? peer_dst : (valid ? p.out + dst_row * p.ldo : nullptr),
@@ -2476,7 +2489,7 @@ int ffnk::ffn_backward_dx(const void* gy, int64_t ldg, const void* t1, const voi
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int r = ffnk_permute_rows(gy, ldg, perm, counts, gr, d, M, d, stream);
   if (r) return r;
-  if ((r = dswiglu_gemm<EPI_DSWIGLU_F32>(gr, w2, u2, 1, h, t1, t3, perm, counts, dt1, dt3, M, d, h, status, s))) return r;
+  if ((r = dswiglu_gemm<EPI_DSWIGLU_PRE>(gr, w2, u2, 1, h, t1, t3, perm, counts, dt1, dt3, M, d, h, status, s))) return r;
   return ffn_dx_gemm(dt1, dt3, w1, w3, u1, u3, 1, d, perm, counts, dx, lddx, M, d, h, status, s);
 }
 

@@ -208,7 +208,7 @@ def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
         ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
         t1 = t3 = None
         if keep:
-            t1, t3 = (torch.empty(((M + 127) // 128 * 128 + 512) * h, device=dev, dtype=torch.float32) for _ in range(2))
+            t1, t3 = (torch.empty(L.ffnk_mxfp4_kept_bytes(M, h), device=dev, dtype=torch.uint8) for _ in range(2))
         check("ffnk_mxfp4_ffn_forward", L.ffnk_mxfp4_ffn_forward(
             x.data_ptr(), x.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]),
             mask.data_ptr(), perm, counts, wp, nbytes, t1.data_ptr() if keep else None,

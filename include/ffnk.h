@@ -353,9 +353,10 @@ int ffnk_mxfp4_linear_forward(const void* x, int64_t ldx, const void* b1_codes, 
 /* Routed SwiGLU FFN on MXFP4 weights (compare ffnk_ffn_forward):
  *     y = Q(silu(Q(x) w1^T) * (Q(x) w3^T)) w2^T for visual tokens, u1, u3, u2 for text tokens
  * codes, scales: HOST arrays of six device pointers each, in the order w1, w2, w3, u1, u2, u3; w1, w3, u1, u3 are
- * [h, d], w2, u2 [d, h].  The hidden activation is quantised from fp32.  t1, t3: both null, or fp32 of
- * (cap + 512) * h elements each, where the pre-activations are kept for the backward pass, in an order of the
- * library's own.  workspace: ffnk_mxfp4_workspace_bytes(M, d, h). */
+ * [h, d], w2, u2 [d, h].  The hidden activation is quantised from fp32.  t1, t3: both null, or
+ * ffnk_mxfp4_kept_bytes(M, h) bytes each, where the pre-activations are kept for the backward pass in a form of the
+ * library's own (fp16 with a shared exponent per 32).  workspace: ffnk_mxfp4_workspace_bytes(M, d, h). */
+int64_t ffnk_mxfp4_kept_bytes(int64_t M, int64_t h);
 int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* const* codes, const void* const* scales,
                            const void* mask, int32_t* perm, int32_t* counts, void* workspace, int64_t workspace_bytes,
                            void* t1, void* t3, void* y, int64_t ldy, int64_t M, int64_t d, int64_t h, int32_t* status,
