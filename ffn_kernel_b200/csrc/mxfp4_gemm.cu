@@ -623,6 +623,13 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
   return v;
 }
 
+// Cluster-wide barrier that orders nothing: only for "no peer touches my shared memory any more" at the end of the
+// kernel (a releasing arrival would wait a microsecond for the stores of the results).
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
 struct MxSmall {
   const uint8_t* mask;    // null: M is larger than a CTA counts
   int M;
@@ -654,6 +661,9 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
+    tma_prefetch_desc(&maps.a);
+    tma_prefetch_desc(&maps.b[up]);
+    tma_prefetch_desc(&maps.b[2 + up]);
   }
   if (warp == 1) {
     tmem_alloc<1>(tmem_slot, 256);
@@ -755,35 +765,41 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
+    auto issue = [&](uint32_t a, int mmas, uint32_t accumulate) {
+      const uint32_t b = a + (q.a_slot >> 4), sa = b + (MXS_B_BYTES >> 4), sb = sa + (MX_SF_BYTES >> 4);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (2 * j < mmas) {
+          tmem_copy_scales<1>(tmem + MXS_SFA + 4 * j, sa + j * kAtomLo);
+          tmem_copy_scales<1>(tmem + MXS_SFB + 4 * j, sb + j * kAtomLo);
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        if (kk < mmas)
+          umma_mxf4<1>(tmem, a + kk * 2, b + kk * 2, mx_idesc(MX_BM, MXS_N, (kk & 1) * 2), tmem + MXS_SFA + 4 * (kk >> 1),
+                       tmem + MXS_SFB + 4 * (kk >> 1), kk == 0 ? accumulate : 1u);
+      }
+    };
+    bool ready = ks0 < ks1 && mbar_test(&full[0], 0);
     for (int ks = ks0; ks < ks1; ++ks) {
-      if (!mbar_wait_warp(&full[stage], phase, abort_flag)) {
+      if (!__all_sync(0xFFFFFFFFu, ready) && !mbar_wait_warp(&full[stage], phase, abort_flag)) {
         if (lead) mx_report(p.status, ST_TIMEOUT_MMA_FULL);
         ok = false;
         break;
       }
       tc_fence_after();
       const uint32_t a = lo0 + stage * (stage_bytes >> 4);
-      const uint32_t b = a + (q.a_slot >> 4), sa = b + (MXS_B_BYTES >> 4), sb = sa + (MX_SF_BYTES >> 4);
       const int left = p.k_bytes - ks * 128;
-      const int mmas = left >= 128 ? 4 : (left + 31) / 32;
+      uint64_t* free_bar = &empty[stage];
+      if (++stage == q.stages) { stage = 0; phase ^= 1; }
+      ready = mbar_test(&full[stage], phase);
       if (lead) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if (2 * j < mmas) {
-            tmem_copy_scales<1>(tmem + MXS_SFA + 4 * j, sa + j * kAtomLo);
-            tmem_copy_scales<1>(tmem + MXS_SFB + 4 * j, sb + j * kAtomLo);
-          }
-        }
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          if (kk < mmas)
-            umma_mxf4<1>(tmem, a + kk * 2, b + kk * 2, mx_idesc(MX_BM, MXS_N, (kk & 1) * 2), tmem + MXS_SFA + 4 * (kk >> 1),
-                         tmem + MXS_SFB + 4 * (kk >> 1), ks > ks0 || kk != 0 ? 1u : 0u);
-        }
-        umma_commit(&empty[stage]);
+        if (left >= 128) issue(a, 4, ks != ks0);
+        else issue(a, (left + 31) / 32, ks != ks0);
+        umma_commit(free_bar);
       }
       __syncwarp();
-      if (++stage == q.stages) { stage = 0; phase ^= 1; }
     }
     if (lead && ok) umma_commit(done);
     __syncwarp();
@@ -816,76 +832,93 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
   __syncthreads();
   cluster_sync_all();                                     // every partial tile of the cluster is in place
 
-  for (int row = rank + csize * warp; row < rows; row += csize * (MXS_THREADS / 32)) {
-    const uint32_t mine = smem_u32(smem + row * 512 + ((lane ^ (row & 31)) << 4));
-    float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
+  // This CTA's rows are rank, rank + csize, ...; a warp takes two of them at a time, so that twice the remote loads are
+  // under way.
+  for (int r0 = rank + csize * warp; r0 < rows; r0 += 2 * csize * (MXS_THREADS / 32)) {
+    float4 sum[2][2] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i < csize) {
-        const float4 v = ld_cluster(mapa_shared(mine, i));
-        float4& d = GLU && (i & 1) ? u : g;
-        d.x += v.x; d.y += v.y; d.z += v.z; d.w += v.w;
-      }
-    }
-    const int n0 = nt * MXS_N + lane * 4;
-    if constexpr (!GLU) {
-      if (n0 < p.n_out) {
-        const int64_t token = p.perm[(text ? p.counts[2] : 0) + row0 + row];
-        *reinterpret_cast<uint2*>(p.out + token * p.ldo + n0) = make_uint2(mx_pack_bf16(g.x, g.y), mx_pack_bf16(g.z, g.w));
-      }
-    } else {
-      const int64_t drow = routed0 + row;
-      if (p.t1) {                                         // uniform
-        uint32_t m1 = 0, m3 = 0;
-        if (n0 < p.n_out) {
-          m1 = max(max(__float_as_uint(g.x) & 0x7FFFFFFFu, __float_as_uint(g.y) & 0x7FFFFFFFu),
-                   max(__float_as_uint(g.z) & 0x7FFFFFFFu, __float_as_uint(g.w) & 0x7FFFFFFFu));
-          m3 = max(max(__float_as_uint(u.x) & 0x7FFFFFFFu, __float_as_uint(u.y) & 0x7FFFFFFFu),
-                   max(__float_as_uint(u.z) & 0x7FFFFFFFu, __float_as_uint(u.w) & 0x7FFFFFFFu));
-        }
+    for (int h = 0; h < 2; ++h) {
+      const int row = r0 + h * csize * (MXS_THREADS / 32);
+      if (row < rows) {
+        const uint32_t mine = smem_u32(smem + row * 512 + ((lane ^ (row & 31)) << 4));
+        float4 v[8];
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-          m1 = max(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
-          m3 = max(m3, __shfl_xor_sync(0xFFFFFFFFu, m3, o));
-        }
-        const uint32_t k1 = pre_scale_byte(m1), k3 = pre_scale_byte(m3);
-        if (n0 < p.n_out) {
-          const float i1 = pre_inverse_scale(k1), i3 = pre_inverse_scale(k3);
-          const int64_t o = pre_tile_offset(drow, n0, p.n_out);
-          const __half2 h1[2] = {__floats2half2_rn(g.x * i1, g.y * i1), __floats2half2_rn(g.z * i1, g.w * i1)};
-          const __half2 h3[2] = {__floats2half2_rn(u.x * i3, u.y * i3), __floats2half2_rn(u.z * i3, u.w * i3)};
-          *reinterpret_cast<uint2*>(p.t1 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h1[0]), *reinterpret_cast<const uint32_t*>(&h1[1]));
-          *reinterpret_cast<uint2*>(p.t3 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h3[0]), *reinterpret_cast<const uint32_t*>(&h3[1]));
-          if ((lane & 7) == 0) {
-            const int64_t so = pre_scale_offset(drow, n0, p.n_out);
-            reinterpret_cast<uint8_t*>(p.t1 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k1);
-            reinterpret_cast<uint8_t*>(p.t3 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k3);
+        for (int i = 0; i < 8; ++i)
+          if (i < csize) v[i] = ld_cluster(mapa_shared(mine, i));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i < csize) {
+            float4& d = sum[h][GLU ? i & 1 : 0];
+            d.x += v[i].x; d.y += v[i].y; d.z += v[i].z; d.w += v[i].w;
           }
         }
       }
-      float v[8] = {};
-      if (n0 < p.n_out) {
-        v[0] = mx_silu_mul(g.x, u.x);
-        v[1] = mx_silu_mul(g.y, u.y);
-        v[2] = mx_silu_mul(g.z, u.z);
-        v[3] = mx_silu_mul(g.w, u.w);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = r0 + h * csize * (MXS_THREADS / 32);
+      if (row >= rows) break;                             // warp-uniform
+      const float4 g = sum[h][0], u = sum[h][1];
+      const int n0 = nt * MXS_N + lane * 4;
+      if constexpr (!GLU) {
+        if (n0 < p.n_out) {
+          const int64_t token = p.perm[(text ? p.counts[2] : 0) + row0 + row];
+          *reinterpret_cast<uint2*>(p.out + token * p.ldo + n0) = make_uint2(mx_pack_bf16(g.x, g.y), mx_pack_bf16(g.z, g.w));
+        }
+      } else {
+        const int64_t drow = routed0 + row;
+        if (p.t1) {                                         // uniform
+          uint32_t m1 = 0, m3 = 0;
+          if (n0 < p.n_out) {
+            m1 = max(max(__float_as_uint(g.x) & 0x7FFFFFFFu, __float_as_uint(g.y) & 0x7FFFFFFFu),
+                     max(__float_as_uint(g.z) & 0x7FFFFFFFu, __float_as_uint(g.w) & 0x7FFFFFFFu));
+            m3 = max(max(__float_as_uint(u.x) & 0x7FFFFFFFu, __float_as_uint(u.y) & 0x7FFFFFFFu),
+                     max(__float_as_uint(u.z) & 0x7FFFFFFFu, __float_as_uint(u.w) & 0x7FFFFFFFu));
+          }
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) {
+            m1 = max(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
+            m3 = max(m3, __shfl_xor_sync(0xFFFFFFFFu, m3, o));
+          }
+          const uint32_t k1 = pre_scale_byte(m1), k3 = pre_scale_byte(m3);
+          if (n0 < p.n_out) {
+            const float i1 = pre_inverse_scale(k1), i3 = pre_inverse_scale(k3);
+            const int64_t o = pre_tile_offset(drow, n0, p.n_out);
+            const __half2 h1[2] = {__floats2half2_rn(g.x * i1, g.y * i1), __floats2half2_rn(g.z * i1, g.w * i1)};
+            const __half2 h3[2] = {__floats2half2_rn(u.x * i3, u.y * i3), __floats2half2_rn(u.z * i3, u.w * i3)};
+            *reinterpret_cast<uint2*>(p.t1 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h1[0]), *reinterpret_cast<const uint32_t*>(&h1[1]));
+            *reinterpret_cast<uint2*>(p.t3 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h3[0]), *reinterpret_cast<const uint32_t*>(&h3[1]));
+            if ((lane & 7) == 0) {
+              const int64_t so = pre_scale_offset(drow, n0, p.n_out);
+              reinterpret_cast<uint8_t*>(p.t1 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k1);
+              reinterpret_cast<uint8_t*>(p.t3 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k3);
+            }
+          }
+        }
+        float v[8] = {};
+        if (n0 < p.n_out) {
+          v[0] = mx_silu_mul(g.x, u.x);
+          v[1] = mx_silu_mul(g.y, u.y);
+          v[2] = mx_silu_mul(g.z, u.z);
+          v[3] = mx_silu_mul(g.w, u.w);
+        }
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        const uint32_t byte = mx_scale_byte(m);
+        const float inv = mx_inverse_scale(byte);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= inv;
+        const uint32_t code = byte == 255u ? 0u : mx_pack8(v);
+        const int block = nt * 4 + (lane >> 3);
+        if (block * 32 < p.n_out) *reinterpret_cast<uint16_t*>(p.codes + drow * p.code_ld + block * 16 + (lane & 7) * 2) = static_cast<uint16_t>(code);
+        if ((lane & 7) == 0) p.scales[mx_scale_word(drow, nt, p.k_atoms_out) + (lane >> 3)] = static_cast<uint8_t>(byte);
       }
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-      const uint32_t byte = mx_scale_byte(m);
-      const float inv = mx_inverse_scale(byte);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] *= inv;
-      const uint32_t code = byte == 255u ? 0u : mx_pack8(v);
-      const int block = nt * 4 + (lane >> 3);
-      if (block * 32 < p.n_out) *reinterpret_cast<uint16_t*>(p.codes + drow * p.code_ld + block * 16 + (lane & 7) * 2) = static_cast<uint16_t>(code);
-      if ((lane & 7) == 0) p.scales[mx_scale_word(drow, nt, p.k_atoms_out) + (lane >> 3)] = static_cast<uint8_t>(byte);
     }
   }
-  cluster_sync_all();                                     // nobody leaves while a peer still reads its shared memory
+  cluster_sync_relaxed();                                 // nobody leaves while a peer still reads its shared memory
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<1>(tmem, 256);
@@ -937,10 +970,13 @@ static int mx_group_m(int64_t k, int64_t rows_per_tile) {
 
 static int mx_a_box_rows(int64_t M) { return M >= MX_BM || tune_overrides().pair > 0 ? MX_BM : static_cast<int>((M + 7) / 8 * 8); }
 
-// CTA pairs or single CTAs.
-static bool mx_pairs(int64_t M) {
+// CTA pairs or single CTAs.  Pairs halve the weight traffic of an SM but hand tiles out in twice the size and pay for
+// signals between the two: worth it for long contractions, or for many rows.  Measured (single / pairs, us): linear
+// 4096 x 4096 1000 tokens 21.0 / 23.8, 1500 tokens 28.8 / 27.2, 8192 tokens 76.9 / 72.6; 1024 x 1024 4096 tokens
+// 14.7 / 15.6; FFN 2048/5504 4096 tokens 80.1 / 73.0; FFN 1024/2816 4096 tokens 36.2 / 38.7, 8192 tokens 55.7 / 55.0.
+static bool mx_pairs(int64_t M, int64_t k) {
   const int forced = tune_overrides().pair;
-  return forced >= 0 ? forced != 0 : M >= 2048;
+  return forced >= 0 ? forced != 0 : M >= 8192 || (k >= 2048 && M > 1024);
 }
 
 // Dynamic shared memory of a kernel, allowed once per device (the driver keeps the attribute).
@@ -968,13 +1004,21 @@ static int mx_launch_as(const MxMaps& maps, const MxParams& p, int64_t M, cudaSt
   cfg.blockDim = dim3(MX_THREADS);
   cfg.dynamicSmemBytes = MxGeom<CTAS>::smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CTAS;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (CTAS == 2) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = CTAS;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  if (M < 4096 && tune_overrides().early_start != 0) {
+    // few tiles leave SMs idle while the kernel before runs: set up beside it
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = CTAS == 2 ? 1 : 0;
+  cfg.numAttrs = n;
   return cuda_status(cudaLaunchKernelEx(&cfg, mx_gemm_kernel<EPI, CTAS>, maps, p));
 }
 
@@ -984,19 +1028,24 @@ static int mx_launch(const MxMaps& maps, const MxParams& p, int64_t M, bool pair
   return pairs ? mx_launch_as<EPI, 2>(maps, p, M, stream) : mx_launch_as<EPI, 1>(maps, p, M, stream);
 }
 
-// The small kernel takes a problem whose 128 x 128 tiles (both matrices of a gate/up pair counted) leave it to be split
-// over two CTAs an SM; the number of ranges is the largest power of two that fits, with at least `kMxMinSteps` k-steps each.
-constexpr int kMxMinSteps = 2;
+// Ranges of the contraction for the small kernel, 0: not the small kernel, which takes calls of one row tile a modality.
+// Measured (whole call by graph replay, small / 128 x 256 tiles, us): FFN 1024/2816 127 tokens 16.4 / 18.5, 200 tokens
+// 19.3 / 18.9, 512 tokens 24.5 / 19.7; FFN 4096/11008 1 token 23.4 / 38.3, 127 tokens 49.6 / 51.1, 200 tokens 57.4 / 52.2;
+// linear 4096 x 4096 1 token 7.4 / 12.3, 127 tokens 13.7 / 15.5, 256 tokens 17.6 / 16.9.
+// The number of ranges: as many as fill the places on the GPU once (two CTAs an SM), at most four, which always beat
+// eight (linear 4096 x 4096, 64 tokens: 1 / 2 / 4 / 8 ranges 13.3 / 11.0 / 10.7 / 18.6 us).  Gate/up tiles add up two
+// matrices and come out in 4 bits, a longer tail, so they take two ranges only where those CTAs nearly fit one an SM
+// (FFN 512/1024, 64 tokens: 12.3 / 11.5 / 12.0 us with 1 / 2 / 4; FFN 4096/11008, 8 tokens 38.0 / 38.4 / 49.5 us).
+constexpr int kMxSmallTokens = 128;
 static int mx_small_splits(int64_t M, int64_t n_out, int64_t k, bool glu) {
   const int forced = tune_overrides().narrow;
-  if (forced == 0) return 0;
-  const int64_t m_tiles = M <= 1 ? 1 : (M + MX_BM - 1) / MX_BM + (M <= MX_BM ? 1 : 0);
+  if (forced == 0 || (M > kMxSmallTokens && forced < 0)) return 0;
+  const int64_t m_tiles = (M + MX_BM - 1) / MX_BM + (M > 1 ? 1 : 0);
   const int64_t tiles = m_tiles * ((n_out + MXS_N - 1) / MXS_N) * (glu ? 2 : 1);
-  const int64_t slots = 2 * usable_sms();
+  const int64_t most = glu ? usable_sms() * 5 / 4 : 2 * usable_sms();
   const int64_t steps = (mx_code_ld(k) + 127) / 128;
-  if (M > 512 && forced < 0) return 0;
   int splits = 1;
-  while (2 * splits * (glu ? 2 : 1) <= 8 && tiles * splits * 2 <= slots && steps / (splits * 2) >= kMxMinSteps) splits *= 2;
+  while (splits < (glu ? 2 : 4) && tiles * splits * 2 <= most && steps >= splits * 2) splits *= 2;
   return splits;
 }
 
@@ -1027,14 +1076,14 @@ static int mx_launch_small(const MxMaps& maps, const MxParams& p, int64_t M, con
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = tune_overrides().early_start != 0 ? 2 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, mx_small_kernel<GLU>, maps, p, q));
 }
 
 // y[token] = routed rows of (codes, scales) by the modality's weight [N, K]
 static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt, const int32_t* perm, const int32_t* counts,
                       const void* mask, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int32_t* status, cudaStream_t s) {
-  const bool pairs = mx_pairs(M);
+  const bool pairs = mx_pairs(M, K);
   const int splits = mx_small_splits(M, N, K, false);
   const MxWeight w[2] = {wv, wt};
   const int slots[2] = {0, 2};
@@ -1062,7 +1111,7 @@ static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* p
                      void* scales, const void* mask, void* t1, void* t3, int64_t M, int64_t d, int64_t h, int32_t* status, cudaStream_t s) {
   const int slots[4] = {0, 1, 2, 3};
   const int splits = mx_small_splits(M, h, d, true);
-  const bool pairs = mx_pairs(M);
+  const bool pairs = mx_pairs(M, d);
   MxMaps m{};
   const int r = mx_maps(m, a, M, w, slots, 4, h, d, mx_a_box_rows(M), MX_BN / 2, pairs && !splits ? 1 : 0);
   if (r) return r;

@@ -14,7 +14,7 @@ the identity); the weights are frozen.  A block that holds an infinity or a NaN 
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
+from functools import lru_cache
 
 import torch
 from torch.autograd import Function
@@ -30,9 +30,27 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _Six = ctypes.c_void_p * 6
 
 
-def _on(dev):
-    """Makes ``dev`` the current device for the block (nothing to do where it is already)."""
-    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+@lru_cache(maxsize=1024)
+def _workspace_bytes(M: int, K: int, h: int) -> int:
+    return lib().ffnk_mxfp4_workspace_bytes(M, K, h)
+
+
+@lru_cache(maxsize=1024)
+def _backward_bytes(M: int, K: int, N: int, h: int) -> int:
+    return lib().ffnk_mxfp4_backward_workspace_bytes(M, K, N, h)
+
+
+def _elsewhere(dev) -> bool:
+    """Is ``dev`` another device than the current one?  (Then the call is made again with it current.)"""
+    return torch.cuda.current_device() != dev.index
+
+
+def _rows(t, name):
+    """``_activation`` with the common case, a contiguous matrix with 16-byte rows, decided at once."""
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.is_cuda and t.dim() == 2 and t.is_contiguous()
+            and not t.shape[1] & 7 and not t.data_ptr() & 15):
+        return t
+    return _activation(t, name)
 
 
 class MXFP4Tensor:
@@ -88,13 +106,16 @@ def quantize_mxfp4(x: torch.Tensor, dim: int = 1) -> MXFP4Tensor:
     if dim in (0, -2):
         rows, cols, rs, cs = cols, rows, cs, rs
     dev = x.device
-    with _on(dev):
-        codes = torch.empty((rows, -(-cols // 32) * 16), dtype=torch.uint8, device=dev)
-        scales = torch.empty((-(-rows // 128), -(-cols // 128), 32, 4, 4), dtype=torch.uint8, device=dev)
-        check("ffnk_mxfp4_quantize", lib().ffnk_mxfp4_quantize(
-            x.data_ptr(), _DTYPES[x.dtype], rs, cs, rows, cols, codes.data_ptr(), scales.data_ptr(),
-            stream_ptr(dev)))
-    return MXFP4Tensor(codes, scales, rows, cols)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return quantize_mxfp4(x, 1 if dim in (1, -1) else 0)
+    codes = torch.empty((rows, -(-cols // 32) * 16), dtype=torch.uint8, device=dev)
+    scales = torch.empty((-(-rows // 128), -(-cols // 128), 32, 4, 4), dtype=torch.uint8, device=dev)
+    q = MXFP4Tensor.__new__(MXFP4Tensor)
+    q.codes, q.scales, q.rows, q.cols, q.device, q.ptrs = codes, scales, rows, cols, dev, (codes.data_ptr(), scales.data_ptr())
+    check("ffnk_mxfp4_quantize", lib().ffnk_mxfp4_quantize(
+        x.data_ptr(), _DTYPES[x.dtype], rs, cs, rows, cols, *q.ptrs, stream_ptr(dev)))
+    return q
 
 
 def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -104,10 +125,12 @@ def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> tor
     if dtype not in _DTYPES:
         raise RuntimeError(f"dtype must be torch.bfloat16, torch.float16 or torch.float32, got {dtype}")
     dev = q.device
-    with _on(dev):
-        out = torch.empty((q.rows, q.cols), dtype=dtype, device=dev)
-        check("ffnk_mxfp4_dequantize", lib().ffnk_mxfp4_dequantize(
-            *q.ptrs, q.rows, q.cols, out.data_ptr(), _DTYPES[dtype], q.cols, stream_ptr(dev)))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return dequantize_mxfp4(q, dtype)
+    out = torch.empty((q.rows, q.cols), dtype=dtype, device=dev)
+    check("ffnk_mxfp4_dequantize", lib().ffnk_mxfp4_dequantize(
+        *q.ptrs, q.rows, q.cols, out.data_ptr(), _DTYPES[dtype], q.cols, stream_ptr(dev)))
     return out
 
 
@@ -115,7 +138,7 @@ def _check_weights(ws, names, shapes, dev):
     for w, n, s in zip(ws, names, shapes):
         if not isinstance(w, MXFP4Tensor):
             raise RuntimeError(f"{n} must be an MXFP4Tensor, got {type(w).__name__}")
-        if (w.rows, w.cols) != s:
+        if w.rows != s[0] or w.cols != s[1]:
             raise RuntimeError(f"{n} must have shape {list(s)} ([out, in]), got [{w.rows}, {w.cols}]")
         if w.device != dev:
             raise RuntimeError(f"{n} must be on the same device as the activations")
@@ -124,9 +147,9 @@ def _check_weights(ws, names, shapes, dev):
 def _check_mask(mask, M, dev):
     if not isinstance(mask, torch.Tensor) or mask.dim() != 1 or mask.shape[0] != M or mask.device != dev:
         raise RuntimeError(f"mask must have shape [{M}] on {dev}")
-    if mask.dtype not in (torch.bool, torch.uint8):
+    if mask.dtype is not torch.bool and mask.dtype is not torch.uint8:
         raise RuntimeError(f"mask must be torch.bool (or uint8), got {mask.dtype}")
-    return mask.contiguous()
+    return mask if mask.is_contiguous() else mask.contiguous()
 
 
 def _scratch(nbytes, M, dev, keep: bool):
@@ -145,44 +168,46 @@ def _scratch(nbytes, M, dev, keep: bool):
 
 def _mxfp4_linear_forward(a, b1, b2, mask, keep: bool = False):
     """y[m] = Q(a[m]) @ (b1 if mask[m] else b2).T -> (y [M, N] bf16, routing lists if ``keep``)."""
-    a = _activation(a, "a")
+    a = _rows(a, "a")
     M, K = a.shape
     dev = a.device
     N = b1.rows if isinstance(b1, MXFP4Tensor) else -1
-    _check_weights((b1, b2), ("b1", "b2"), ((N, K),) * 2, dev)
-    _check_dims(K=K, N=N)
+    _check_weights((b1, b2), ("b1", "b2"), ((N, K), (N, K)), dev)
+    if K & 7 or N & 7 or not K or not N:
+        _check_dims(K=K, N=N)
     mask = _check_mask(mask, M, dev)
-    L = lib()
-    with _on(dev):
-        y = a.new_empty((M, N))
-        if M == 0:
-            return y, None
-        nbytes = L.ffnk_mxfp4_workspace_bytes(M, K, 0)
-        ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
-        check("ffnk_mxfp4_linear_forward", L.ffnk_mxfp4_linear_forward(
-            a.data_ptr(), a.stride(0), *b1.ptrs, *b2.ptrs, mask.data_ptr(), perm, counts, wp, nbytes, y.data_ptr(), N, M, N, K,
-            status_word(dev).data_ptr(), stream_ptr(dev)))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _mxfp4_linear_forward(a, b1, b2, mask, keep)
+    y = a.new_empty((M, N))
+    if M == 0:
+        return y, None
+    nbytes = _workspace_bytes(M, K, 0)
+    ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
+    check("ffnk_mxfp4_linear_forward", lib().ffnk_mxfp4_linear_forward(
+        a.data_ptr(), a.stride(0), *b1.ptrs, *b2.ptrs, mask.data_ptr(), perm, counts, wp, nbytes, y.data_ptr(), N, M, N, K,
+        status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return y, lists
 
 
 def _mxfp4_linear_backward(g, b1, b2, lists):
     """dx[m] = g[m] @ (b1 if mask[m] else b2)."""
+    g = _rows(g, "grad")
     M, (N, K) = g.shape[0], b1.shape
-    g = _activation(g, "grad")
     dev = g.device
-    L = lib()
-    with _on(dev):
-        dx = torch.empty((M, K), device=dev, dtype=torch.bfloat16)
-        if M == 0:
-            return dx
-        nbytes = L.ffnk_mxfp4_backward_workspace_bytes(M, K, N, 0)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        perm = lists.data_ptr()
-        check("ffnk_mxfp4_linear_backward", L.ffnk_mxfp4_linear_backward(
-            g.data_ptr(), g.stride(0), *b1.ptrs, *b2.ptrs,
-            perm, perm + 4 * (lists.numel() - 8), ws.data_ptr(), nbytes, dx.data_ptr(), K, M, N, K,
-            status_word(dev).data_ptr(), stream_ptr(dev)))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _mxfp4_linear_backward(g, b1, b2, lists)
+    dx = g.new_empty((M, K))
+    if M == 0:
+        return dx
+    nbytes = _backward_bytes(M, K, N, 0)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    perm = lists.data_ptr()
+    check("ffnk_mxfp4_linear_backward", lib().ffnk_mxfp4_linear_backward(
+        g.data_ptr(), g.stride(0), *b1.ptrs, *b2.ptrs, perm, perm + 4 * (lists.numel() - 8), ws.data_ptr(), nbytes, dx.data_ptr(),
+        K, M, N, K, status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return dx
 
@@ -192,27 +217,31 @@ _FFN_NAMES = ("w1", "w2", "w3", "u1", "u2", "u3")
 
 def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
     """The whole FFN forward -> (y [M, d] bf16, what the backward pass needs or None)."""
-    x = _activation(x, "x")
+    x = _rows(x, "x")
     M, d = x.shape
     dev = x.device
     h = ws6[0].rows if isinstance(ws6[0], MXFP4Tensor) else -1
-    _check_weights(ws6, _FFN_NAMES, ((h, d), (d, h), (h, d)) * 2, dev)
-    _check_dims(d=d, h=h)
+    _check_weights(ws6, _FFN_NAMES, ((h, d), (d, h), (h, d), (h, d), (d, h), (h, d)), dev)
+    if d & 7 or h & 7 or not d or not h:
+        _check_dims(d=d, h=h)
     mask = _check_mask(mask, M, dev)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _mxfp4_ffn_forward(x, ws6, mask, keep)
     L = lib()
-    with _on(dev):
-        y = x.new_empty((M, d))
-        if M == 0:
-            return y, (None, None, None)
-        nbytes = L.ffnk_mxfp4_workspace_bytes(M, d, h)
-        ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
-        t1 = t3 = None
-        if keep:
-            t1, t3 = (torch.empty(L.ffnk_mxfp4_kept_bytes(M, h), device=dev, dtype=torch.uint8) for _ in range(2))
-        check("ffnk_mxfp4_ffn_forward", L.ffnk_mxfp4_ffn_forward(
-            x.data_ptr(), x.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]),
-            mask.data_ptr(), perm, counts, wp, nbytes, t1.data_ptr() if keep else None,
-            t3.data_ptr() if keep else None, y.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
+    y = x.new_empty((M, d))
+    if M == 0:
+        return y, (None, None, None)
+    nbytes = _workspace_bytes(M, d, h)
+    ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
+    t1 = t3 = p1 = p3 = None
+    if keep:
+        n = L.ffnk_mxfp4_kept_bytes(M, h)
+        t1, t3 = torch.empty(n, device=dev, dtype=torch.uint8), torch.empty(n, device=dev, dtype=torch.uint8)
+        p1, p3 = t1.data_ptr(), t3.data_ptr()
+    check("ffnk_mxfp4_ffn_forward", L.ffnk_mxfp4_ffn_forward(
+        x.data_ptr(), x.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), mask.data_ptr(), perm,
+        counts, wp, nbytes, p1, p3, y.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return y, (lists, t1, t3)
 
@@ -220,20 +249,22 @@ def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
 def _mxfp4_ffn_backward(gy, ws6, saved):
     """Gradient of the activations."""
     lists, t1, t3 = saved
+    gy = _rows(gy, "grad")
     M, (h, d) = gy.shape[0], ws6[0].shape
-    gy = _activation(gy, "grad")
     dev = gy.device
-    L = lib()
-    with _on(dev):
-        dx = torch.empty((M, d), device=dev, dtype=torch.bfloat16)
-        if M == 0:
-            return dx
-        nbytes = L.ffnk_mxfp4_backward_workspace_bytes(M, d, d, h)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        perm = lists.data_ptr()
-        check("ffnk_mxfp4_ffn_backward", L.ffnk_mxfp4_ffn_backward(
-            gy.data_ptr(), gy.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), t1.data_ptr(), t3.data_ptr(), perm, perm + 4 * (lists.numel() - 8),
-            ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _mxfp4_ffn_backward(gy, ws6, saved)
+    dx = gy.new_empty((M, d))
+    if M == 0:
+        return dx
+    nbytes = _backward_bytes(M, d, d, h)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    perm = lists.data_ptr()
+    check("ffnk_mxfp4_ffn_backward", lib().ffnk_mxfp4_ffn_backward(
+        gy.data_ptr(), gy.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), t1.data_ptr(),
+        t3.data_ptr(), perm, perm + 4 * (lists.numel() - 8), ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h,
+        status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return dx
 
