@@ -19,6 +19,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace ffnk {
 
 constexpr int kMxBlock = 32;        // values per scale
@@ -82,6 +84,69 @@ __device__ __forceinline__ void mx_unpack8(uint32_t c, float (&v)[8]) {
     v[2 * i] = f.x;
     v[2 * i + 1] = f.y;
   }
+}
+
+// A lane holds 32 bytes of a row, one 256-bit load: 16 values of a 16-bit type (two lanes a block) or 8 of fp32 (four).
+template <typename T> struct MxLane {
+  static constexpr int values = 32 / sizeof(T);
+  static constexpr int chunk = 32 * values;          // columns of one warp step
+  static constexpr int lanes_per_block = 32 / values;
+};
+struct MxRaw {
+  uint32_t w[8];
+};
+
+// Values c ... of a row; beyond `cols` zeros.  align: bytes the rows are aligned to (32, 16, or less).
+template <typename T>
+__device__ __forceinline__ MxRaw load_lane(const T* row, int c, int cols, int align) {
+  MxRaw r;
+  if (align >= 16 && c + MxLane<T>::values <= cols) {
+    if (align >= 32) {
+      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+                   : "l"(row + c));
+    } else {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c)), b = __ldg(reinterpret_cast<const uint4*>(row + c) + 1);
+      r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+      r.w[4] = b.x; r.w[5] = b.y; r.w[6] = b.z; r.w[7] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const int k = c + 2 * i;
+        const uint32_t lo = k < cols ? reinterpret_cast<const unsigned short*>(row)[k] : 0u;
+        const uint32_t hi = k + 1 < cols ? reinterpret_cast<const unsigned short*>(row)[k + 1] : 0u;
+        r.w[i] = lo | hi << 16;
+      } else {
+        r.w[i] = c + i < cols ? reinterpret_cast<const uint32_t*>(row)[c + i] : 0u;
+      }
+    }
+  }
+  return r;
+}
+
+// bits of the lane's max |x| as fp32 (16-bit types: packed integer maxima of two values at a time, converted once)
+template <typename T>
+__device__ __forceinline__ uint32_t absmax_bits(const MxRaw& r) {
+  constexpr uint32_t mask = sizeof(T) == 2 ? 0x7FFF7FFFu : 0x7FFFFFFFu;
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 2) m = __vmaxu2(m, r.w[i] & mask);
+    else m = max(m, r.w[i] & mask);
+  }
+  if constexpr (sizeof(T) == 2) m = max(m & 0xFFFFu, m >> 16);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return m << 16;
+  else if constexpr (sizeof(T) == 2) return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+  else return m;
+}
+
+template <typename T>
+__device__ __forceinline__ float raw_value(const MxRaw& r, int i) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? r.w[i >> 1] & 0xFFFF0000u : r.w[i >> 1] << 16);
+  else if constexpr (sizeof(T) == 2) return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? r.w[i >> 1] >> 16 : r.w[i >> 1])));
+  else return __uint_as_float(r.w[i]);
 }
 
 }  // namespace ffnk

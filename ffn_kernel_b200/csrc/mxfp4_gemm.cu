@@ -606,6 +606,11 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
 //
 // The weights do not depend on the kernel before this one: launched with programmatic stream serialization, a CTA
 // counts the mask itself, asks for its first stages of weights, and only then waits for the activations.
+//
+// SELF (a handful of tokens): no kernel before this one at all.  Every CTA finds its rows in the mask, rounds their part
+// of its contraction range to 4 bits straight into shared memory, in the layout TMA would have given it, while its
+// weights are on their way, and the first CTA leaves the routing lists.  One launch less: one token, linear
+// 4096 x 4096 7.5 -> 6.3 us, FFN 1024/2816 11.2 -> 10.0 us.
 // ---------------------------------------------------------------------------------------------
 constexpr int MXS_N = 128;
 constexpr int MXS_THREADS = 192;
@@ -613,7 +618,7 @@ constexpr int MXS_B_BYTES = MXS_N * 128;                    // 16 KiB
 constexpr int MXS_STAGE_FIXED = MXS_B_BYTES + 2 * MX_SF_BYTES;
 constexpr int MXS_MAX_STAGES = 6;
 constexpr int MXS_SMEM_STAGES = 104 * 1024;                 // stages, later the partial tile (at most 64 KiB)
-constexpr int MXS_SMEM = MXS_SMEM_STAGES + 256 + 1024;
+constexpr int MXS_SMEM = MXS_SMEM_STAGES + 256 + MX_BM * 4 + 1024;
 constexpr int MXS_MASK_MAX = 4096;                          // tokens a CTA counts itself
 constexpr uint32_t MXS_SFA = 128, MXS_SFB = 136;            // tensor-memory columns of the scales, behind the accumulator
 
@@ -634,11 +639,64 @@ struct MxSmall {
   const uint8_t* mask;    // null: M is larger than a CTA counts
   int M;
   int splits;             // ranges of the contraction; the cluster has splits (gate/up: 2 x splits) CTAs
-  int a_slot;             // bytes of a stage's A rows (a multiple of 1 KiB; what the MMA reads past them is B, in rows nobody stores)
+  int a_slot;             // bytes of a k-step's A rows (a multiple of 1 KiB; what the MMA reads past them is in rows nobody stores)
   int stages;
+  // SELF: the activations, the lists to leave, and how many k-steps of A rows shared memory is laid out for
+  const __nv_bfloat16* x;
+  int64_t ldx;
+  int K;
+  int x_align;
+  int a_steps;
+  int* perm;
+  int* counts;
+  int cap;
 };
 
-template <bool GLU>
+// Rows `tok[0..rows)` of x, columns of k-steps ks0 ... ks1, to 4 bits in shared memory: codes of k-step i at
+// a + i * a_slot as 128-byte rows with the 128-byte swizzle, scales at sa + i * 1 KiB as two atoms.  Four warps, units of
+// (row, two k-steps), the loads of four units of a warp in flight together.
+__device__ __forceinline__ void mx_self_quantize(const MxSmall& q, const int* tok, int rows, int ks0, int ks1, uint8_t* a, uint8_t* sa,
+                                                 int warp, int lane) {
+  using L = MxLane<__nv_bfloat16>;
+  const int groups = (ks1 - ks0 + 1) / 2, units = rows * groups;
+  for (int u0 = warp; u0 < units; u0 += 16) {
+    MxRaw raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int u = u0 + 4 * i;
+      if (u < units) {
+        const int row = u / groups, c = (ks0 + 2 * (u - row * groups)) * 256 + lane * L::values;
+        raw[i] = load_lane(q.x + static_cast<int64_t>(tok[row]) * q.ldx, c, q.K, q.x_align);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int u = u0 + 4 * i;
+      if (u >= units) break;                             // warp-uniform
+      const int row = u / groups, ks = 2 * (u - row * groups) + (lane >> 4);   // a k-step is 16 lanes
+      uint32_t m = absmax_bits<__nv_bfloat16>(raw[i]);
+      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+      const uint32_t byte = mx_scale_byte(m);
+      const float inv = mx_inverse_scale(byte);
+      uint32_t code[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = mul_keep_subnormals(raw_value<__nv_bfloat16>(raw[i], 8 * j + e), inv);
+        code[j] = byte == 255u ? 0u : mx_pack8(v);
+      }
+      if (ks0 + ks < ks1) {
+        const int piece = (lane & 15) >> 1;              // 16-byte piece of the row = block of the k-step
+        *reinterpret_cast<uint2*>(a + ks * q.a_slot + row * 128 + ((piece ^ (row & 7)) << 4) + (lane & 1) * 8) = make_uint2(code[0], code[1]);
+        if ((lane & 1) == 0)
+          sa[ks * MX_SF_BYTES + (piece >> 2) * kMxAtomBytes + (row & 31) * 16 + (row >> 5) * 4 + (piece & 3)] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+}
+
+template <bool GLU, bool SELF>
 __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_constant__ MxMaps maps, const MxParams p, const MxSmall q) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -647,6 +705,8 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
   uint64_t* done = empty + MXS_MAX_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_count = reinterpret_cast<int*>(tmem_slot + 2);           // one word a warp
+  int* s_tok = reinterpret_cast<int*>(smem + MXS_SMEM_STAGES + 256);   // SELF: tokens of this CTA's tile
 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
@@ -661,7 +721,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&maps.a);
+    if (!SELF) tma_prefetch_desc(&maps.a);
     tma_prefetch_desc(&maps.b[up]);
     tma_prefetch_desc(&maps.b[2 + up]);
   }
@@ -673,12 +733,21 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
 
   // rows of each modality: counted here, or read from what the kernel before left
   int Mv;
-  if (q.mask) {
+  uint32_t vis = 0;                                       // SELF: the visual tokens among the 32 of this thread's warp
+  if (SELF || q.mask) {
     int n = 0;
-    for (int i = threadIdx.x; i < q.M; i += MXS_THREADS) n += q.mask[i] != 0 ? 1 : 0;
-    n = __reduce_add_sync(0xFFFFFFFFu, n);
-    int* s_count = reinterpret_cast<int*>(const_cast<int*>(abort_flag) + 1);
-    if (lane == 0) s_count[warp] = n;
+    if constexpr (SELF) {                                 // M <= 128: warp w < 4 holds tokens 32 w ... 32 w + 31
+      const int i = threadIdx.x;
+      vis = __ballot_sync(0xFFFFFFFFu, i < q.M && q.mask[i] != 0);
+      n = __popc(vis);
+    } else {
+      for (int i = threadIdx.x; i < q.M; i += MXS_THREADS) n += q.mask[i] != 0 ? 1 : 0;
+      n = __reduce_add_sync(0xFFFFFFFFu, n);
+    }
+    if (lane == 0) {
+      s_count[warp] = n;
+      if constexpr (SELF) s_count[MXS_THREADS / 32 + warp] = static_cast<int>(vis);
+    }
     tc_fence_before();
     __syncthreads();
     Mv = 0;
@@ -705,22 +774,53 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
   const int routed0 = (text ? mx_text_base(Mv) : 0) + row0;
   const int k_steps = (p.k_bytes + 127) / 128;
   const int ks0 = split * k_steps / q.splits, ks1 = work ? (split + 1) * k_steps / q.splits : ks0;
-  const int stage_bytes = q.a_slot + MXS_STAGE_FIXED;
+  // SELF: [A of every k-step][A scales of every k-step][stages of B, B scales]; else stages of A, B, A scales, B scales
+  const int stage_bytes = SELF ? MXS_B_BYTES + MX_SF_BYTES : q.a_slot + MXS_STAGE_FIXED;
+  const int b_base = SELF ? q.a_steps * (q.a_slot + MX_SF_BYTES) : q.a_slot;
+  constexpr int sb_off = SELF ? MXS_B_BYTES : MXS_B_BYTES + MX_SF_BYTES;   // of a stage's B scales behind its B codes
+
+  if constexpr (SELF) {
+    const int i = threadIdx.x;
+    if (i < q.M) {
+      int before = __popc(vis & ((1u << lane) - 1u));     // visual tokens before this one
+      for (int w = 0; w < warp; ++w) before += s_count[w];
+      const bool v = (vis >> lane) & 1u;
+      const int pos = v ? before : i - before;
+      if (v != text) s_tok[pos] = i;
+      if (blockIdx.x == 0) q.perm[(v ? 0 : q.cap) + pos] = i;
+    }
+    if (blockIdx.x == 0 && i == 0) {
+      int runs = 1;
+      for (int k = 0; k < q.M; k += 32) {                 // changes of modality between neighbouring tokens
+        const uint32_t v = static_cast<uint32_t>(s_count[MXS_THREADS / 32 + (k >> 5)]);
+        const int n = min(32, q.M - k);
+        runs += __popc((v ^ (v >> 1)) & ((1u << (n - 1)) - 1u));
+        if (k + 32 < q.M) runs += ((v >> 31) ^ static_cast<uint32_t>(s_count[MXS_THREADS / 32 + (k >> 5) + 1])) & 1u;
+      }
+      q.counts[0] = Mv;
+      q.counts[1] = Mt;
+      q.counts[2] = q.cap;
+      q.counts[3] = q.M;
+      q.counts[4] = runs;
+    }
+    __syncthreads();
+  }
 
   if (warp == 0) {
     const bool lead = elect_one();
     const CUtensorMap* mb = &maps.b[(text ? 2 : 0) + up];
     const uint8_t* sb = maps.sb[(text ? 2 : 0) + up];
-    const uint32_t code_bytes = p.a_rows * 128 + MXS_B_BYTES;
+    const uint32_t code_bytes = (SELF ? 0 : p.a_rows * 128) + MXS_B_BYTES;
     int issued = 0;
     auto load_b = [&](int ks, int stage) {
-      uint8_t* b = smem + stage * stage_bytes + q.a_slot;
+      uint8_t* b = smem + stage * stage_bytes + b_base;
       const uint32_t sf = mx_step_scale_bytes(ks, maps.k_atoms);
-      mbar_arrive_expect_tx(&full[stage], code_bytes + 2 * sf);
+      mbar_arrive_expect_tx(&full[stage], code_bytes + (SELF ? 1 : 2) * sf);
       tma_load_2d(b, mb, &full[stage], ks * 128, nt * MXS_N);
-      bulk_load(b + MXS_B_BYTES + MX_SF_BYTES, mx_scale_at(sb, nt, ks, maps.k_atoms), sf, smem_u32(&full[stage]));
+      bulk_load(b + sb_off, mx_scale_at(sb, nt, ks, maps.k_atoms), sf, smem_u32(&full[stage]));
     };
     auto load_a = [&](int ks, int stage) {
+      if constexpr (SELF) return;
       uint8_t* a = smem + stage * stage_bytes;
       tma_load_2d(a, &maps.a, &full[stage], ks * 128, routed0);
       bulk_load(a + q.a_slot + MXS_B_BYTES, mx_scale_at(maps.sa, routed0 >> 7, ks, maps.k_atoms),
@@ -765,8 +865,8 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    auto issue = [&](uint32_t a, int mmas, uint32_t accumulate) {
-      const uint32_t b = a + (q.a_slot >> 4), sa = b + (MXS_B_BYTES >> 4), sb = sa + (MX_SF_BYTES >> 4);
+    if constexpr (SELF) asm volatile("bar.sync 1, 160;" ::: "memory");        // the activations are in shared memory
+    auto issue = [&](uint32_t a, uint32_t b, uint32_t sa, uint32_t sb, int mmas, uint32_t accumulate) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (2 * j < mmas) {
@@ -789,14 +889,17 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
         break;
       }
       tc_fence_after();
-      const uint32_t a = lo0 + stage * (stage_bytes >> 4);
+      const uint32_t st = lo0 + stage * (stage_bytes >> 4);
+      const uint32_t b = st + (b_base >> 4), sb = b + (sb_off >> 4);
+      const uint32_t a = SELF ? lo0 + (ks - ks0) * (q.a_slot >> 4) : st;
+      const uint32_t sa = SELF ? lo0 + ((q.a_steps * q.a_slot + (ks - ks0) * MX_SF_BYTES) >> 4) : b + (MXS_B_BYTES >> 4);
       const int left = p.k_bytes - ks * 128;
       uint64_t* free_bar = &empty[stage];
       if (++stage == q.stages) { stage = 0; phase ^= 1; }
       ready = mbar_test(&full[stage], phase);
       if (lead) {
-        if (left >= 128) issue(a, 4, ks != ks0);
-        else issue(a, (left + 31) / 32, ks != ks0);
+        if (left >= 128) issue(a, b, sa, sb, 4, ks != ks0);
+        else issue(a, b, sa, sb, (left + 31) / 32, ks != ks0);
         umma_commit(free_bar);
       }
       __syncwarp();
@@ -804,6 +907,11 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
     if (lead && ok) umma_commit(done);
     __syncwarp();
   } else {
+    if constexpr (SELF) {
+      mx_self_quantize(q, s_tok, rows, ks0, ks1, smem, smem + q.a_steps * q.a_slot, warp - 2, lane);
+      fence_proxy_async_smem();
+      asm volatile("bar.sync 1, 160;" ::: "memory");
+    }
     // the partial tile to shared memory, [row][32 pieces of four columns], pieces XOR-swizzled by the row
     const int quarter = warp & 3, row = quarter * 32 + lane;
     if (quarter * 32 < rows) {
@@ -862,7 +970,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
       const int n0 = nt * MXS_N + lane * 4;
       if constexpr (!GLU) {
         if (n0 < p.n_out) {
-          const int64_t token = p.perm[(text ? p.counts[2] : 0) + row0 + row];
+          const int64_t token = SELF ? s_tok[row] : p.perm[(text ? p.counts[2] : 0) + row0 + row];
           *reinterpret_cast<uint2*>(p.out + token * p.ldo + n0) = make_uint2(mx_pack_bf16(g.x, g.y), mx_pack_bf16(g.z, g.w));
         }
       } else {
@@ -948,7 +1056,7 @@ static int mx_scale_map(CUtensorMap* m, const void* scales, int64_t rows, int64_
 static int mx_maps(MxMaps& m, const MxWeight& a, int64_t M, const MxWeight* w, const int* slots, int n, int64_t n_rows, int64_t k,
                    int a_box, int b_box, int pair_sb_box) {
   const int64_t a_rows = ffnk_route_capacity(M) + 512;
-  int r = mx_code_map(&m.a, a.codes, a_rows, k, a_box);
+  int r = a.codes ? mx_code_map(&m.a, a.codes, a_rows, k, a_box) : 0;     // no codes yet: the kernel rounds the rows itself
   if (r) return r;
   if (pair_sb_box && (r = mx_scale_map(&m.tsa, a.scales, a_rows, k, 1))) return r;
   m.sa = static_cast<const uint8_t*>(a.scales);
@@ -1049,8 +1157,24 @@ static int mx_small_splits(int64_t M, int64_t n_out, int64_t k, bool glu) {
   return splits;
 }
 
-template <bool GLU>
-static int mx_launch_small(const MxMaps& maps, const MxParams& p, int64_t M, const void* mask, int splits, cudaStream_t stream) {
+// The activations of a call that a small kernel rounds itself (SELF), and where it leaves the routing lists.
+struct MxSelf {
+  const void* x;
+  int64_t ldx;
+  int32_t* perm;
+  int32_t* counts;
+};
+// Does it?  Few enough (row, two k-steps) units a CTA that rounding them takes less than the weights do to arrive (at most
+// eight a warp), and room for all of A beside three stages of B.
+static bool mx_takes_self(int64_t M, int64_t k, int splits) {
+  if (splits == 0 || M > MX_BM || tune_overrides().permute == 0) return false;
+  const int64_t steps = ((mx_code_ld(k) + 127) / 128 + splits - 1) / splits;
+  return M * ((steps + 1) / 2) <= 32 && steps * (((M + 7) / 8) * 1024 + MX_SF_BYTES) + 3 * (MXS_B_BYTES + MX_SF_BYTES) <= MXS_SMEM_STAGES;
+}
+
+template <bool GLU, bool SELF>
+static int mx_launch_small(const MxMaps& maps, const MxParams& p, int64_t M, int64_t k, const void* mask, int splits, const MxSelf& self,
+                           cudaStream_t stream) {
   if (device_info().cc_major != 10) return FFNK_ERR_DEVICE;
   MxSmall q{};
   q.mask = M <= MXS_MASK_MAX ? static_cast<const uint8_t*>(mask) : nullptr;
@@ -1058,11 +1182,22 @@ static int mx_launch_small(const MxMaps& maps, const MxParams& p, int64_t M, con
   q.splits = splits;
   q.a_slot = (p.a_rows * 128 + 1023) & ~1023;
   q.stages = MXS_SMEM_STAGES / (q.a_slot + MXS_STAGE_FIXED);
+  if constexpr (SELF) {
+    q.x = static_cast<const __nv_bfloat16*>(self.x);
+    q.ldx = self.ldx;
+    q.K = static_cast<int>(k);
+    q.x_align = (reinterpret_cast<uintptr_t>(self.x) | static_cast<uintptr_t>(2 * self.ldx)) & 31 ? 16 : 32;
+    q.perm = self.perm;
+    q.counts = self.counts;
+    q.cap = static_cast<int>(ffnk_route_capacity(M));
+    q.a_steps = static_cast<int>(((mx_code_ld(k) + 127) / 128 + splits - 1) / splits);
+    q.stages = (MXS_SMEM_STAGES - q.a_steps * (q.a_slot + MX_SF_BYTES)) / (MXS_B_BYTES + MX_SF_BYTES);
+  }
   if (q.stages > MXS_MAX_STAGES) q.stages = MXS_MAX_STAGES;
   const int csize = GLU ? 2 * splits : splits;
   const int64_t tiles = ((M + MX_BM - 1) / MX_BM + (M > 1 ? 1 : 0)) * ((p.n_out + MXS_N - 1) / MXS_N);
   static std::atomic<uint64_t> allowed{0};
-  if (const int r = mx_allow_smem(mx_small_kernel<GLU>, MXS_SMEM, allowed)) return r;
+  if (const int r = mx_allow_smem(mx_small_kernel<GLU, SELF>, MXS_SMEM, allowed)) return r;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * csize));
   cfg.blockDim = dim3(MXS_THREADS);
@@ -1076,13 +1211,14 @@ static int mx_launch_small(const MxMaps& maps, const MxParams& p, int64_t M, con
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = tune_overrides().early_start != 0 ? 2 : 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, mx_small_kernel<GLU>, maps, p, q));
+  cfg.numAttrs = !SELF && tune_overrides().early_start != 0 ? 2 : 1;    // SELF is a call's first kernel: it reads x at once
+  return cuda_status(cudaLaunchKernelEx(&cfg, mx_small_kernel<GLU, SELF>, maps, p, q));
 }
 
 // y[token] = routed rows of (codes, scales) by the modality's weight [N, K]
 static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt, const int32_t* perm, const int32_t* counts,
-                      const void* mask, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int32_t* status, cudaStream_t s) {
+                      const void* mask, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, const MxSelf* self, int32_t* status,
+                      cudaStream_t s) {
   const bool pairs = mx_pairs(M, K);
   const int splits = mx_small_splits(M, N, K, false);
   const MxWeight w[2] = {wv, wt};
@@ -1103,12 +1239,14 @@ static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt,
   p.group_m = mx_group_m(K, pairs ? 2 * MX_BM : MX_BM);
   p.out = static_cast<__nv_bfloat16*>(y);
   p.ldo = ldy;
-  return splits ? mx_launch_small<false>(m, p, M, mask, splits, s) : mx_launch<MX_EPI_STORE>(m, p, M, pairs, s);
+  if (self) return mx_launch_small<false, true>(m, p, M, K, mask, splits, *self, s);
+  return splits ? mx_launch_small<false, false>(m, p, M, K, mask, splits, MxSelf{}, s) : mx_launch<MX_EPI_STORE>(m, p, M, pairs, s);
 }
 
 // quantised silu(gate) * up of the routed rows, optionally with the pre-activations kept (t1, t3 both or neither)
 static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* perm, const int32_t* counts, void* codes,
-                     void* scales, const void* mask, void* t1, void* t3, int64_t M, int64_t d, int64_t h, int32_t* status, cudaStream_t s) {
+                     void* scales, const void* mask, void* t1, void* t3, int64_t M, int64_t d, int64_t h, const MxSelf* self,
+                     int32_t* status, cudaStream_t s) {
   const int slots[4] = {0, 1, 2, 3};
   const int splits = mx_small_splits(M, h, d, true);
   const bool pairs = mx_pairs(M, d);
@@ -1128,7 +1266,8 @@ static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* p
   p.t1 = static_cast<__half*>(t1);
   p.t3 = static_cast<__half*>(t3);
   p.pre_rows = ffnk_route_capacity(M) + 512;
-  if (splits) return mx_launch_small<true>(m, p, M, mask, splits, s);
+  if (self) return mx_launch_small<true, true>(m, p, M, d, mask, splits, *self, s);
+  if (splits) return mx_launch_small<true, false>(m, p, M, d, mask, splits, MxSelf{}, s);
   return t1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, pairs, s) : mx_launch<MX_EPI_GLU>(m, p, M, pairs, s);
 }
 
@@ -1185,10 +1324,13 @@ extern "C" int ffnk_mxfp4_linear_forward(const void* x, int64_t ldx, const void*
   const MxWorkspace w = mx_workspace(M, K, 0);
   if (workspace_bytes < w.total) return FFNK_ERR_CAPACITY;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  int r = mx_route_quantize(mask, M, x, ldx, K, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
+  const MxSelf self{x, ldx, perm, counts};
+  const bool takes = mx_takes_self(M, K, mx_small_splits(M, N, K, false));
+  int r = takes ? 0 : mx_route_quantize(mask, M, x, ldx, K, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
   if (r) return r;
-  return mx_product(MxWeight{ws + w.xc, ws + w.xs}, MxWeight{b1_codes, b1_scales}, MxWeight{b2_codes, b2_scales}, perm, counts,
-                    mask, y, ldy, M, N, K, status, static_cast<cudaStream_t>(stream));
+  return mx_product(takes ? MxWeight{} : MxWeight{ws + w.xc, ws + w.xs}, MxWeight{b1_codes, b1_scales},
+                    MxWeight{b2_codes, b2_scales}, perm, counts, mask, y, ldy, M, N, K, takes ? &self : nullptr, status,
+                    static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* const* codes, const void* const* scales,
@@ -1209,12 +1351,16 @@ extern "C" int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* co
   if (workspace_bytes < w.total) return FFNK_ERR_CAPACITY;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int r = mx_route_quantize(mask, M, x, ldx, d, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
+  const MxSelf self{x, ldx, perm, counts};
+  const bool takes = mx_takes_self(M, d, mx_small_splits(M, h, d, true));
+  int r = takes ? 0 : mx_route_quantize(mask, M, x, ldx, d, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
   if (r) return r;
   const MxWeight gu[4] = {{codes[0], scales[0]}, {codes[2], scales[2]}, {codes[3], scales[3]}, {codes[5], scales[5]}};
-  if ((r = mx_gateup(MxWeight{ws + w.xc, ws + w.xs}, gu, perm, counts, ws + w.hc, ws + w.hs, mask, t1, t3, M, d, h, status, s))) return r;
+  if ((r = mx_gateup(takes ? MxWeight{} : MxWeight{ws + w.xc, ws + w.xs}, gu, perm, counts, ws + w.hc, ws + w.hs, mask, t1, t3, M, d,
+                     h, takes ? &self : nullptr, status, s)))
+    return r;
   return mx_product(MxWeight{ws + w.hc, ws + w.hs}, MxWeight{codes[1], scales[1]}, MxWeight{codes[4], scales[4]}, perm, counts, mask,
-                    y, ldy, M, d, h, status, s);
+                    y, ldy, M, d, h, nullptr, status, s);
 }
 
 // ---------------------------------------------------------------------------------------------
