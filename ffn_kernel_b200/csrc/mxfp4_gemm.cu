@@ -89,11 +89,12 @@ struct MxParams {
   int k_bytes;             // code bytes of a row along the contraction (a multiple of 16)
   int a_rows;              // rows of an A box (fewer than 128 when no tile has more)
   int group_m;
-  // MX_EPI_STORE: out[token][n]; MX_EPI_GLU_SAVE: t1, t3 of pre_rows = cap + 512 routed rows (pre_tile_offset)
+  // MX_EPI_STORE: out[token][n]; MX_EPI_GLU_SAVE: the backward pass's factors f1, f3 of pre_rows =
+  // cap + 512 routed rows (pre_tile_offset)
   __nv_bfloat16* out;
   int64_t ldo;
-  __half* t1;
-  __half* t3;
+  __half* f1;
+  __half* f3;
   int64_t pre_rows;
   // MX_EPI_GLU*: codes [routed row][code_ld] and scales of the quantised product
   uint8_t* codes;
@@ -185,6 +186,15 @@ __device__ __forceinline__ void mx_store_rows(const float (&v)[32], unsigned lon
 // to four bits next must not sit on the wrong side of a tie more often than fp32 sums put it there anyway
 // (a hyperbolic tangent of 2^-11 would move one value in a thousand by a whole step).
 __device__ __forceinline__ float mx_silu_mul(float t1, float t3) { return __fdividef(t1, 1.0f + __expf(-t1)) * t3; }
+// The same value, and the two factors of the backward pass: f3 = dh/dt3 = silu(t1), f1 = dh/dt1 = t3 s (1 + t1 (1 - s)).
+__device__ __forceinline__ float mx_silu_mul_keep(float& t1, float& t3) {
+  const float d = 1.0f + __expf(-t1);
+  const float f3 = __fdividef(t1, d), s = __fdividef(1.0f, d);
+  const float h = f3 * t3;
+  t1 = t3 * fmaf(f3, 1.0f - s, s);
+  t3 = f3;
+  return h;
+}
 
 // One block (32 values of one row): scale byte and 16 bytes of codes.
 __device__ __forceinline__ uint32_t mx_quantize_block(const float (&v)[32], uint4& codes) {
@@ -228,12 +238,6 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag));
 }
 
-// Arrival at another CTA's barrier that hands over tensor memory only (tcgen05 fences order that).  A release at
-// cluster scope would first wait for this thread's global stores, the rows of the tile before: 1800 cycles a tile.
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
 __device__ __forceinline__ void mx_report(int* status, int code) {
   if (status) atomicCAS(status, 0, code);
 }
@@ -268,7 +272,7 @@ __device__ __forceinline__ void mx_issue_step(uint32_t d, uint32_t tmem, uint32_
   }
 }
 
-// One row's 32 pre-activations for the backward pass (pre_tile_offset: fp16 with a shared exponent).
+// One row's 32 factors for the backward pass (pre_tile_offset: fp16 with a shared exponent).
 __device__ __forceinline__ void mx_keep_block(const float (&v)[32], __half* base, int64_t pre_rows, int64_t row, int n0, int h) {
   uint32_t m = 0;
 #pragma unroll
@@ -333,17 +337,24 @@ __device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, c
         a[e] = __uint_as_float(g[e]);
         b[e] = __uint_as_float(u[e]);
       }
-      if constexpr (EPI == MX_EPI_GLU_SAVE) {
-        if (valid && n0 < p.n_out) {
-          mx_keep_block(a, p.t1, p.pre_rows, drow, n0, p.n_out);
-          mx_keep_block(b, p.t3, p.pre_rows, drow, n0, p.n_out);
-        }
-      }
+      float v[32];
       // columns past h are weight rows that do not exist: zeros, whatever their scales hold
+      if constexpr (EPI == MX_EPI_GLU_SAVE) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) a[e] = n0 + e < p.n_out ? mx_silu_mul(a[e], b[e]) : 0.0f;
+        for (int e = 0; e < 32; ++e) {
+          v[e] = mx_silu_mul_keep(a[e], b[e]);
+          if (n0 + e >= p.n_out) v[e] = a[e] = b[e] = 0.0f;
+        }
+        if (valid && n0 < p.n_out) {
+          mx_keep_block(a, p.f1, p.pre_rows, drow, n0, p.n_out);
+          mx_keep_block(b, p.f3, p.pre_rows, drow, n0, p.n_out);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = n0 + e < p.n_out ? mx_silu_mul(a[e], b[e]) : 0.0f;
+      }
       uint4 codes;
-      const uint32_t byte = mx_quantize_block(a, codes);
+      const uint32_t byte = mx_quantize_block(v, codes);
       const int block = tc.nt * (HALF / 32) + c;
       if (valid) {
         // every scale byte of an atom is written, also those of blocks past h (0): the next contraction reads them
@@ -975,13 +986,17 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
         }
       } else {
         const int64_t drow = routed0 + row;
-        if (p.t1) {                                         // uniform
+        float v[8] = {};
+        if (p.f1) {                                         // uniform: the factors of the backward pass are kept
+          float t[4] = {g.x, g.y, g.z, g.w}, w[4] = {u.x, u.y, u.z, u.w};
           uint32_t m1 = 0, m3 = 0;
           if (n0 < p.n_out) {
-            m1 = max(max(__float_as_uint(g.x) & 0x7FFFFFFFu, __float_as_uint(g.y) & 0x7FFFFFFFu),
-                     max(__float_as_uint(g.z) & 0x7FFFFFFFu, __float_as_uint(g.w) & 0x7FFFFFFFu));
-            m3 = max(max(__float_as_uint(u.x) & 0x7FFFFFFFu, __float_as_uint(u.y) & 0x7FFFFFFFu),
-                     max(__float_as_uint(u.z) & 0x7FFFFFFFu, __float_as_uint(u.w) & 0x7FFFFFFFu));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              v[i] = mx_silu_mul_keep(t[i], w[i]);
+              m1 = max(m1, __float_as_uint(t[i]) & 0x7FFFFFFFu);
+              m3 = max(m3, __float_as_uint(w[i]) & 0x7FFFFFFFu);
+            }
           }
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) {
@@ -992,19 +1007,17 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
           if (n0 < p.n_out) {
             const float i1 = pre_inverse_scale(k1), i3 = pre_inverse_scale(k3);
             const int64_t o = pre_tile_offset(drow, n0, p.n_out);
-            const __half2 h1[2] = {__floats2half2_rn(g.x * i1, g.y * i1), __floats2half2_rn(g.z * i1, g.w * i1)};
-            const __half2 h3[2] = {__floats2half2_rn(u.x * i3, u.y * i3), __floats2half2_rn(u.z * i3, u.w * i3)};
-            *reinterpret_cast<uint2*>(p.t1 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h1[0]), *reinterpret_cast<const uint32_t*>(&h1[1]));
-            *reinterpret_cast<uint2*>(p.t3 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h3[0]), *reinterpret_cast<const uint32_t*>(&h3[1]));
+            const __half2 h1[2] = {__floats2half2_rn(t[0] * i1, t[1] * i1), __floats2half2_rn(t[2] * i1, t[3] * i1)};
+            const __half2 h3[2] = {__floats2half2_rn(w[0] * i3, w[1] * i3), __floats2half2_rn(w[2] * i3, w[3] * i3)};
+            *reinterpret_cast<uint2*>(p.f1 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h1[0]), *reinterpret_cast<const uint32_t*>(&h1[1]));
+            *reinterpret_cast<uint2*>(p.f3 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h3[0]), *reinterpret_cast<const uint32_t*>(&h3[1]));
             if ((lane & 7) == 0) {
               const int64_t so = pre_scale_offset(drow, n0, p.n_out);
-              reinterpret_cast<uint8_t*>(p.t1 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k1);
-              reinterpret_cast<uint8_t*>(p.t3 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k3);
+              reinterpret_cast<uint8_t*>(p.f1 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k1);
+              reinterpret_cast<uint8_t*>(p.f3 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k3);
             }
           }
-        }
-        float v[8] = {};
-        if (n0 < p.n_out) {
+        } else if (n0 < p.n_out) {
           v[0] = mx_silu_mul(g.x, u.x);
           v[1] = mx_silu_mul(g.y, u.y);
           v[2] = mx_silu_mul(g.z, u.z);
@@ -1243,9 +1256,9 @@ static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt,
   return splits ? mx_launch_small<false, false>(m, p, M, K, mask, splits, MxSelf{}, s) : mx_launch<MX_EPI_STORE>(m, p, M, pairs, s);
 }
 
-// quantised silu(gate) * up of the routed rows, optionally with the pre-activations kept (t1, t3 both or neither)
+// quantised silu(gate) * up of the routed rows, optionally with the pre-activations kept (f1, f3 both or neither)
 static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* perm, const int32_t* counts, void* codes,
-                     void* scales, const void* mask, void* t1, void* t3, int64_t M, int64_t d, int64_t h, const MxSelf* self,
+                     void* scales, const void* mask, void* f1, void* f3, int64_t M, int64_t d, int64_t h, const MxSelf* self,
                      int32_t* status, cudaStream_t s) {
   const int slots[4] = {0, 1, 2, 3};
   const int splits = mx_small_splits(M, h, d, true);
@@ -1263,12 +1276,12 @@ static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* p
   p.scales = static_cast<uint8_t*>(scales);
   p.code_ld = mx_code_ld(h);
   p.k_atoms_out = static_cast<int>(mx_k_atoms(h));
-  p.t1 = static_cast<__half*>(t1);
-  p.t3 = static_cast<__half*>(t3);
+  p.f1 = static_cast<__half*>(f1);
+  p.f3 = static_cast<__half*>(f3);
   p.pre_rows = ffnk_route_capacity(M) + 512;
   if (self) return mx_launch_small<true, true>(m, p, M, d, mask, splits, *self, s);
   if (splits) return mx_launch_small<true, false>(m, p, M, d, mask, splits, MxSelf{}, s);
-  return t1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, pairs, s) : mx_launch<MX_EPI_GLU>(m, p, M, pairs, s);
+  return f1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, pairs, s) : mx_launch<MX_EPI_GLU>(m, p, M, pairs, s);
 }
 
 static int64_t mx_align(int64_t v) { return (v + 255) & ~int64_t(255); }
@@ -1335,15 +1348,15 @@ extern "C" int ffnk_mxfp4_linear_forward(const void* x, int64_t ldx, const void*
 
 extern "C" int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* const* codes, const void* const* scales,
                                       const void* mask, int32_t* perm, int32_t* counts, void* workspace,
-                                      int64_t workspace_bytes, void* t1, void* t3, void* y, int64_t ldy, int64_t M, int64_t d,
+                                      int64_t workspace_bytes, void* f1, void* f3, void* y, int64_t ldy, int64_t M, int64_t d,
                                       int64_t h, int32_t* status, void* stream) {
   if (M == 0) return 0;
-  if (!x || !codes || !scales || !mask || !perm || !counts || !workspace || !y || !status || !t1 != !t3) return FFNK_ERR_NULL;
+  if (!x || !codes || !scales || !mask || !perm || !counts || !workspace || !y || !status || !f1 != !f3) return FFNK_ERR_NULL;
   for (int i = 0; i < 6; ++i)
     if (!codes[i] || !scales[i]) return FFNK_ERR_NULL;
   if (M < 0 || M >= (1ll << 30) || mx_bad_dim(d) || mx_bad_dim(h)) return FFNK_ERR_SHAPE;
-  if ((ldx & 7) || (ldy & 7) || ldx < d || ldy < d || misaligned(x) || misaligned(y) || misaligned(perm) || misaligned(t1) ||
-      misaligned(t3) || (reinterpret_cast<uintptr_t>(workspace) & 255))
+  if ((ldx & 7) || (ldy & 7) || ldx < d || ldy < d || misaligned(x) || misaligned(y) || misaligned(perm) || misaligned(f1) ||
+      misaligned(f3) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return FFNK_ERR_ALIGN;
   for (int i = 0; i < 6; ++i)
     if (misaligned(codes[i]) || misaligned(scales[i])) return FFNK_ERR_ALIGN;
@@ -1356,7 +1369,7 @@ extern "C" int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* co
   int r = takes ? 0 : mx_route_quantize(mask, M, x, ldx, d, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
   if (r) return r;
   const MxWeight gu[4] = {{codes[0], scales[0]}, {codes[2], scales[2]}, {codes[3], scales[3]}, {codes[5], scales[5]}};
-  if ((r = mx_gateup(takes ? MxWeight{} : MxWeight{ws + w.xc, ws + w.xs}, gu, perm, counts, ws + w.hc, ws + w.hs, mask, t1, t3, M, d,
+  if ((r = mx_gateup(takes ? MxWeight{} : MxWeight{ws + w.xc, ws + w.xs}, gu, perm, counts, ws + w.hc, ws + w.hs, mask, f1, f3, M, d,
                      h, takes ? &self : nullptr, status, s)))
     return r;
   return mx_product(MxWeight{ws + w.hc, ws + w.hs}, MxWeight{codes[1], scales[1]}, MxWeight{codes[4], scales[4]}, perm, counts, mask,
@@ -1422,15 +1435,15 @@ extern "C" int ffnk_mxfp4_linear_backward(const void* g, int64_t ldg, const void
 }
 
 extern "C" int ffnk_mxfp4_ffn_backward(const void* gy, int64_t ldg, const void* const* codes, const void* const* scales,
-                                       const void* t1, const void* t3, const int32_t* perm, const int32_t* counts,
+                                       const void* f1, const void* f3, const int32_t* perm, const int32_t* counts,
                                        void* workspace, int64_t workspace_bytes, void* dx, int64_t lddx, int64_t M, int64_t d,
                                        int64_t h, int32_t* status, void* stream) {
   if (M == 0) return 0;
-  if (!gy || !codes || !scales || !t1 || !t3 || !perm || !counts || !workspace || !dx || !status) return FFNK_ERR_NULL;
+  if (!gy || !codes || !scales || !f1 || !f3 || !perm || !counts || !workspace || !dx || !status) return FFNK_ERR_NULL;
   for (int i = 0; i < 6; ++i)
     if (!codes[i] || !scales[i]) return FFNK_ERR_NULL;
   if (M < 0 || M >= (1ll << 30) || mx_bad_dim(d) || mx_bad_dim(h)) return FFNK_ERR_SHAPE;
-  if ((ldg & 7) || (lddx & 7) || ldg < d || lddx < d || misaligned(gy) || misaligned(dx) || misaligned(t1) || misaligned(t3) ||
+  if ((ldg & 7) || (lddx & 7) || ldg < d || lddx < d || misaligned(gy) || misaligned(dx) || misaligned(f1) || misaligned(f3) ||
       (reinterpret_cast<uintptr_t>(workspace) & 255))
     return FFNK_ERR_ALIGN;
   for (int i = 0; i < 6; ++i)
@@ -1448,6 +1461,6 @@ extern "C" int ffnk_mxfp4_ffn_backward(const void* gy, int64_t ldg, const void* 
   }
   const int r = mx_dequantize_weights(codes, scales, rows, cols, gate, 6, counts, wd, stream);
   if (r) return r;
-  return ffn_backward_dx(gy, ldg, t1, t3, wd[0], wd[1], wd[2], wd[3], wd[4], wd[5], perm, counts, ws + w.gr, ws + w.dt1,
+  return ffn_backward_dx(gy, ldg, f1, f3, wd[0], wd[1], wd[2], wd[3], wd[4], wd[5], perm, counts, ws + w.gr, ws + w.dt1,
                          ws + w.dt3, dx, lddx, M, d, h, status, stream);
 }

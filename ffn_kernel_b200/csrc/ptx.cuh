@@ -46,10 +46,12 @@ __device__ __forceinline__ bool mask_is_scattered(const int* counts, int run_thr
   return static_cast<long long>(counts[4]) * run_threshold > counts[3];
 }
 
-// Pre-activations kept between the forward and the backward pass of the FFN on 4-bit weights: fp16 with one power of
-// two per row and 32 columns (byte b stands for 2^(b - 127)), chosen so that the largest of the 32 lands in [2^14, 2^15).
-// bf16 copies would add as much error to dx as its own rounding does, fp32 ones are twice the traffic; the shared
-// exponent keeps 11 bits for everything down to 2^-28 of the largest and leaves no value out of range.
+// What the FFN on 4-bit weights keeps between its passes: the two factors dh/dt1 and dh/dt3 of h = silu(t1) t3, in fp16
+// with one power of two per row and 32 columns (byte b stands for 2^(b - 127)), chosen so that the largest of the 32 lands
+// in [2^14, 2^15).  bf16 would add as much error to dx as its own rounding does, fp32 is twice the traffic (4099 tokens,
+// 1024/2816: that GEMM 58 us against 41); the shared exponent keeps 11 bits for everything down to 2^-28 of the
+// largest and leaves no value out of range.  The factors rather than t1 and t3, because the forward pass has the exponential
+// already (its kernel takes 27 us with both stores) and the backward pass's epilogue then is two products (41 us).
 //   values  element (routed row, column) at pre_tile_offset: tiles of 128 rows x 8 columns
 //   scales  byte (routed row, column / 32) at pre_scale_offset, behind the (cap + 512) * h values
 // so that the 32 rows of a warp are 512 (scales: 32) contiguous bytes.
@@ -92,6 +94,11 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
 // arrive on a barrier in another CTA of the cluster (address from mapa)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Arrival at another CTA's barrier that hands over tensor memory only (tcgen05 fences order that).  A release at
+// cluster scope would first wait for this thread's global stores, the rows of the tile before: 1800 cycles a tile.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ uint32_t mapa_shared(uint32_t cta_addr, uint32_t cta_rank) {
   uint32_t r;

@@ -64,7 +64,8 @@ enum { A_GATHER = 0, A_ROUTED = 1 };
 // EPI_DSWIGLU     : acc = dH; with t1 = aux0, t3 = aux1 at the same position:
 //                   out = dH * t3 * s * (1 + t1 * (1 - s)),  aux2 = dH * t1 * s,  s = sigmoid(t1)
 //                   (the element-wise terms of the FFN backward, reference README.md:159-172)
-// EPI_DSWIGLU_PRE : the same with t1, t3 as the forward pass on 4-bit weights keeps them (pre_tile_offset, ptx.cuh)
+// EPI_DSWIGLU_PRE : out = dH * f1, aux2 = dH * f3 with the factors f1 = t3 s (1 + t1 (1 - s)) and f3 = t1 s as the forward
+//                   pass on 4-bit weights keeps them in aux0, aux1 (pre_tile_offset, ptx.cuh)
 enum { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_SWIGLU_SAVE = 2, EPI_DSWIGLU = 3, EPI_DSWIGLU_PRE = 4 };
 __host__ __device__ constexpr bool epi_glu(int e) { return e == EPI_SWIGLU || e == EPI_SWIGLU_SAVE; }
 // OUT_SCATTER : row of token t -> out[t]            OUT_ROUTED : row i of the routed order -> out[i]
@@ -310,8 +311,9 @@ __device__ __forceinline__ void epilogue_glu_staged(uint32_t taddr, const GemmPa
 // the saved pre-activations as well as for the two stores: four accesses per element, each of which
 // would otherwise touch 32 rows per instruction.
 //
-// PRE: t1 and t3 come in fp16 with a shared exponent per 32 columns instead, tiled so that a lane reads its own row:
-// the 32 lanes of a warp are 512 contiguous bytes an access and nothing is transposed.
+// PRE: instead of t1 and t3 the two factors come in, in fp16 with a shared exponent per 32 columns, tiled so that a lane
+// reads its own row: the 32 lanes of a warp are 512 contiguous bytes an access, nothing is transposed and nothing left to
+// do but two products.
 template <int BN_T, bool PRE = false>
 __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const GemmParams& p, long long row_off,
                                                         int n_base, int part, int parts, uint8_t* stg, int lane) {
@@ -422,6 +424,11 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
       const float dh = __uint_as_float(acc[e]);
+      if constexpr (PRE) {
+        t1[e] *= dh;
+        t3[e] *= dh;
+        continue;
+      }
       const float sg = sigmoid_fast(t1[e]);
       const float d1 = dh * t3[e] * sg * (1.0f + t1[e] * (1.0f - sg));
       t3[e] = dh * t1[e] * sg;     // d3
@@ -1149,7 +1156,7 @@ routed_gemm_pair_kernel(const __grid_constant__ AMaps am, const __grid_constant_
                                  smem + PAIR_STAGES * PAIR_STAGE_BYTES + 256 + (warp - 2) * 4096, lane);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+      if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&tempty[acc]), 0));
     }
     if (p.prof && warp == 2 && lane == 0) {
       p.prof[blockIdx.x * 8 + 5] = t_wait;
@@ -2391,7 +2398,7 @@ extern "C" int ffnk_ffn_forward_train(const void* x, int64_t ldx, const void* w1
 }
 
 namespace ffnk {
-// (dt1, dt3) = dswiglu(gr @ W2^T): contraction over d, output columns over h
+// (dt1, dt3) = dswiglu(gr @ W2^T): contraction over d, output columns over h; t1, t3 (or f1, f3) as EPI reads them
 template <int EPI>
 static int dswiglu_gemm(const void* gr, const void* w2, const void* u2, int64_t w2_stride_k, int64_t w2_stride_n, const void* t1,
                         const void* t3, const int32_t* perm, const int32_t* counts, void* dt1, void* dt3, int64_t M, int64_t d,
@@ -2482,14 +2489,14 @@ extern "C" int ffnk_ffn_backward(const void* gy, int64_t ldg, const void* xr, co
   return ffn_dx_gemm(dt1, dt3, w1, w3, u1, u3, w13_stride_k, w13_stride_n, perm, counts, dx, lddx, M, d, h, status, s);
 }
 
-int ffnk::ffn_backward_dx(const void* gy, int64_t ldg, const void* t1, const void* t3, const void* w1, const void* w2,
+int ffnk::ffn_backward_dx(const void* gy, int64_t ldg, const void* f1, const void* f3, const void* w1, const void* w2,
                           const void* w3, const void* u1, const void* u2, const void* u3, const int32_t* perm,
                           const int32_t* counts, void* gr, void* dt1, void* dt3, void* dx, int64_t lddx, int64_t M, int64_t d,
                           int64_t h, int32_t* status, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int r = ffnk_permute_rows(gy, ldg, perm, counts, gr, d, M, d, stream);
   if (r) return r;
-  if ((r = dswiglu_gemm<EPI_DSWIGLU_PRE>(gr, w2, u2, 1, h, t1, t3, perm, counts, dt1, dt3, M, d, h, status, s))) return r;
+  if ((r = dswiglu_gemm<EPI_DSWIGLU_PRE>(gr, w2, u2, 1, h, f1, f3, perm, counts, dt1, dt3, M, d, h, status, s))) return r;
   return ffn_dx_gemm(dt1, dt3, w1, w3, u1, u3, 1, d, perm, counts, dx, lddx, M, d, h, status, s);
 }
 

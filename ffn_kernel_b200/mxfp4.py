@@ -234,21 +234,21 @@ def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
         return y, (None, None, None)
     nbytes = _workspace_bytes(M, d, h)
     ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
-    t1 = t3 = p1 = p3 = None
+    f1 = f3 = p1 = p3 = None
     if keep:
         n = L.ffnk_mxfp4_kept_bytes(M, h)
-        t1, t3 = torch.empty(n, device=dev, dtype=torch.uint8), torch.empty(n, device=dev, dtype=torch.uint8)
-        p1, p3 = t1.data_ptr(), t3.data_ptr()
+        f1, f3 = torch.empty(n, device=dev, dtype=torch.uint8), torch.empty(n, device=dev, dtype=torch.uint8)
+        p1, p3 = f1.data_ptr(), f3.data_ptr()
     check("ffnk_mxfp4_ffn_forward", L.ffnk_mxfp4_ffn_forward(
         x.data_ptr(), x.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), mask.data_ptr(), perm,
         counts, wp, nbytes, p1, p3, y.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
-    return y, (lists, t1, t3)
+    return y, (lists, f1, f3)
 
 
 def _mxfp4_ffn_backward(gy, ws6, saved):
     """Gradient of the activations."""
-    lists, t1, t3 = saved
+    lists, f1, f3 = saved
     gy = _rows(gy, "grad")
     M, (h, d) = gy.shape[0], ws6[0].shape
     dev = gy.device
@@ -262,8 +262,8 @@ def _mxfp4_ffn_backward(gy, ws6, saved):
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     perm = lists.data_ptr()
     check("ffnk_mxfp4_ffn_backward", lib().ffnk_mxfp4_ffn_backward(
-        gy.data_ptr(), gy.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), t1.data_ptr(),
-        t3.data_ptr(), perm, perm + 4 * (lists.numel() - 8), ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h,
+        gy.data_ptr(), gy.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), f1.data_ptr(),
+        f3.data_ptr(), perm, perm + 4 * (lists.numel() - 8), ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h,
         status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return dx

@@ -353,21 +353,21 @@ int ffnk_mxfp4_linear_forward(const void* x, int64_t ldx, const void* b1_codes, 
 /* Routed SwiGLU FFN on MXFP4 weights (compare ffnk_ffn_forward):
  *     y = Q(silu(Q(x) w1^T) * (Q(x) w3^T)) w2^T for visual tokens, u1, u3, u2 for text tokens
  * codes, scales: HOST arrays of six device pointers each, in the order w1, w2, w3, u1, u2, u3; w1, w3, u1, u3 are
- * [h, d], w2, u2 [d, h].  The hidden activation is quantised from fp32.  t1, t3: both null, or
- * ffnk_mxfp4_kept_bytes(M, h) bytes each, where the pre-activations are kept for the backward pass in a form of the
- * library's own (fp16 with a shared exponent per 32).  workspace: ffnk_mxfp4_workspace_bytes(M, d, h). */
+ * [h, d], w2, u2 [d, h].  The hidden activation is quantised from fp32.  f1, f3: both null, or
+ * ffnk_mxfp4_kept_bytes(M, h) bytes each, where the factors of the backward pass are kept in a form of the library's
+ * own (fp16 with a shared exponent per 32).  workspace: ffnk_mxfp4_workspace_bytes(M, d, h). */
 int64_t ffnk_mxfp4_kept_bytes(int64_t M, int64_t h);
 int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* const* codes, const void* const* scales,
                            const void* mask, int32_t* perm, int32_t* counts, void* workspace, int64_t workspace_bytes,
-                           void* t1, void* t3, void* y, int64_t ldy, int64_t M, int64_t d, int64_t h, int32_t* status,
+                           void* f1, void* f3, void* y, int64_t ldy, int64_t M, int64_t d, int64_t h, int32_t* status,
                            void* stream);
 
 /* Gradients of the activations of the two forward passes above, the weights being frozen and the rounding of
  * activations to 4 bits counting as the identity:
  *     linear: dx[m, :] = g[m, :] @ (mask[m] ? b1 : b2)
- *     ffn:    dh = gy w2, dt1 = dh * t3 * s * (1 + t1 * (1 - s)), dt3 = dh * t1 * s, s = sigmoid(t1),
- *             dx = dt1 w1 + dt3 w3      (per modality)
- * perm, counts (and t1, t3) as the forward call left them.  The weights of the modalities present are read back
+ *     ffn:    dh = gy w2, dt1 = dh * f1, dt3 = dh * f3, dx = dt1 w1 + dt3 w3      (per modality)
+ *             with f1 = t3 * s * (1 + t1 * (1 - s)), f3 = t1 * s, s = sigmoid(t1)
+ * perm, counts (and f1, f3) as the forward call left them.  The weights of the modalities present are read back
  * to bf16, exactly, in the workspace; the products are bf16 with fp32 sums.  workspace:
  * ffnk_mxfp4_backward_workspace_bytes(M, K, N, 0) for the linear layer, (M, d, d, h) for the FFN, 256-byte aligned. */
 int64_t ffnk_mxfp4_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t h);
@@ -376,7 +376,7 @@ int ffnk_mxfp4_linear_backward(const void* g, int64_t ldg, const void* b1_codes,
                                void* workspace, int64_t workspace_bytes, void* dx, int64_t lddx, int64_t M, int64_t N,
                                int64_t K, int32_t* status, void* stream);
 int ffnk_mxfp4_ffn_backward(const void* gy, int64_t ldg, const void* const* codes, const void* const* scales,
-                            const void* t1, const void* t3, const int32_t* perm, const int32_t* counts, void* workspace,
+                            const void* f1, const void* f3, const int32_t* perm, const int32_t* counts, void* workspace,
                             int64_t workspace_bytes, void* dx, int64_t lddx, int64_t M, int64_t d, int64_t h,
                             int32_t* status, void* stream);
 

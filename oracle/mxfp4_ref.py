@@ -142,9 +142,9 @@ def ffn(x, w, mask):
 def ffn_dx(g, x, w, mask):
     """Gradient of the activations, the roundings to 4 bits counting as the identity -> (dx, bound).
 
-    On the way: t1 and t3 kept in fp16 with a shared power of two per 32 (half a step 2^-11 relative, and 2^-39 of the
-    block's largest below its normal range); dH in fp32; sigmoid from a hyperbolic tangent good to 2^-11 relative, 2^-12 absolute in sigmoid;
-    dT1, dT3 rounded to bf16; fp32 sums; dx rounded to bf16."""
+    On the way: the factors f1 = dh/dt1 and f3 = dh/dt3 from fp32 t1, t3 and the exponential (as in `ffn`), kept in
+    fp16 with a shared power of two per 32 (half a step 2^-11 relative, and 2^-39 of the block's largest below its
+    normal range); dH in fp32; dT1, dT3 rounded to bf16; fp32 sums; dx rounded to bf16."""
     w1, w2, w3, u1, u2, u3 = w
     q = rounded(x.cpu().double())
     g = g.cpu().double()
@@ -154,16 +154,16 @@ def ffn_dx(g, x, w, mask):
     edh = 2 * U32 * g.shape[1] * by_rows(g.abs(), mask, w2.abs(), u2.abs())
     f1, f3 = t3 * s * (1 + t1 * (1 - s)), t1 * s
     d1, d3 = dh * f1, dh * f3
-    es = 2.0 ** -12
     et = 2 * U32 * q.shape[1]
     et1 = et * by_rows(q.abs(), mask, w1.T.abs(), u1.T.abs())
     et3 = et * by_rows(q.abs(), mask, w3.T.abs(), u3.T.abs())
-    top1, top3 = (_blocks(t).abs().amax(-1).repeat_interleave(32, 1)[:, : t.shape[1]] for t in (t1, t3))
-    et1 = et1 + 2.0 ** -11 * (t1.abs() + et1) + 2.0 ** -39 * top1
-    et3 = et3 + 2.0 ** -11 * (t3.abs() + et3) + 2.0 ** -39 * top3
-    # d f1 / d s = t3 (1 + t1 (1 - 2 s)), second order t1 t3; the slopes in t1 are below 1.1 (silu') and 0.5 (silu'')
-    ef1 = (t3.abs() + et3) * ((1 + t1 * (1 - 2 * s)).abs() * es + t1.abs() * es * es + 0.5 * et1) + 1.1 * et3
-    ef3 = t1.abs() * es + 1.1 * et1
+    # silu'(t1) is below 1.1, its slope below 0.5; 16 * U32 relative (and 2 * U32 |t1| from the exponential) of the terms
+    fine = 16 * U32 * (1 + t1.abs() / 8)
+    ef1 = 1.1 * et3 + 0.5 * (t3.abs() + et3) * et1 + fine * t3.abs() * (s + t1.abs() * s * (1 - s))
+    ef3 = 1.1 * et1 + fine * f3.abs()
+    top1, top3 = (_blocks(f).abs().amax(-1).repeat_interleave(32, 1)[:, : f.shape[1]] for f in (f1, f3))
+    ef1 = ef1 + 2.0 ** -11 * (f1.abs() + ef1) + 2.0 ** -38 * top1 + 2.0 ** -126
+    ef3 = ef3 + 2.0 ** -11 * (f3.abs() + ef3) + 2.0 ** -38 * top3 + 2.0 ** -126
     off1 = dh.abs() * ef1 + edh * (f1.abs() + ef1)
     off3 = dh.abs() * ef3 + edh * (f3.abs() + ef3)
     off1 = off1 + U16 * (d1.abs() + off1) + 8 * U32 * d1.abs() + 2.0 ** -126

@@ -72,7 +72,7 @@ def test_argument_errors_are_reported_before_any_launch(libffnk):
     assert b(p, 64, p, p, p, p, p, p, p, 16, p, 64, 4, 64, 64, p, None) == -8
     g = L.ffnk_mxfp4_ffn_forward
     assert g(p, 64, six, holes, p, p, p, p, big, None, None, p, 64, 4, 64, 64, p, None) == -1
-    assert g(p, 64, six, six, p, p, p, p, big, p, None, p, 64, 4, 64, 64, p, None) == -1       # t1 without t3
+    assert g(p, 64, six, six, p, p, p, p, big, p, None, p, 64, 4, 64, 64, p, None) == -1       # f1 without f3
     assert g(p, 64, six, six_odd, p, p, p, p, big, None, None, p, 64, 4, 64, 64, p, None) == -3
     assert g(p, 64, six, six, p, p, p, p, big, None, None, p, 64, 4, 64, 68, p, None) == -2
     assert g(p, 64, six, six, p, p, p, p, 16, None, None, p, 64, 4, 64, 64, p, None) == -8
