@@ -74,7 +74,7 @@ int ffn_gateup_early(const void* x, int64_t ldx, const void* w1, const void* w3,
                      int32_t* status, void* stream);
 
 // Routing of the mask and the activations in MXFP4 in routed order (codes [(cap + 512), ceil(d/32)*16], scales), in one
-// launch for masks of one routing tile.
+// launch for masks of up to 32768 tokens.
 int mx_route_quantize(const void* mask, int64_t M, const void* x, int64_t ldx, int64_t d, int32_t* perm, int32_t* counts,
                       void* scan, void* codes, void* scales, int32_t* status, void* stream);
 

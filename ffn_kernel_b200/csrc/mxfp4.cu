@@ -3,7 +3,7 @@
 //   mx_quantize_rows_kernel    x contiguous along the blocks: weights in nn.Linear storage, activations; with
 //                              routing lists the rows come out in routed order
 //   mx_route_quantize_kernel   routing, the copy into routed order and the quantisation of the activations in one
-//                              launch, for masks of one routing tile
+//                              launch, for masks of up to 32768 tokens
 //   mx_quantize_cols_kernel    x contiguous across the blocks: [in, out] weights
 //   mx_dequantize_kernel       codes and scales -> bf16 / fp16 / fp32
 //
@@ -126,47 +126,73 @@ __global__ void __launch_bounds__(kQuantThreads, kQuantPerSm) mx_quantize_rows_k
     for (int a = a0 + lane; a < a1; a += 32) *reinterpret_cast<uint32_t*>(scales + mx_scale_word(r, a, k_atoms)) = 0u;
 }
 
-// Routing and quantisation of the activations in one launch (M <= 8192): every CTA routes the whole mask for
-// itself in shared memory, CTA (0, 0) also writes perm and counts, then every warp quantises its share of the rows.
+// Routing and quantisation of the activations in one launch (M <= kMxRouteTokens).  Every CTA keeps the whole mask as bits
+// with the visual tokens before each word (8 KiB of shared memory), so a warp knows where a token's row goes without any
+// list: the tokens are taken in their own order, and each leaves its entry of the lists on the way.  (A compaction of the
+// whole mask in every CTA, as for the copy of bf16 rows, was bound by its shared-memory stores: 8192 x 4096 34 us, now
+// 20, from cold caches.  A routing kernel and then mx_quantize_rows_kernel take as long from 16384 tokens on, 35 us and
+// 68 us at 32768, in three launches.)
+constexpr int kMxRouteWords = 4;             // words of 32 tokens a thread, consecutive
+constexpr int kMxRouteTokens = kRouteThreads * 32 * kMxRouteWords;
 __global__ void __launch_bounds__(kRouteThreads, kQuantPerSm) mx_route_quantize_kernel(
     const uint8_t* __restrict__ mask, int M, int cap, int* __restrict__ perm, int* __restrict__ counts,
     const __nv_bfloat16* __restrict__ x, int64_t ldx, int cols, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
     int align, int per_warp) {
-  __shared__ int s_list[kRouteTile];   // visual tokens ascending, then text tokens ascending
+  __shared__ uint32_t s_bits[kRouteThreads * kMxRouteWords];   // token 32 i + k is visual: bit k of word i
+  __shared__ int s_before[kRouteThreads * kMxRouteWords];      // visual tokens before word i
   __shared__ int s_warp[kRouteThreads / 32];
   __shared__ int s_runs;
   const int tid = threadIdx.x, lane = tid & 31;
   const bool writer = blockIdx.x == 0 && blockIdx.y == 0;
   griddep_launch_dependents();
-  const ThreadTokens tt = load_thread_tokens(mask, M, tid * kRoutePerThread);
+  const int words = (M + kRouteThreads * 32 - 1) / (kRouteThreads * 32);
+  uint32_t bits[kMxRouteWords] = {};
+  int count = 0, runs = 0;
+#pragma unroll
+  for (int w = 0; w < kMxRouteWords; ++w) {
+    if (w < words) {
+      const ThreadTokens tt = load_thread_tokens(mask, M, (tid * words + w) * 32);
+      bits[w] = tt.bits;
+      count += __popc(tt.bits);
+      runs += tt.nruns;
+    }
+  }
   if (tid == 0) s_runs = 0;
   int Mv = 0;
-  const int ev = block_exclusive_scan(__popc(tt.bits), s_warp, &Mv);
+  int before = block_exclusive_scan(count, s_warp, &Mv);
+#pragma unroll
+  for (int w = 0; w < kMxRouteWords; ++w) {
+    if (w < words) {
+      s_bits[tid * words + w] = bits[w];
+      s_before[tid * words + w] = before;
+      before += __popc(bits[w]);
+    }
+  }
   if (writer) {
-    const int wr = __reduce_add_sync(0xFFFFFFFFu, tt.nruns);
+    const int wr = __reduce_add_sync(0xFFFFFFFFu, runs);
     if (lane == 0 && wr) atomicAdd(&s_runs, wr);
   }
-  compact_tile(s_list, s_list + Mv, 0, tt.bits, ev, tt.valid);
   __syncthreads();
-  const int Mt = M - Mv;
-  if (writer) {
-    for (int i = tid; i < Mv; i += kRouteThreads) perm[i] = s_list[i];
-    for (int i = tid; i < Mt; i += kRouteThreads) perm[cap + i] = s_list[Mv + i];
-    if (tid == 0) {
-      counts[0] = Mv;
-      counts[1] = Mt;
-      counts[2] = cap;
-      counts[3] = M;
-      counts[4] = s_runs;
-    }
+  if (writer && tid == 0) {
+    counts[0] = Mv;
+    counts[1] = M - Mv;
+    counts[2] = cap;
+    counts[3] = M;
+    counts[4] = s_runs;
   }
   const int text_base = ((Mv + 255) >> 8) << 8;
   const int chunks = (cols + MxLane<__nv_bfloat16>::chunk - 1) / MxLane<__nv_bfloat16>::chunk;
   const int first = blockIdx.y * per_warp, n = min(per_warp, chunks - first);
   const int step = gridDim.x * (kRouteThreads / 32), r0 = blockIdx.x * (kRouteThreads / 32) + (tid >> 5);
+  const bool lists = blockIdx.y == 0 && lane == 0;
   quantize_rows(x, ldx, align, cols, first, n, codes, scales, lane, [&](int i) {
-    const int r = r0 + i * step;
-    return r < M ? MxRowRef{s_list[r], r >= Mv ? text_base + (r - Mv) : r} : MxRowRef{-1, 0};
+    const int t = r0 + i * step;
+    if (t >= M) return MxRowRef{-1, 0};
+    const uint32_t word = s_bits[t >> 5];
+    const int visual = s_before[t >> 5] + __popc(word & ((1u << (t & 31)) - 1u));
+    const bool v = (word >> (t & 31)) & 1u;
+    if (lists) perm[v ? visual : cap + (t - visual)] = t;
+    return MxRowRef{t, v ? visual : text_base + (t - visual)};
   });
 }
 
@@ -389,7 +415,7 @@ int mx_route_quantize(const void* mask, int64_t M, const void* x, int64_t ldx, i
   const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
   uint8_t* c = static_cast<uint8_t*>(codes);
   uint8_t* sc = static_cast<uint8_t*>(scales);
-  if (M <= kRouteTile) {
+  if (M <= kMxRouteTokens) {
     const QuantShape q = quant_shape(M, d, MxLane<__nv_bfloat16>::chunk, kChunksMax, kQuantPerSm);
     mx_route_quantize_kernel<<<q.grid, kRouteThreads, 0, s>>>(static_cast<const uint8_t*>(mask), static_cast<int>(M),
                                                               static_cast<int>(ffnk_route_capacity(M)), perm, counts, xb, ldx,

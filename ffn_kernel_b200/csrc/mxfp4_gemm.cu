@@ -75,8 +75,6 @@ constexpr int MX_BM = 128;                    // rows of a CTA's tile
 constexpr int MX_BN = 256;                    // accumulator columns (gate/up tiles: 128 gate | 128 up)
 constexpr int MX_A_BYTES = MX_BM * 128;       // 16 KiB of codes
 constexpr int MX_SF_BYTES = 2 * kMxAtomBytes; // scales of 128 rows x one k-step
-constexpr int MX_THREADS = 320;               // producer, MMA, eight epilogue warps
-constexpr int MX_STAGING = 8 * 2048;          // one 32-row x 64-byte transposition buffer per epilogue warp
 
 enum { MX_EPI_STORE = 0, MX_EPI_GLU = 1, MX_EPI_GLU_SAVE = 2 };
 __host__ __device__ constexpr bool mx_glu(int e) { return e != MX_EPI_STORE; }
@@ -294,18 +292,18 @@ __device__ __forceinline__ void mx_keep_block(const float (&v)[32], __half* base
   reinterpret_cast<uint8_t*>(base + pre_rows * h)[pre_scale_offset(row, n0, h)] = static_cast<uint8_t>(byte);
 }
 
-// Epilogue of one warp: TMEM lane quarter q, columns of `part` (0/1 of two).  `on_shared` runs once after the
-// first chunk has been read (the chunk holding the columns the two accumulators share, for the part that has it).
-template <int EPI, class F>
+// Epilogue of one warp: TMEM lane quarter q, columns of `part` of PARTS.  `on_first` runs once after the first chunk has
+// been read (the chunk holding the columns the two accumulators share, for the part that has it).
+template <int EPI, int PARTS, class F>
 __device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, const MxTile& tc, int acc, int row, int part,
                                             unsigned long long dst, uint8_t* stg, int lane, F&& on_first) {
   const bool valid = row < tc.rows;
   if constexpr (!mx_glu(EPI)) {
-    constexpr int CH = MX_BN / 64;            // 32-column chunks per part
+    constexpr int CH = MX_BN / 32 / PARTS;    // 32-column chunks per part
 #pragma unroll 1
     for (int i = 0; i < CH; ++i) {
       // accumulator 0 shares its last chunk, accumulator 1 its first
-      const int c = acc == 0 ? (part ? 2 * CH - 1 - i : CH - 1 - i) : part * CH + i;
+      const int c = acc == 0 ? (part + 1) * CH - 1 - i : part * CH + i;
       uint32_t v[32];
       tmem_ld_32x32(taddr + c * 32, v);
       tmem_ld_wait();
@@ -319,12 +317,12 @@ __device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, c
     }
   } else {
     constexpr int HALF = MX_BN / 2;            // gate columns | up columns
-    constexpr int CH = HALF / 64;             // blocks of the product per part
+    constexpr int CH = HALF / 32 / PARTS;     // blocks of the product per part
     const int64_t drow = tc.routed0 + row;
 #pragma unroll 1
     for (int i = 0; i < CH; ++i) {
-      // shared columns: up block HALF/32 - 1 of accumulator 0 (part 1's last), gate block 0 of accumulator 1
-      const int c = acc == 0 ? (part ? 2 * CH - 1 - i : CH - 1 - i) : part * CH + i;
+      // shared columns: up block HALF/32 - 1 of accumulator 0 (the last part's last), gate block 0 of accumulator 1
+      const int c = acc == 0 ? (part + 1) * CH - 1 - i : part * CH + i;
       uint32_t g[32], u[32];
       tmem_ld_32x32(taddr + c * 32, g);
       tmem_ld_32x32(taddr + HALF + c * 32, u);
@@ -371,13 +369,18 @@ __device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, c
 // rows (gate/up: the leader the gate rows, the partner the up rows), 35 KiB a k-step instead of 51; the scales of all
 // 256 weight rows are needed in both.  The leader (rank 0) issues everything; its `full` barriers count both CTAs'
 // bytes, its commits free the stage and publish the accumulator in both, both epilogues report to its `tempty`.
-// Persistent, warp specialised: warp 0 producer (TMA), warp 1 scale copies and MMAs, warps 2..9 epilogue.
+// Persistent, warp specialised: warp 0 producer (TMA), warp 1 scale copies and MMAs, the other warps epilogue.
 // ---------------------------------------------------------------------------------------------
-template <int CTAS> struct MxGeom {
+// Eight epilogue warps, two a lane quarter: sixteen are slower at every size (FFN 1024/2816, 4099 tokens 39.6 -> 42.6 us,
+// 4096/11008, 16384 tokens 0.90 -> 0.94 ms).
+template <int EPI, int CTAS> struct MxGeom {
   static constexpr int b_bytes = MX_BN / CTAS * 128;
   static constexpr int stage_bytes = MX_A_BYTES + b_bytes + 3 * MX_SF_BYTES;
   static constexpr int stages = CTAS == 2 ? 5 : 4;
-  static constexpr int smem = stages * stage_bytes + MX_STAGING + 256 + 1024;
+  static constexpr int epi_warps = 8;
+  static constexpr int threads = 64 + 32 * epi_warps;
+  static constexpr int staging = mx_glu(EPI) ? 0 : epi_warps * 2048;     // a 32-row x 64-byte transposition buffer a warp
+  static constexpr int smem = stages * stage_bytes + staging + 256 + 1024;
 };
 
 template <int CTAS>
@@ -387,12 +390,12 @@ __device__ __forceinline__ void mx_load(void* dst, const CUtensorMap* m, uint64_
 }
 
 template <int EPI, int CTAS>
-__global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
-  using G = MxGeom<CTAS>;
+__global__ void __launch_bounds__(MxGeom<EPI, CTAS>::threads, 1) mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
+  using G = MxGeom<EPI, CTAS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + G::stages * G::stage_bytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(staging + MX_STAGING);
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + G::staging);
   uint64_t* empty = full + G::stages;
   uint64_t* tfull = empty + G::stages;     // accumulator ready for the epilogue [2]
   uint64_t* tempty = tfull + 2;            // the epilogue has read the first chunk of a tile
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&tfull[i], 1);
-    mbar_init(tempty, 8 * CTAS);
+    mbar_init(tempty, G::epi_warps * CTAS);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&maps.a);
@@ -583,7 +586,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_gemm_kernel(const __grid_con
       }
       tc_fence_after();
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + (acc ? MX_ACC1 : 0);
-      mx_epilogue<EPI>(taddr, p, tc, acc, row, part, dst, staging + (warp - 2) * 2048, lane, [&] {
+      mx_epilogue<EPI, G::epi_warps / 4>(taddr, p, tc, acc, row, part, dst, staging + (warp - 2) * 2048, lane, [&] {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -1119,11 +1122,11 @@ static int mx_launch_as(const MxMaps& maps, const MxParams& p, int64_t M, cudaSt
   int64_t units = ((M + MX_BM * CTAS - 1) / (MX_BM * CTAS) + 1) * ((p.n_out + n_per_tile - 1) / n_per_tile);
   if (units > usable_sms() / CTAS) units = usable_sms() / CTAS;
   static std::atomic<uint64_t> allowed{0};
-  if (const int r = mx_allow_smem(mx_gemm_kernel<EPI, CTAS>, MxGeom<CTAS>::smem, allowed)) return r;
+  if (const int r = mx_allow_smem(mx_gemm_kernel<EPI, CTAS>, MxGeom<EPI, CTAS>::smem, allowed)) return r;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(units * CTAS));
-  cfg.blockDim = dim3(MX_THREADS);
-  cfg.dynamicSmemBytes = MxGeom<CTAS>::smem;
+  cfg.blockDim = dim3(MxGeom<EPI, CTAS>::threads);
+  cfg.dynamicSmemBytes = MxGeom<EPI, CTAS>::smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;

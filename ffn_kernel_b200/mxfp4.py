@@ -50,7 +50,9 @@ def _rows(t, name):
     if (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.is_cuda and t.dim() == 2 and t.is_contiguous()
             and not t.shape[1] & 7 and not t.data_ptr() & 15):
         return t
-    return _activation(t, name)
+    t = _activation(t, name)
+    # a single row at an odd address counts as contiguous and comes back as it was
+    return t.clone() if t.data_ptr() & 15 else t
 
 
 class MXFP4Tensor:
@@ -285,14 +287,15 @@ class MXFP4MaskedLinear(Function):
 
     @staticmethod
     def forward(ctx, a, b1, b2, mask):
-        y, ctx.lists = _mxfp4_linear_forward(a, b1, b2, mask, keep=True)
+        y, lists = _mxfp4_linear_forward(a, b1, b2, mask, keep=True)
+        ctx.save_for_backward(lists)
         ctx.weights = (b1, b2)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return _mxfp4_linear_backward(grad, *ctx.weights, ctx.lists), None, None, None
+        return _mxfp4_linear_backward(grad, *ctx.weights, *ctx.saved_tensors), None, None, None
 
 
 class MXFP4MaskedFFN(Function):
@@ -310,10 +313,11 @@ class MXFP4MaskedFFN(Function):
     @staticmethod
     def forward(ctx, a, w1, w2, w3, u1, u2, u3, mask):
         ctx.weights = (w1, w2, w3, u1, u2, u3)
-        y, ctx.kept = _mxfp4_ffn_forward(a, ctx.weights, mask, keep=True)
+        y, kept = _mxfp4_ffn_forward(a, ctx.weights, mask, keep=True)
+        ctx.save_for_backward(*kept)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return (_mxfp4_ffn_backward(grad, ctx.weights, ctx.kept), *([None] * 7))
+        return (_mxfp4_ffn_backward(grad, ctx.weights, ctx.saved_tensors), *([None] * 7))

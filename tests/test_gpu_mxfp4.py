@@ -109,7 +109,7 @@ def inside(got, want_and_bound):
 
 
 MASKS = ["all_visual", "all_text", "alternating", "bernoulli", "span"]
-LINEAR_SIZES = [(1, 64, 64), (1, 4096, 264), (2, 8, 8), (7, 40, 136), (33, 1000, 72), (127, 264, 520), (128, 256, 256),
+LINEAR_SIZES = [(1, 64, 64), (3, 2056, 328), (1, 4096, 264), (2, 8, 8), (7, 40, 136), (33, 1000, 72), (127, 264, 520), (128, 256, 256),
                 (129, 128, 1032), (300, 2056, 328), (515, 96, 2048), (1030, 520, 264), (8200, 72, 64)]
 
 
@@ -245,6 +245,44 @@ def test_strided_activations_gradients_and_uint8_mask(dev):
     b = torch.autograd.grad(y, xg, torch.cat([g, g], 1)[:, :N], retain_graph=True)[0]      # strided upstream gradient
     c = torch.autograd.grad(y.sum(), xg)[0]                                                # an expanded one
     assert torch.equal(a, b) and torch.isfinite(c).all()
+
+
+@pytest.mark.parametrize("M", [1, 2, 5, 31, 32, 33, 64, 65, 127, 128, 129, 300, 9000])
+@pytest.mark.parametrize("kind", MASKS)
+def test_routing_lists_are_those_of_route(dev, M, kind):
+    # few tokens are routed inside the product's kernel (K <= 512: up to 32 of them), more by a kernel before it
+    from ffn_kernel_b200 import route
+    from ffn_kernel_b200.mxfp4 import _mxfp4_linear_forward
+    mask = edge_mask(M, kind, seed=M + 1).to(dev)
+    want = route(mask)
+    for K in (64, 2056):
+        (b1, b2), _ = weights([(72, K)] * 2, 1, dev)
+        lists = _mxfp4_linear_forward(spread(M, K, 1).to(dev), b1, b2, mask, keep=True)[1]
+        perm, counts = lists[:-8], lists[-8:]
+        assert torch.equal(counts[:5], want.counts[:5])
+        mv = int(counts[0])
+        assert torch.equal(perm[:mv], want.perm[:mv]) and torch.equal(perm[want.cap:want.cap + M - mv], want.perm[want.cap:want.cap + M - mv])
+
+
+def test_a_few_strided_tokens(dev):
+    K, N = 264, 136
+    wide = spread(40, 3 * K + 8, 1).to(dev)
+    (b1, b2), vs = weights([(N, K)] * 2, 2, dev)
+    mask = edge_mask(20, "alternating").to(dev)
+    for v in (wide[::2, 8:8 + K], wide[1::2, K + 8:2 * K + 8], wide[::2, 1:1 + K], wide[:20, :K].T.contiguous().T):
+        for n in (1, 3, 20):
+            inside(MXFP4MaskedLinear.apply(v[:n], b1, b2, mask[:n]), R.linear(v[:n].cpu(), *vs, mask[:n].cpu()))
+
+
+def test_a_second_backward_needs_retain_graph(dev):
+    M, d, h = 6, 64, 96
+    qs, _ = ffn_weights(d, h, 1, dev)
+    x = spread(M, d, 1).to(dev).requires_grad_(True)
+    y = MXFP4MaskedFFN.apply(x, *qs, edge_mask(M, "alternating").to(dev))
+    first = torch.autograd.grad(y.sum(), x, retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(y.sum(), x)[0], first)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), x)
 
 
 def test_no_tokens(dev):
