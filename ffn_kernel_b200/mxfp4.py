@@ -154,22 +154,34 @@ def _check_mask(mask, M, dev):
     return mask if mask.is_contiguous() else mask.contiguous()
 
 
-def _scratch(nbytes, M, dev, keep: bool):
-    """Workspace and routing lists (perm int32 [2 * cap], counts int32 [8]) of one call -> (tensors to hold, workspace,
-    perm, counts).  Inference takes one allocation for both; a backward pass wants the lists alone."""
+@lru_cache(maxsize=1024)
+def _kept_bytes(M: int, h: int) -> int:
+    return lib().ffnk_mxfp4_kept_bytes(M, h)
+
+
+def _scratch(nbytes, M, dev, keep: bool, factors: int = 0):
+    """Workspace, and the routing lists (perm int32 [2 * cap], counts int32 [8]) of one call -> (tensors to hold, workspace,
+    perm, counts).  Inference takes one allocation for both; what a backward pass wants, the lists behind ``factors``
+    bytes, gets one of its own."""
     cap = (M + 127) // 128 * 128
     if keep:
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        lists = torch.empty(2 * cap + 8, dtype=torch.int32, device=dev)
-        p = lists.data_ptr()
-        return ws, lists, ws.data_ptr(), p, p + 8 * cap
+        kept = torch.empty(factors + 8 * cap + 32, device=dev, dtype=torch.uint8)
+        p = kept.data_ptr() + factors
+        return ws, kept, ws.data_ptr(), p, p + 8 * cap
     ws = torch.empty(nbytes + 8 * cap + 32, device=dev, dtype=torch.uint8)
     p = ws.data_ptr()
     return ws, None, p, p + nbytes, p + nbytes + 8 * cap
 
 
+def _lists(kept, M):
+    """(perm, counts) at the end of what ``_scratch`` keeps."""
+    p = kept.data_ptr() + kept.numel() - 32
+    return p - 8 * ((M + 127) // 128 * 128), p
+
+
 def _mxfp4_linear_forward(a, b1, b2, mask, keep: bool = False):
-    """y[m] = Q(a[m]) @ (b1 if mask[m] else b2).T -> (y [M, N] bf16, routing lists if ``keep``)."""
+    """y[m] = Q(a[m]) @ (b1 if mask[m] else b2).T -> (y [M, N] bf16, with ``keep`` what the backward pass needs)."""
     a = _rows(a, "a")
     M, K = a.shape
     dev = a.device
@@ -185,31 +197,30 @@ def _mxfp4_linear_forward(a, b1, b2, mask, keep: bool = False):
     if M == 0:
         return y, None
     nbytes = _workspace_bytes(M, K, 0)
-    ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
+    ws, kept, wp, perm, counts = _scratch(nbytes, M, dev, keep)
     check("ffnk_mxfp4_linear_forward", lib().ffnk_mxfp4_linear_forward(
         a.data_ptr(), a.stride(0), *b1.ptrs, *b2.ptrs, mask.data_ptr(), perm, counts, wp, nbytes, y.data_ptr(), N, M, N, K,
         status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
-    return y, lists
+    return y, kept
 
 
-def _mxfp4_linear_backward(g, b1, b2, lists):
+def _mxfp4_linear_backward(g, b1, b2, kept):
     """dx[m] = g[m] @ (b1 if mask[m] else b2)."""
     g = _rows(g, "grad")
     M, (N, K) = g.shape[0], b1.shape
     dev = g.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
-            return _mxfp4_linear_backward(g, b1, b2, lists)
+            return _mxfp4_linear_backward(g, b1, b2, kept)
     dx = g.new_empty((M, K))
     if M == 0:
         return dx
     nbytes = _backward_bytes(M, K, N, 0)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    perm = lists.data_ptr()
     check("ffnk_mxfp4_linear_backward", lib().ffnk_mxfp4_linear_backward(
-        g.data_ptr(), g.stride(0), *b1.ptrs, *b2.ptrs, perm, perm + 4 * (lists.numel() - 8), ws.data_ptr(), nbytes, dx.data_ptr(),
-        K, M, N, K, status_word(dev).data_ptr(), stream_ptr(dev)))
+        g.data_ptr(), g.stride(0), *b1.ptrs, *b2.ptrs, *_lists(kept, M), ws.data_ptr(), nbytes, dx.data_ptr(), K, M, N, K,
+        status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return dx
 
@@ -218,7 +229,7 @@ _FFN_NAMES = ("w1", "w2", "w3", "u1", "u2", "u3")
 
 
 def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
-    """The whole FFN forward -> (y [M, d] bf16, what the backward pass needs or None)."""
+    """The whole FFN forward -> (y [M, d] bf16, with ``keep`` what the backward pass needs)."""
     x = _rows(x, "x")
     M, d = x.shape
     dev = x.device
@@ -233,39 +244,38 @@ def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
     L = lib()
     y = x.new_empty((M, d))
     if M == 0:
-        return y, (None, None, None)
+        return y, None
     nbytes = _workspace_bytes(M, d, h)
-    ws, lists, wp, perm, counts = _scratch(nbytes, M, dev, keep)
-    f1 = f3 = p1 = p3 = None
+    n = _kept_bytes(M, h) if keep else 0
+    ws, kept, wp, perm, counts = _scratch(nbytes, M, dev, keep, 2 * n)
+    f1 = f3 = None
     if keep:
-        n = L.ffnk_mxfp4_kept_bytes(M, h)
-        f1, f3 = torch.empty(n, device=dev, dtype=torch.uint8), torch.empty(n, device=dev, dtype=torch.uint8)
-        p1, p3 = f1.data_ptr(), f3.data_ptr()
+        f1 = kept.data_ptr()
+        f3 = f1 + n
     check("ffnk_mxfp4_ffn_forward", L.ffnk_mxfp4_ffn_forward(
         x.data_ptr(), x.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), mask.data_ptr(), perm,
-        counts, wp, nbytes, p1, p3, y.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
+        counts, wp, nbytes, f1, f3, y.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
-    return y, (lists, f1, f3)
+    return y, kept
 
 
-def _mxfp4_ffn_backward(gy, ws6, saved):
+def _mxfp4_ffn_backward(gy, ws6, kept):
     """Gradient of the activations."""
-    lists, f1, f3 = saved
     gy = _rows(gy, "grad")
     M, (h, d) = gy.shape[0], ws6[0].shape
     dev = gy.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
-            return _mxfp4_ffn_backward(gy, ws6, saved)
+            return _mxfp4_ffn_backward(gy, ws6, kept)
     dx = gy.new_empty((M, d))
     if M == 0:
         return dx
     nbytes = _backward_bytes(M, d, d, h)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    perm = lists.data_ptr()
+    f1 = kept.data_ptr()
     check("ffnk_mxfp4_ffn_backward", lib().ffnk_mxfp4_ffn_backward(
-        gy.data_ptr(), gy.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), f1.data_ptr(),
-        f3.data_ptr(), perm, perm + 4 * (lists.numel() - 8), ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h,
+        gy.data_ptr(), gy.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), f1,
+        f1 + _kept_bytes(M, h), *_lists(kept, M), ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h,
         status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return dx
@@ -287,8 +297,8 @@ class MXFP4MaskedLinear(Function):
 
     @staticmethod
     def forward(ctx, a, b1, b2, mask):
-        y, lists = _mxfp4_linear_forward(a, b1, b2, mask, keep=True)
-        ctx.save_for_backward(lists)
+        y, kept = _mxfp4_linear_forward(a, b1, b2, mask, keep=True)
+        ctx.save_for_backward(kept)
         ctx.weights = (b1, b2)
         return y
 
@@ -314,10 +324,10 @@ class MXFP4MaskedFFN(Function):
     def forward(ctx, a, w1, w2, w3, u1, u2, u3, mask):
         ctx.weights = (w1, w2, w3, u1, u2, u3)
         y, kept = _mxfp4_ffn_forward(a, ctx.weights, mask, keep=True)
-        ctx.save_for_backward(*kept)
+        ctx.save_for_backward(kept)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return (_mxfp4_ffn_backward(grad, ctx.weights, ctx.saved_tensors), *([None] * 7))
+        return (_mxfp4_ffn_backward(grad, ctx.weights, *ctx.saved_tensors), *([None] * 7))

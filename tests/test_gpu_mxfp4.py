@@ -110,7 +110,7 @@ def inside(got, want_and_bound):
 
 MASKS = ["all_visual", "all_text", "alternating", "bernoulli", "span"]
 LINEAR_SIZES = [(1, 64, 64), (3, 2056, 328), (1, 4096, 264), (2, 8, 8), (7, 40, 136), (33, 1000, 72), (127, 264, 520), (128, 256, 256),
-                (129, 128, 1032), (300, 2056, 328), (515, 96, 2048), (1030, 520, 264), (8200, 72, 64)]
+                (129, 128, 1032), (300, 2056, 328), (515, 96, 2048), (1030, 520, 264), (8200, 72, 64), (33000, 40, 72)]
 
 
 @pytest.mark.parametrize("M,K,N", LINEAR_SIZES)
@@ -247,7 +247,7 @@ def test_strided_activations_gradients_and_uint8_mask(dev):
     assert torch.equal(a, b) and torch.isfinite(c).all()
 
 
-@pytest.mark.parametrize("M", [1, 2, 5, 31, 32, 33, 64, 65, 127, 128, 129, 300, 9000])
+@pytest.mark.parametrize("M", [1, 2, 5, 31, 32, 33, 64, 65, 127, 128, 129, 300, 8193, 32768, 32769])
 @pytest.mark.parametrize("kind", MASKS)
 def test_routing_lists_are_those_of_route(dev, M, kind):
     # few tokens are routed inside the product's kernel (K <= 512: up to 32 of them), more by a kernel before it
@@ -257,7 +257,7 @@ def test_routing_lists_are_those_of_route(dev, M, kind):
     want = route(mask)
     for K in (64, 2056):
         (b1, b2), _ = weights([(72, K)] * 2, 1, dev)
-        lists = _mxfp4_linear_forward(spread(M, K, 1).to(dev), b1, b2, mask, keep=True)[1]
+        lists = _mxfp4_linear_forward(spread(M, K, 1).to(dev), b1, b2, mask, keep=True)[1].view(torch.int32)
         perm, counts = lists[:-8], lists[-8:]
         assert torch.equal(counts[:5], want.counts[:5])
         mv = int(counts[0])
