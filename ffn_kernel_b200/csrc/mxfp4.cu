@@ -21,10 +21,6 @@ template <> struct MxType<FFNK_BF16> { using t = __nv_bfloat16; };
 template <> struct MxType<FFNK_FP16> { using t = __half; };
 template <> struct MxType<FFNK_FP32> { using t = float; };
 
-__device__ __forceinline__ float mx_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float mx_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float mx_float(float v) { return v; }
-
 constexpr int kQuantThreads = 256;
 constexpr int kQuantPerSm = 4;        // resident CTAs the row kernels are compiled for
 constexpr int kChunksMax = 2;         // warp steps of a row in flight together (for few rows one, on more warps)
