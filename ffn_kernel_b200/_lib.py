@@ -70,12 +70,12 @@ SIGNATURES = {
     "ffnk_mxfp4_kept_bytes": (c_int64, [c_int64, c_int64]),
     "ffnk_mxfp4_linear_forward": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + [c_int64, c_void_p] + [c_int64] * 4
                                   + [c_void_p, c_void_p]),
-    "ffnk_mxfp4_ffn_forward": (c_int, [c_void_p, c_int64, POINTER(c_void_p), POINTER(c_void_p)] + [c_void_p] * 4
+    "ffnk_mxfp4_ffn_forward": (c_int, [c_void_p, c_int64, c_void_p, c_void_p] + [c_void_p] * 4
                                + [c_int64, c_void_p, c_void_p, c_void_p] + [c_int64] * 4 + [c_void_p, c_void_p]),
     "ffnk_mxfp4_backward_workspace_bytes": (c_int64, [c_int64] * 4),
     "ffnk_mxfp4_linear_backward": (c_int, [c_void_p, c_int64] + [c_void_p] * 7 + [c_int64, c_void_p] + [c_int64] * 4
                                    + [c_void_p, c_void_p]),
-    "ffnk_mxfp4_ffn_backward": (c_int, [c_void_p, c_int64, POINTER(c_void_p), POINTER(c_void_p)] + [c_void_p] * 5
+    "ffnk_mxfp4_ffn_backward": (c_int, [c_void_p, c_int64, c_void_p, c_void_p] + [c_void_p] * 5
                                 + [c_int64, c_void_p] + [c_int64] * 4 + [c_void_p, c_void_p]),
     "ffnk_read_status": (c_int, [c_void_p, c_int, c_void_p]),
     "ffnk_selftest_bounded_wait": (c_int, [c_void_p, c_int64, c_void_p]),

@@ -13,7 +13,7 @@ the identity); the weights are frozen.  A block that holds an infinity or a NaN 
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from functools import lru_cache
 
 import torch
@@ -27,7 +27,7 @@ from .route import _require_cuda, maybe_check, status_word, stream_ptr
 __all__ = ["MXFP4Tensor", "quantize_mxfp4", "dequantize_mxfp4", "MXFP4MaskedLinear", "MXFP4MaskedFFN"]
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_Six = ctypes.c_void_p * 6
+_six = struct.Struct("6P").pack        # a host array of six pointers
 
 
 @lru_cache(maxsize=1024)
@@ -111,8 +111,8 @@ def quantize_mxfp4(x: torch.Tensor, dim: int = 1) -> MXFP4Tensor:
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return quantize_mxfp4(x, 1 if dim in (1, -1) else 0)
-    codes = torch.empty((rows, -(-cols // 32) * 16), dtype=torch.uint8, device=dev)
-    scales = torch.empty((-(-rows // 128), -(-cols // 128), 32, 4, 4), dtype=torch.uint8, device=dev)
+    codes = torch.empty(rows, -(-cols // 32) * 16, dtype=torch.uint8, device=dev)
+    scales = torch.empty(-(-rows // 128), -(-cols // 128), 32, 4, 4, dtype=torch.uint8, device=dev)
     q = MXFP4Tensor.__new__(MXFP4Tensor)
     q.codes, q.scales, q.rows, q.cols, q.device, q.ptrs = codes, scales, rows, cols, dev, (codes.data_ptr(), scales.data_ptr())
     check("ffnk_mxfp4_quantize", lib().ffnk_mxfp4_quantize(
@@ -130,7 +130,7 @@ def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> tor
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return dequantize_mxfp4(q, dtype)
-    out = torch.empty((q.rows, q.cols), dtype=dtype, device=dev)
+    out = torch.empty(q.rows, q.cols, dtype=dtype, device=dev)
     check("ffnk_mxfp4_dequantize", lib().ffnk_mxfp4_dequantize(
         *q.ptrs, q.rows, q.cols, out.data_ptr(), _DTYPES[dtype], q.cols, stream_ptr(dev)))
     return out
@@ -193,7 +193,7 @@ def _mxfp4_linear_forward(a, b1, b2, mask, keep: bool = False):
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return _mxfp4_linear_forward(a, b1, b2, mask, keep)
-    y = a.new_empty((M, N))
+    y = a.new_empty(M, N)
     if M == 0:
         return y, None
     nbytes = _workspace_bytes(M, K, 0)
@@ -213,7 +213,7 @@ def _mxfp4_linear_backward(g, b1, b2, kept):
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return _mxfp4_linear_backward(g, b1, b2, kept)
-    dx = g.new_empty((M, K))
+    dx = g.new_empty(M, K)
     if M == 0:
         return dx
     nbytes = _backward_bytes(M, K, N, 0)
@@ -242,7 +242,7 @@ def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
         with torch.cuda.device(dev):
             return _mxfp4_ffn_forward(x, ws6, mask, keep)
     L = lib()
-    y = x.new_empty((M, d))
+    y = x.new_empty(M, d)
     if M == 0:
         return y, None
     nbytes = _workspace_bytes(M, d, h)
@@ -253,7 +253,7 @@ def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
         f1 = kept.data_ptr()
         f3 = f1 + n
     check("ffnk_mxfp4_ffn_forward", L.ffnk_mxfp4_ffn_forward(
-        x.data_ptr(), x.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), mask.data_ptr(), perm,
+        x.data_ptr(), x.stride(0), _six(*[w.ptrs[0] for w in ws6]), _six(*[w.ptrs[1] for w in ws6]), mask.data_ptr(), perm,
         counts, wp, nbytes, f1, f3, y.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return y, kept
@@ -267,14 +267,14 @@ def _mxfp4_ffn_backward(gy, ws6, kept):
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return _mxfp4_ffn_backward(gy, ws6, kept)
-    dx = gy.new_empty((M, d))
+    dx = gy.new_empty(M, d)
     if M == 0:
         return dx
     nbytes = _backward_bytes(M, d, d, h)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     f1 = kept.data_ptr()
     check("ffnk_mxfp4_ffn_backward", lib().ffnk_mxfp4_ffn_backward(
-        gy.data_ptr(), gy.stride(0), _Six(*[w.ptrs[0] for w in ws6]), _Six(*[w.ptrs[1] for w in ws6]), f1,
+        gy.data_ptr(), gy.stride(0), _six(*[w.ptrs[0] for w in ws6]), _six(*[w.ptrs[1] for w in ws6]), f1,
         f1 + _kept_bytes(M, h), *_lists(kept, M), ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h,
         status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
