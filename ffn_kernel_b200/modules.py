@@ -150,15 +150,17 @@ class GraphedMaskedFFN:
         self.mask = torch.zeros(tokens, device=w.device, dtype=torch.bool)
         views = module.weights() if four_bit else tuple(v.detach() for v in module.weight_views())
         forward = MXFP4MaskedFFN.apply if four_bit else _bf16_ffn_fused_forward
-        side = torch.cuda.Stream(device=w.device)
-        side.wait_stream(torch.cuda.current_stream(w.device))
-        with torch.cuda.stream(side), torch.no_grad():
-            for _ in range(max(1, warmup)):       # allocator warm-up outside the capture
-                forward(self.x, *views, self.mask)
-        torch.cuda.current_stream(w.device).wait_stream(side)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph), torch.no_grad():
-            self.y = forward(self.x, *views, self.mask)
+        self.weights = views                      # the graph reads their memory, whatever becomes of the module
+        with torch.cuda.device(w.device):
+            side = torch.cuda.Stream(device=w.device)
+            side.wait_stream(torch.cuda.current_stream(w.device))
+            with torch.cuda.stream(side), torch.no_grad():
+                for _ in range(max(1, warmup)):       # allocator warm-up outside the capture
+                    forward(self.x, *views, self.mask)
+            torch.cuda.current_stream(w.device).wait_stream(side)
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph), torch.no_grad():
+                self.y = forward(self.x, *views, self.mask)
 
     def __call__(self, x: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
         if x.numel() != self.x.numel() or mask.numel() != self.tokens:
