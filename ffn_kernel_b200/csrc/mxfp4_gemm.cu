@@ -501,8 +501,9 @@ __global__ void __launch_bounds__(MxGeom<EPI, CTAS>::threads, 1) mx_gemm_kernel(
         if (++stage == G::stages) { stage = 0; phase ^= 1; }
       }
     }
-    if (CTAS == 1 && *abort_flag && lead) {
-      // let the copies already issued land before the CTA gives its shared memory back
+    if (rank == 0 && *abort_flag && lead) {
+      // let the copies already issued land before the CTA gives its shared memory back (pairs: those of both, which the
+      // partner waits for at the end)
       for (int i = 0; i < (issued < G::stages ? issued : G::stages); ++i) {
         if (--stage < 0) { stage = G::stages - 1; phase ^= 1; }
         int dummy = 0;
