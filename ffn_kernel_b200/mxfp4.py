@@ -17,7 +17,7 @@ import struct
 from functools import lru_cache
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
@@ -55,6 +55,11 @@ def _rows(t, name):
     return t.clone() if t.data_ptr() & 15 else t
 
 
+def _ld(t) -> int:
+    """Elements from one row to the next; the stride of a single row may be anything."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 class MXFP4Tensor:
     """A matrix [rows, cols] in MXFP4, blocks of 32 along the columns (the contraction: a weight is [out, in]).
 
@@ -62,16 +67,15 @@ class MXFP4Tensor:
     scales  uint8 [ceil(rows / 128), ceil(cols / 128), 32, 4, 4]; 2^(byte - 127) of (row r, block b) sits at
             [r // 128, b // 4, r % 32, r % 128 // 32, b % 4]; entries without a row or block are 0
     """
-    __slots__ = ("codes", "scales", "rows", "cols", "device", "ptrs")
+    __slots__ = ("_codes", "_scales", "_rows", "_cols", "_device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
         try:
-            ptrs = (codes.data_ptr(), scales.data_ptr())
             device = codes.device
             ok = (codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_cuda and scales.device == device
                   and codes.shape == (rows, (cols + 31) // 32 * 16)
                   and scales.shape == ((rows + 127) // 128, (cols + 127) // 128, 32, 4, 4)
-                  and codes.is_contiguous() and scales.is_contiguous() and not (ptrs[0] | ptrs[1]) & 15)
+                  and codes.is_contiguous() and scales.is_contiguous() and not (codes.data_ptr() | scales.data_ptr()) & 15)
         except AttributeError:
             ok = False
         if not ok:
@@ -80,11 +84,21 @@ class MXFP4Tensor:
                 f"[{-(-rows // 128)}, {-(-cols // 128)}, 32, 4, 4], both contiguous, 16-byte aligned and on one CUDA device; got "
                 + " and ".join(f"{t.dtype} {list(t.shape)} strides {list(t.stride())} on {t.device}" if isinstance(t, torch.Tensor)
                                else type(t).__name__ for t in (codes, scales)))
-        self.codes, self.scales, self.rows, self.cols, self.device, self.ptrs = codes, scales, rows, cols, device, ptrs
+        self._codes, self._scales, self._rows, self._cols, self._device = codes, scales, rows, cols, device
 
-    @property
-    def shape(self):
-        return (self.rows, self.cols)
+    # the fields have been checked against one another: they can be read, not replaced
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    rows = property(lambda self: self._rows)
+    cols = property(lambda self: self._cols)
+    device = property(lambda self: self._device)
+    shape = property(lambda self: (self._rows, self._cols))
+
+    def _ptrs(self):
+        return self._codes.data_ptr(), self._scales.data_ptr()
+
+    def __reduce__(self):
+        return MXFP4Tensor, (self._codes, self._scales, self._rows, self._cols)
 
     def __repr__(self):
         return f"MXFP4Tensor([{self.rows}, {self.cols}], device={self.codes.device})"
@@ -92,7 +106,7 @@ class MXFP4Tensor:
 
 def quantize_mxfp4(x: torch.Tensor, dim: int = 1) -> MXFP4Tensor:
     """``x`` (2-D; bf16, fp16 or fp32) with blocks along ``dim``.  The result's columns are ``x``'s dimension
-    ``dim``: an ``nn.Linear`` weight [out, in] is quantised along 1, its ``.T`` view or an [in, out] weight along 0."""
+    ``dim`` and it carries no gradient: an ``nn.Linear`` weight [out, in] is quantised along 1, its ``.T`` view or an [in, out] weight along 0."""
     _require_cuda(x, "x")
     if x.dim() != 2:
         raise RuntimeError(f"x must be 2-D, got shape {tuple(x.shape)}")
@@ -114,9 +128,9 @@ def quantize_mxfp4(x: torch.Tensor, dim: int = 1) -> MXFP4Tensor:
     codes = torch.empty(rows, -(-cols // 32) * 16, dtype=torch.uint8, device=dev)
     scales = torch.empty(-(-rows // 128), -(-cols // 128), 32, 4, 4, dtype=torch.uint8, device=dev)
     q = MXFP4Tensor.__new__(MXFP4Tensor)
-    q.codes, q.scales, q.rows, q.cols, q.device, q.ptrs = codes, scales, rows, cols, dev, (codes.data_ptr(), scales.data_ptr())
+    q._codes, q._scales, q._rows, q._cols, q._device = codes, scales, rows, cols, dev
     check("ffnk_mxfp4_quantize", lib().ffnk_mxfp4_quantize(
-        x.data_ptr(), _DTYPES[x.dtype], rs, cs, rows, cols, *q.ptrs, stream_ptr(dev)))
+        x.data_ptr(), _DTYPES[x.dtype], rs, cs, rows, cols, *q._ptrs(), stream_ptr(dev)))
     return q
 
 
@@ -132,7 +146,7 @@ def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> tor
             return dequantize_mxfp4(q, dtype)
     out = torch.empty(q.rows, q.cols, dtype=dtype, device=dev)
     check("ffnk_mxfp4_dequantize", lib().ffnk_mxfp4_dequantize(
-        *q.ptrs, q.rows, q.cols, out.data_ptr(), _DTYPES[dtype], q.cols, stream_ptr(dev)))
+        *q._ptrs(), q.rows, q.cols, out.data_ptr(), _DTYPES[dtype], q.cols, stream_ptr(dev)))
     return out
 
 
@@ -140,9 +154,9 @@ def _check_weights(ws, names, shapes, dev):
     for w, n, s in zip(ws, names, shapes):
         if not isinstance(w, MXFP4Tensor):
             raise RuntimeError(f"{n} must be an MXFP4Tensor, got {type(w).__name__}")
-        if w.rows != s[0] or w.cols != s[1]:
+        if w._rows != s[0] or w._cols != s[1]:
             raise RuntimeError(f"{n} must have shape {list(s)} ([out, in]), got [{w.rows}, {w.cols}]")
-        if w.device != dev:
+        if w._device != dev:
             raise RuntimeError(f"{n} must be on the same device as the activations")
 
 
@@ -199,7 +213,7 @@ def _mxfp4_linear_forward(a, b1, b2, mask, keep: bool = False):
     nbytes = _workspace_bytes(M, K, 0)
     ws, kept, wp, perm, counts = _scratch(nbytes, M, dev, keep)
     check("ffnk_mxfp4_linear_forward", lib().ffnk_mxfp4_linear_forward(
-        a.data_ptr(), a.stride(0), *b1.ptrs, *b2.ptrs, mask.data_ptr(), perm, counts, wp, nbytes, y.data_ptr(), N, M, N, K,
+        a.data_ptr(), _ld(a), *b1._ptrs(), *b2._ptrs(), mask.data_ptr(), perm, counts, wp, nbytes, y.data_ptr(), N, M, N, K,
         status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return y, kept
@@ -219,7 +233,7 @@ def _mxfp4_linear_backward(g, b1, b2, kept):
     nbytes = _backward_bytes(M, K, N, 0)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     check("ffnk_mxfp4_linear_backward", lib().ffnk_mxfp4_linear_backward(
-        g.data_ptr(), g.stride(0), *b1.ptrs, *b2.ptrs, *_lists(kept, M), ws.data_ptr(), nbytes, dx.data_ptr(), K, M, N, K,
+        g.data_ptr(), _ld(g), *b1._ptrs(), *b2._ptrs(), *_lists(kept, M), ws.data_ptr(), nbytes, dx.data_ptr(), K, M, N, K,
         status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return dx
@@ -253,7 +267,7 @@ def _mxfp4_ffn_forward(x, ws6, mask, keep: bool):
         f1 = kept.data_ptr()
         f3 = f1 + n
     check("ffnk_mxfp4_ffn_forward", L.ffnk_mxfp4_ffn_forward(
-        x.data_ptr(), x.stride(0), _six(*[w.ptrs[0] for w in ws6]), _six(*[w.ptrs[1] for w in ws6]), mask.data_ptr(), perm,
+        x.data_ptr(), _ld(x), _six(*[w._codes.data_ptr() for w in ws6]), _six(*[w._scales.data_ptr() for w in ws6]), mask.data_ptr(), perm,
         counts, wp, nbytes, f1, f3, y.data_ptr(), d, M, d, h, status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
     return y, kept
@@ -274,7 +288,7 @@ def _mxfp4_ffn_backward(gy, ws6, kept):
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     f1 = kept.data_ptr()
     check("ffnk_mxfp4_ffn_backward", lib().ffnk_mxfp4_ffn_backward(
-        gy.data_ptr(), gy.stride(0), _six(*[w.ptrs[0] for w in ws6]), _six(*[w.ptrs[1] for w in ws6]), f1,
+        gy.data_ptr(), _ld(gy), _six(*[w._codes.data_ptr() for w in ws6]), _six(*[w._scales.data_ptr() for w in ws6]), f1,
         f1 + _kept_bytes(M, h), *_lists(kept, M), ws.data_ptr(), nbytes, dx.data_ptr(), d, M, d, h,
         status_word(dev).data_ptr(), stream_ptr(dev)))
     maybe_check(dev)
@@ -282,7 +296,14 @@ def _mxfp4_ffn_backward(gy, ws6, kept):
 
 
 def _wants_grad(a) -> bool:
-    return isinstance(a, torch.Tensor) and a.requires_grad and torch.is_grad_enabled()
+    """Does this call go through autograd?  (Under forward-mode differentiation too, for its refusal.)"""
+    return isinstance(a, torch.Tensor) and (a.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0)
+
+
+def _storage(ws):
+    """The weights' tensors, saved so that a change between the forward and the backward pass is noticed (one made in
+    inference mode has no version to compare and cannot be saved)."""
+    return [t for w in ws for t in (w._codes, w._scales) if not t.is_inference()]
 
 
 class MXFP4MaskedLinear(Function):
@@ -298,14 +319,14 @@ class MXFP4MaskedLinear(Function):
     @staticmethod
     def forward(ctx, a, b1, b2, mask):
         y, kept = _mxfp4_linear_forward(a, b1, b2, mask, keep=True)
-        ctx.save_for_backward(kept)
+        ctx.save_for_backward(kept, *_storage((b1, b2)))
         ctx.weights = (b1, b2)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return _mxfp4_linear_backward(grad, *ctx.weights, *ctx.saved_tensors), None, None, None
+        return _mxfp4_linear_backward(grad, *ctx.weights, ctx.saved_tensors[0]), None, None, None
 
 
 class MXFP4MaskedFFN(Function):
@@ -324,10 +345,10 @@ class MXFP4MaskedFFN(Function):
     def forward(ctx, a, w1, w2, w3, u1, u2, u3, mask):
         ctx.weights = (w1, w2, w3, u1, u2, u3)
         y, kept = _mxfp4_ffn_forward(a, ctx.weights, mask, keep=True)
-        ctx.save_for_backward(kept)
+        ctx.save_for_backward(kept, *_storage(ctx.weights))
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        return (_mxfp4_ffn_backward(grad, ctx.weights, *ctx.saved_tensors), *([None] * 7))
+        return (_mxfp4_ffn_backward(grad, ctx.weights, ctx.saved_tensors[0]), *([None] * 7))

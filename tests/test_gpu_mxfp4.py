@@ -2,6 +2,9 @@
 
 Quantisation is compared bit for bit.  Products are compared element by element with bounds that the oracle derives
 from the roundings on the way (``oracle/mxfp4_ref.py``)."""
+import copy
+import io
+
 import pytest
 import torch
 
@@ -396,3 +399,129 @@ def test_repeated_calls_give_the_same_bits(dev):
     y = MXFP4MaskedFFN.apply(x, *qs, mask)
     for _ in range(5):
         assert torch.equal(MXFP4MaskedFFN.apply(x, *qs, mask), y)
+
+
+def test_a_single_row_of_any_stride(dev):
+    # PyTorch calls a one-row view contiguous whatever its stride
+    K, N = 72, 136
+    wide = spread(4, 77, 1).to(dev)
+    (b1, b2), _ = weights([(N, K)] * 2, 2, dev)
+    qs, _ = ffn_weights(K, N, 3, dev)
+    mask = torch.ones(1, dtype=torch.bool, device=dev)
+    for v in (wide[0:1, :K], wide[1:2, :K], wide[:, 1:].as_strided((1, K), (1, 1)), wide[2:3, 5:]):
+        plain = v.reshape(-1).clone().view(1, K)
+        assert torch.equal(MXFP4MaskedLinear.apply(v, b1, b2, mask), MXFP4MaskedLinear.apply(plain, b1, b2, mask))
+        a, b = v.detach().requires_grad_(True), plain.requires_grad_(True)
+        ya, yb = MXFP4MaskedFFN.apply(a, *qs, mask), MXFP4MaskedFFN.apply(b, *qs, mask)
+        assert torch.equal(ya, yb)
+        assert torch.equal(torch.autograd.grad(ya, a, v)[0], torch.autograd.grad(yb, b, plain)[0])
+    for v in (wide[0:1, ::3], wide[1:2, 1::2], wide[:, 3:4]):
+        same_matrix(quantize_mxfp4(v), v)
+        same_matrix(quantize_mxfp4(v, dim=0), v.T)
+
+
+def test_a_copied_or_loaded_matrix_has_its_own_memory(dev):
+    q = quantize_mxfp4(spread(70, 200, 1).to(dev))
+    want = dequantize_mxfp4(q)
+    stored = io.BytesIO()
+    torch.save(q, stored)
+    stored.seek(0)
+    twins = [copy.deepcopy(q), torch.load(stored, weights_only=False), copy.copy(q)]
+    assert twins[0].codes.data_ptr() != q.codes.data_ptr() != twins[1].codes.data_ptr()
+    del q
+    poison(dev)
+    for t in twins:
+        assert torch.equal(dequantize_mxfp4(t), want) and t.shape == (70, 200)
+        for name in ("codes", "scales", "rows", "cols", "shape", "device"):
+            with pytest.raises(AttributeError):
+                setattr(t, name, getattr(t, name))
+
+
+def test_weights_changed_before_the_backward_pass_are_noticed(dev):
+    K, N = 64, 96
+    mask = edge_mask(6, "alternating").to(dev)
+    x = spread(6, K, 1).to(dev).requires_grad_(True)
+    for run, ws in ((MXFP4MaskedLinear, [(N, K)] * 2), (MXFP4MaskedFFN, [(N, K), (K, N), (N, K)] * 2)):
+        qs, _ = weights(ws, 1, dev)
+        y = run.apply(x, *qs, mask)
+        qs[-1].scales.add_(1)
+        with pytest.raises(RuntimeError):
+            y.sum().backward()
+        with torch.inference_mode():
+            frozen = [quantize_mxfp4(spread(r, c, 1).to(dev)) for r, c in ws]
+        assert torch.isfinite(torch.autograd.grad(run.apply(x, *frozen, mask).sum(), x)[0]).all()
+        with torch.autograd.forward_ad.dual_level():              # no forward-mode derivative: refused, not dropped
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                run.apply(torch.autograd.forward_ad.make_dual(x.detach(), x.detach()), *qs, mask)
+
+
+def test_a_graph_outlives_the_module_it_was_captured_from(dev):
+    d, h, T = 136, 264, 9
+    torch.manual_seed(1)
+    ffn = MaskedFFNModule(d, h, device=dev)
+    x, mask = spread(T, d, 1).to(dev), edge_mask(T, "span").to(dev)
+    with torch.no_grad():                     # a graph holds the inference forward
+        want4, want = MXFP4MaskedFFNModule.from_module(ffn)(x, mask), ffn(x, mask)
+    g4, g = GraphedMaskedFFN(MXFP4MaskedFFNModule.from_module(ffn), T), GraphedMaskedFFN(ffn, T)
+    del ffn
+    poison(dev)
+    assert torch.equal(g4(x, mask), want4) and torch.equal(g(x, mask), want)
+
+
+def test_nothing_of_the_workspace_reaches_the_results(dev):
+    # every byte 255: scales that stand for NaN, in rows and blocks that exist only as padding
+    def stain():
+        junk = [torch.full((n,), 255, dtype=torch.uint8, device=dev) for n in (1 << 12, 1 << 16, 1 << 20, 1 << 24, 1 << 26)]
+        del junk
+
+    for M, d, h in ((1, 40, 72), (5, 200, 136), (130, 328, 1000), (700, 136, 264), (8200, 72, 136), (33000, 40, 72)):
+        x, mask, g = spread(M, d, 1).to(dev), edge_mask(M, "span", 2).to(dev), spread(M, d, 3).to(dev)
+        qs, _ = ffn_weights(d, h, 4, dev)
+        x.requires_grad_(True)
+        runs = []
+        for _ in range(2):
+            stain()
+            z = MXFP4MaskedLinear.apply(x, qs[0], qs[3], mask)
+            stain()
+            y = MXFP4MaskedFFN.apply(x, *qs, mask)
+            stain()
+            dz = torch.autograd.grad(z, x, z.detach())[0]
+            stain()
+            runs.append((z.detach(), y.detach(), dz, torch.autograd.grad(y, x, g)[0]))
+        for a, b in zip(*runs):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits(dev):
+    K = 32768
+    x = torch.randn(140000, K, device=dev, dtype=torch.bfloat16)          # 4.6e9 values, 2.3e9 bytes of codes
+    q = quantize_mxfp4(x)
+    back = dequantize_mxfp4(q)
+    for s in (slice(65500, 65700), slice(131000, 131200), slice(139900, 140000)):
+        part = quantize_mxfp4(x[s].clone())
+        assert torch.equal(q.codes[s], part.codes) and torch.equal(back[s], dequantize_mxfp4(part))
+    del back
+    q = quantize_mxfp4(x, dim=0)
+    part = quantize_mxfp4(x[:, -128:].contiguous(), dim=0)
+    assert torch.equal(q.codes[-128:], part.codes) and torch.equal(q.scales[-1], part.scales[0])
+    del x, q, part
+    torch.cuda.empty_cache()
+
+    def tail(M, d, ws, run, forward, backward):
+        qs, vs = weights(ws, 1, dev)
+        x = torch.randn(M, d, device=dev, dtype=torch.bfloat16, requires_grad=True)
+        mask = edge_mask(M, "bernoulli", 1)
+        y = run.apply(x, *qs, mask.to(dev))
+        g = torch.randn_like(y)
+        dx = torch.autograd.grad(y, x, g)[0]
+        check_status()
+        for s in (slice(0, 40), slice(M // 2, M // 2 + 40), slice(M - 60, M)):
+            xs, gs, ms = x[s].detach().cpu(), g[s].cpu(), mask[s]
+            inside(y[s].detach(), forward(xs, vs, ms))
+            inside(dx[s], backward(gs, xs, vs, ms))
+
+    tail(1_100_000, 4096, [(4104, 4096)] * 2, MXFP4MaskedLinear, lambda x, vs, m: R.linear(x, *vs, m),
+         lambda g, x, vs, m: R.linear_dx(g, *vs, m))
+    torch.cuda.empty_cache()
+    tail(540_000, 64, [(8200, 64), (64, 8200), (8200, 64)] * 2, MXFP4MaskedFFN, R.ffn, R.ffn_dx)
+    torch.cuda.empty_cache()
