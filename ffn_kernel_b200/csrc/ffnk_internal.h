@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/ffnk.h"
 
 namespace ffnk {
@@ -33,6 +35,19 @@ int make_tensor_map_2d(CUtensorMap* out, const void* base, uint64_t inner, uint6
 // The same for any element type and swizzle: extents and boxes in elements, row stride in bytes (a multiple of 16).
 int make_tensor_map_2d_of(CUtensorMap* out, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
                           uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);
+
+// Runs `set` (-> cudaError_t), a kernel attribute that the driver keeps, once per device; `done` holds a bit a device.
+template <class F>
+int once_per_device(std::atomic<uint64_t>& done, F&& set) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return 0;
+  e = set();
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return cuda_status(e);
+}
 
 // SMs a persistent grid may occupy (all but the margin of ffnk_set_sm_margin, at least two).
 int usable_sms();

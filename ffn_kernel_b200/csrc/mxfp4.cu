@@ -128,24 +128,27 @@ __global__ void __launch_bounds__(kQuantThreads, kQuantPerSm) mx_quantize_rows_k
 // whole mask in every CTA, as for the copy of bf16 rows, was bound by its shared-memory stores: 8192 x 4096 34 us, now
 // 20, from cold caches.  A routing kernel and then mx_quantize_rows_kernel take as long from 16384 tokens on, 35 us and
 // 68 us at 32768, in three launches.)
-constexpr int kMxRouteWords = 4;             // words of 32 tokens a thread, consecutive
+// WORDS: words of 32 tokens a thread, consecutive.
+constexpr int kMxRouteWords = 4;
 constexpr int kMxRouteTokens = kRouteThreads * 32 * kMxRouteWords;
+constexpr int kMxBesideTokens = 1024;        // few tokens: the product starts beside this kernel (mx_route_quantize)
+template <int WORDS>
 __global__ void __launch_bounds__(kRouteThreads, kQuantPerSm) mx_route_quantize_kernel(
     const uint8_t* __restrict__ mask, int M, int cap, int* __restrict__ perm, int* __restrict__ counts,
     const __nv_bfloat16* __restrict__ x, int64_t ldx, int cols, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
     int align, int per_warp) {
-  __shared__ uint32_t s_bits[kRouteThreads * kMxRouteWords];   // token 32 i + k is visual: bit k of word i
-  __shared__ int s_before[kRouteThreads * kMxRouteWords];      // visual tokens before word i
+  __shared__ uint32_t s_bits[kRouteThreads * WORDS];   // token 32 i + k is visual: bit k of word i
+  __shared__ int s_before[kRouteThreads * WORDS];      // visual tokens before word i
   __shared__ int s_warp[kRouteThreads / 32];
   __shared__ int s_runs;
   const int tid = threadIdx.x, lane = tid & 31;
   const bool writer = blockIdx.x == 0 && blockIdx.y == 0;
   griddep_launch_dependents();
   const int words = (M + kRouteThreads * 32 - 1) / (kRouteThreads * 32);
-  uint32_t bits[kMxRouteWords] = {};
+  uint32_t bits[WORDS] = {};
   int count = 0, runs = 0;
 #pragma unroll
-  for (int w = 0; w < kMxRouteWords; ++w) {
+  for (int w = 0; w < WORDS; ++w) {
     if (w < words) {
       const ThreadTokens tt = load_thread_tokens(mask, M, (tid * words + w) * 32);
       bits[w] = tt.bits;
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(kRouteThreads, kQuantPerSm) mx_route_quantize_
   int Mv = 0;
   int before = block_exclusive_scan(count, s_warp, &Mv);
 #pragma unroll
-  for (int w = 0; w < kMxRouteWords; ++w) {
+  for (int w = 0; w < WORDS; ++w) {
     if (w < words) {
       s_bits[tid * words + w] = bits[w];
       s_before[tid * words + w] = before;
@@ -405,6 +408,10 @@ static int quantize_typed(const void* x_, int64_t row_stride, int64_t col_stride
   return cuda_status(cudaGetLastError());
 }
 
+// Few tokens: 2 KiB of shared memory, and the SM's memory divided as the products want it, so that their CTAs get their places while this
+// kernel runs (an SM does not change the division while it is busy, and a cluster whose place is taken at first may wait
+// until all others are done): linear 11008 -> 4096, 8 tokens of both modalities 20.0 -> 14.4 us, 4096 x 4096, 127
+// tokens 13.0 -> 11.9.  Many tokens: CTAs that wait beside it only slow it down (4096 x 4096, 4000 tokens 38.3 -> 40.4).
 int mx_route_quantize(const void* mask, int64_t M, const void* x, int64_t ldx, int64_t d, int32_t* perm, int32_t* counts,
                       void* scan, void* codes, void* scales, int32_t* status, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -413,9 +420,19 @@ int mx_route_quantize(const void* mask, int64_t M, const void* x, int64_t ldx, i
   uint8_t* sc = static_cast<uint8_t*>(scales);
   if (M <= kMxRouteTokens) {
     const QuantShape q = quant_shape(M, d, MxLane<__nv_bfloat16>::chunk, kChunksMax, kQuantPerSm);
-    mx_route_quantize_kernel<<<q.grid, kRouteThreads, 0, s>>>(static_cast<const uint8_t*>(mask), static_cast<int>(M),
-                                                              static_cast<int>(ffnk_route_capacity(M)), perm, counts, xb, ldx,
-                                                              static_cast<int>(d), c, sc, row_alignment(x, 2 * ldx), q.per_warp);
+    const bool beside = M <= kMxBesideTokens;
+    if (beside) {
+      static std::atomic<uint64_t> prepared{0};
+      const int r = once_per_device(prepared, [] {
+        return cudaFuncSetAttribute(mx_route_quantize_kernel<1>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                    cudaSharedmemCarveoutMaxShared);
+      });
+      if (r) return r;
+    }
+    const auto kernel = beside ? mx_route_quantize_kernel<1> : mx_route_quantize_kernel<kMxRouteWords>;
+    kernel<<<q.grid, kRouteThreads, 0, s>>>(static_cast<const uint8_t*>(mask), static_cast<int>(M),
+                                            static_cast<int>(ffnk_route_capacity(M)), perm, counts, xb, ldx, static_cast<int>(d), c,
+                                            sc, row_alignment(x, 2 * ldx), q.per_warp);
     return cuda_status(cudaGetLastError());
   }
   const int r = ffnk_route(mask, M, perm, counts, scan, status, stream);

@@ -10,8 +10,6 @@
 // Epilogues: bf16 rows scattered to token order; or silu(gate) * up, which leaves as MXFP4 again: the 32
 // accumulator columns a lane reads at a time are one block of its row, so the maximum, the scale and the codes
 // need no other lane.
-#include <atomic>
-
 #include "ffnk_internal.h"
 #include "mxfp4.cuh"
 #include "ptx.cuh"
@@ -1104,17 +1102,10 @@ static bool mx_pairs(int64_t M, int64_t k) {
   return forced >= 0 ? forced != 0 : M >= 8192 || (k >= 2048 && M > 1024);
 }
 
-// Dynamic shared memory of a kernel, allowed once per device (the driver keeps the attribute).
+// Dynamic shared memory of a kernel
 template <class K>
 static int mx_allow_smem(K kernel, int bytes, std::atomic<uint64_t>& allowed) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_status(e);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev < 64 && (allowed.load(std::memory_order_relaxed) & bit)) return 0;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) allowed.fetch_or(bit, std::memory_order_relaxed);
-  return cuda_status(e);
+  return once_per_device(allowed, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
 }
 
 template <int EPI, int CTAS>
@@ -1181,12 +1172,14 @@ struct MxSelf {
   int32_t* perm;
   int32_t* counts;
 };
-// Does it?  Few enough (row, two k-steps) units a CTA that rounding them takes less than the weights do to arrive (at most
-// eight a warp), and room for all of A beside three stages of B.
+// Does it?  At most 16 (row, two k-steps) units a CTA, whose loads its four warps have in flight at once; and room for all of
+// A beside three stages of B.  Measured (itself / a kernel before it, whole call by graph replay, us): linear 2048 x 2048, 8 tokens
+// 6.2 / 7.0, 16 tokens (16 units) 7.0 / 7.0, 24 tokens 7.9 / 7.0; 4096 x 4096, 4 tokens 7.5 / 7.4, 16 tokens (32 units)
+// 9.1 / 7.5; FFN 4096/11008, 2 tokens (16 units) 23.6 / 22.7, 4 tokens (32) 25.4 / 22.6; the launch saved is 2 us of the host's time.
 static bool mx_takes_self(int64_t M, int64_t k, int splits) {
   if (splits == 0 || M > MX_BM || tune_overrides().permute == 0) return false;
   const int64_t steps = ((mx_code_ld(k) + 127) / 128 + splits - 1) / splits;
-  return M * ((steps + 1) / 2) <= 32 && steps * (((M + 7) / 8) * 1024 + MX_SF_BYTES) + 3 * (MXS_B_BYTES + MX_SF_BYTES) <= MXS_SMEM_STAGES;
+  return M * ((steps + 1) / 2) <= 16 && steps * (((M + 7) / 8) * 1024 + MX_SF_BYTES) + 3 * (MXS_B_BYTES + MX_SF_BYTES) <= MXS_SMEM_STAGES;
 }
 
 template <bool GLU, bool SELF>

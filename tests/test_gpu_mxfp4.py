@@ -253,7 +253,7 @@ def test_strided_activations_gradients_and_uint8_mask(dev):
 @pytest.mark.parametrize("M", [1, 2, 5, 31, 32, 33, 64, 65, 127, 128, 129, 300, 8193, 32768, 32769])
 @pytest.mark.parametrize("kind", MASKS)
 def test_routing_lists_are_those_of_route(dev, M, kind):
-    # few tokens are routed inside the product's kernel (K <= 512: up to 32 of them), more by a kernel before it
+    # few tokens are routed inside the product's kernel (K <= 512: up to 16 of them), more by a kernel before it
     from ffn_kernel_b200 import route
     from ffn_kernel_b200.mxfp4 import _mxfp4_linear_forward
     mask = edge_mask(M, kind, seed=M + 1).to(dev)
