@@ -1144,10 +1144,14 @@ static int mx_launch(const MxMaps& maps, const MxParams& p, int64_t M, bool pair
   return pairs ? mx_launch_as<EPI, 2>(maps, p, M, stream) : mx_launch_as<EPI, 1>(maps, p, M, stream);
 }
 
-// Ranges of the contraction for the small kernel, 0: not the small kernel, which takes calls of one row tile a modality.
-// Measured (whole call by graph replay, small / 128 x 256 tiles, us): FFN 1024/2816 127 tokens 16.4 / 18.5, 200 tokens
-// 19.3 / 18.9, 512 tokens 24.5 / 19.7; FFN 4096/11008 1 token 23.4 / 38.3, 127 tokens 49.6 / 51.1, 200 tokens 57.4 / 52.2;
-// linear 4096 x 4096 1 token 7.4 / 12.3, 127 tokens 13.7 / 15.5, 256 tokens 17.6 / 16.9.
+// Ranges of the contraction for the small kernel, 0: not the small kernel, which takes calls of one row tile a modality, and
+// more of them where 128 x 256 tiles would leave most SMs idle for a long contraction: that can be cut into four ranges, or into
+// two that are still long, while the rows do not outgrow the contraction.
+// Measured (whole call by graph replay, small / 128 x 256 tiles, us): FFN 1024/2816 127 tokens 16.0 / 16.4, 200 tokens
+// 19.4 / 16.9; FFN 4096/11008 1 token 22.6 / 36.0, 127 tokens 49.6 / 48.0, 200 tokens 56.8 / 49.4; linear 4096 x 4096 1 token
+// 6.6 / 11.0, 127 tokens 12.1 / 14.4, 200 tokens 14.8 / 14.8 (two ranges), 512 tokens 23.1 / 17.3 (one); 4096 -> 1024, 512 tokens (four)
+// 13.2 / 14.8; 11008 -> 4096, 300 tokens (two) 24.7 / 27.6; 16384 -> 1024, 1024 tokens (four) 27.4 / 38.4, 2048 tokens
+// (two) 40.3 / 40.8.
 // The number of ranges: as many as fill the places on the GPU once (two CTAs an SM), at most four, which always beat
 // eight (linear 4096 x 4096, 64 tokens: 1 / 2 / 4 / 8 ranges 13.3 / 11.0 / 10.7 / 18.6 us).  Gate/up tiles add up two
 // matrices and come out in 4 bits, a longer tail, so they take two ranges only where those CTAs nearly fit one an SM
@@ -1155,13 +1159,14 @@ static int mx_launch(const MxMaps& maps, const MxParams& p, int64_t M, bool pair
 constexpr int kMxSmallTokens = 128;
 static int mx_small_splits(int64_t M, int64_t n_out, int64_t k, bool glu) {
   const int forced = tune_overrides().narrow;
-  if (forced == 0 || (M > kMxSmallTokens && forced < 0)) return 0;
+  const int64_t steps = (mx_code_ld(k) + 127) / 128;
+  if (forced == 0 || (forced < 0 && M > kMxSmallTokens && (glu || M > 32 * steps))) return 0;
   const int64_t m_tiles = (M + MX_BM - 1) / MX_BM + (M > 1 ? 1 : 0);
   const int64_t tiles = m_tiles * ((n_out + MXS_N - 1) / MXS_N) * (glu ? 2 : 1);
   const int64_t most = glu ? usable_sms() * 5 / 4 : 2 * usable_sms();
-  const int64_t steps = (mx_code_ld(k) + 127) / 128;
   int splits = 1;
   while (splits < (glu ? 2 : 4) && tiles * splits * 2 <= most && steps >= splits * 2) splits *= 2;
+  if (forced < 0 && M > kMxSmallTokens && (splits == 1 || splits * steps < 64)) return 0;
   return splits;
 }
 

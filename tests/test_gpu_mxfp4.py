@@ -134,6 +134,16 @@ def test_linear_forward_and_gradient(dev, M, K, N, kind):
     inside(xg.grad, R.linear_dx(g, v1, v2, mask))
 
 
+@pytest.mark.parametrize("M,K,N", [(300, 4104, 264), (513, 4104, 136), (1000, 8200, 72), (200, 11008, 1032)])
+@pytest.mark.parametrize("kind", MASKS)
+def test_linear_of_several_row_tiles_and_a_long_contraction(dev, M, K, N, kind):
+    x, mask = spread(M, K, M + K), edge_mask(M, kind, seed=M)
+    (b1, b2), (v1, v2) = weights([(N, K)] * 2, K, dev)
+    poison(dev)
+    inside(MXFP4MaskedLinear.apply(x.to(dev), b1, b2, mask.to(dev)), R.linear(x, v1, v2, mask))
+    check_status()
+
+
 FFN_SIZES = [(1, 64, 64), (1, 1024, 1416), (2, 8, 8), (7, 40, 136), (33, 1000, 72), (127, 264, 520), (128, 256, 256),
              (130, 128, 1032), (300, 512, 328), (515, 96, 1000), (1030, 264, 136), (8200, 64, 72)]
 
