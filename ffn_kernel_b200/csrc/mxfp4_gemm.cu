@@ -1144,30 +1144,33 @@ static int mx_launch(const MxMaps& maps, const MxParams& p, int64_t M, bool pair
   return pairs ? mx_launch_as<EPI, 2>(maps, p, M, stream) : mx_launch_as<EPI, 1>(maps, p, M, stream);
 }
 
-// Ranges of the contraction for the small kernel, 0: not the small kernel, which takes calls of one row tile a modality, and
-// more of them where 128 x 256 tiles would leave most SMs idle for a long contraction: that can be cut into four ranges, or into
-// two that are still long, while the rows do not outgrow the contraction.
-// Measured (whole call by graph replay, small / 128 x 256 tiles, us): FFN 1024/2816 127 tokens 16.0 / 16.4, 200 tokens
-// 19.4 / 16.9; FFN 4096/11008 1 token 22.6 / 36.0, 127 tokens 49.6 / 48.0, 200 tokens 56.8 / 49.4; linear 4096 x 4096 1 token
-// 6.6 / 11.0, 127 tokens 12.1 / 14.4, 200 tokens 14.8 / 14.8 (two ranges), 512 tokens 23.1 / 17.3 (one); 4096 -> 1024, 512 tokens (four)
-// 13.2 / 14.8; 11008 -> 4096, 300 tokens (two) 24.7 / 27.6; 16384 -> 1024, 1024 tokens (four) 27.4 / 38.4, 2048 tokens
-// (two) 40.3 / 40.8.
+// Ranges of the contraction for the small kernel, 0: not the small kernel.
+// Plain products: one row tile a modality, and more of them where 128 x 256 tiles would leave most SMs idle for a long
+// contraction: one that can be cut into four ranges, or into two that are still long, while the rows do not outgrow it.
+// Gate/up: up to 64 rows, whose longer tail (two matrices added up, rounded to 4 bits) still costs less than the few 128 x 256
+// tiles; up to 16 where its CTAs, both modalities present, need a second wave.
+// Measured (whole call by graph replay, small / 128 x 256 tiles, us): linear 4096 x 4096 1 token 6.6 / 11.0, 127 tokens 12.1 / 14.4,
+// 200 tokens 14.8 / 14.8 (two ranges), 512 tokens 23.1 / 17.3 (one); 4096 -> 1024, 512 tokens (four) 13.2 / 14.8; 11008 -> 4096,
+// 300 tokens (two) 24.7 / 27.6; 16384 -> 1024, 1024 tokens (four) 27.4 / 38.4, 2048 tokens (two) 40.3 / 40.8.
+// Gate/up one way or the other, one modality, and both: FFN 1024/2816, 48 tokens 12.8 / 13.6, 12.8 / 13.6; 64 tokens
+// 13.6 / 14.0, 13.2 / 13.6; 96 tokens 14.9 / 14.6, 14.5 / 14.2; FFN 4096/11008 (second wave), 16 tokens 23.7 / 26.2,
+// 40.1 / 36.4; 32 tokens 25.2 / 26.7, 40.7 / 37.1.
 // The number of ranges: as many as fill the places on the GPU once (two CTAs an SM), at most four, which always beat
-// eight (linear 4096 x 4096, 64 tokens: 1 / 2 / 4 / 8 ranges 13.3 / 11.0 / 10.7 / 18.6 us).  Gate/up tiles add up two
-// matrices and come out in 4 bits, a longer tail, so they take two ranges only where those CTAs nearly fit one an SM
-// (FFN 512/1024, 64 tokens: 12.3 / 11.5 / 12.0 us with 1 / 2 / 4; FFN 4096/11008, 8 tokens 38.0 / 38.4 / 49.5 us).
-constexpr int kMxSmallTokens = 128;
+// eight (linear 4096 x 4096, 64 tokens: 1 / 2 / 4 / 8 ranges 13.3 / 11.0 / 10.7 / 18.6 us).  Gate/up tiles take two ranges
+// only where those CTAs nearly fit one an SM (FFN 512/1024, 64 tokens: 12.3 / 11.5 / 12.0 us with 1 / 2 / 4; FFN 4096/11008,
+// 8 tokens 38.0 / 38.4 / 49.5 us).
 static int mx_small_splits(int64_t M, int64_t n_out, int64_t k, bool glu) {
   const int forced = tune_overrides().narrow;
-  const int64_t steps = (mx_code_ld(k) + 127) / 128;
-  if (forced == 0 || (forced < 0 && M > kMxSmallTokens && (glu || M > 32 * steps))) return 0;
+  const int64_t steps = (mx_code_ld(k) + 127) / 128, places = 2 * usable_sms();
+  if (forced == 0) return 0;
   const int64_t m_tiles = (M + MX_BM - 1) / MX_BM + (M > 1 ? 1 : 0);
   const int64_t tiles = m_tiles * ((n_out + MXS_N - 1) / MXS_N) * (glu ? 2 : 1);
-  const int64_t most = glu ? usable_sms() * 5 / 4 : 2 * usable_sms();
+  const int64_t most = glu ? usable_sms() * 5 / 4 : places;
   int splits = 1;
   while (splits < (glu ? 2 : 4) && tiles * splits * 2 <= most && steps >= splits * 2) splits *= 2;
-  if (forced < 0 && M > kMxSmallTokens && (splits == 1 || splits * steps < 64)) return 0;
-  return splits;
+  const bool fits = glu ? M <= (tiles <= places ? 64 : 16)
+                        : M <= MX_BM || (M <= 32 * steps && splits > 1 && splits * steps >= 64);
+  return fits || forced > 0 ? splits : 0;
 }
 
 // The activations of a call that a small kernel rounds itself (SELF), and where it leaves the routing lists.
