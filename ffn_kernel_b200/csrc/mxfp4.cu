@@ -199,6 +199,8 @@ __global__ void __launch_bounds__(kRouteThreads, kQuantPerSm) mx_route_quantize_
 // rows x one atom of four blocks; a thread reads the 32 values of one block of one row, or of two neighbouring rows at
 // once, so that a warp reads 128 contiguous bytes a column; the codes go through shared memory so that a row leaves as
 // 64 contiguous bytes.  `pairs`: the 16-bit columns are 4-byte aligned.
+// Bound by HBM once the inner tiles did without a predicate and a 64-bit product a load (uniform column addresses) and the
+// maximum is one instruction for two values: 11008 x 4096 fp32 37.9 -> 32.9 us = 6.2 TB/s, bf16 34.5 -> 20.7 us = 5.5 TB/s.
 template <typename T> struct MxCols {
   static constexpr int per_thread = 4 / sizeof(T);
   static constexpr int rows = 64 * per_thread;
@@ -214,35 +216,52 @@ __global__ void __launch_bounds__(kQuantThreads, 4) mx_quantize_cols_kernel(cons
   const int64_t ld = mx_code_ld(cols), k_atoms = mx_k_atoms(cols);
   const int64_t row_tiles = mx_row_atoms(rows) * (128 / R);
   const int64_t tiles = row_tiles * k_atoms;
-  const int lr = (tid & 63) * P, b = tid >> 6;
+  const int lr = (tid & 63) * P, b = __shfl_sync(0xFFFFFFFFu, tid >> 6, 0);     // a warp has one block
   for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
     const int64_t atom = t / row_tiles, r0 = (t - atom * row_tiles) * R;
-    const int64_t r = r0 + lr, c0 = atom * 128 + b * 32;
     uint32_t w[32];                          // one fp32, or two 16-bit values of neighbouring rows
-    const T* src = x + c0 * ldc + r;
+    if (pairs && r0 + R <= rows && atom * 128 + 128 <= cols) {       // the same for the whole CTA
+      // uniform addresses of the columns, one offset a lane
+      const T* base = x + (atom * 128 + b * 32) * ldc + r0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      w[i] = 0;
-      if (c0 + i < cols) {
-        if constexpr (P == 1) {
-          if (r < rows) w[i] = reinterpret_cast<const uint32_t*>(src)[i * ldc];
-        } else {
-          const unsigned short* q = reinterpret_cast<const unsigned short*>(src) + i * ldc;
-          if (pairs && r + 1 < rows) w[i] = __ldg(reinterpret_cast<const uint32_t*>(q));
-          else if (r < rows) w[i] = q[0] | (r + 1 < rows ? static_cast<uint32_t>(q[1]) << 16 : 0u);
+      for (int i = 0; i < 32; ++i)
+        w[i] = __ldg(reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(base + i * ldc) + lr * static_cast<int>(sizeof(T))));
+    } else {
+      const int64_t r = r0 + lr, c0 = atom * 128 + b * 32;
+      const T* src = x + c0 * ldc + r;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        w[i] = 0;
+        if (c0 + i < cols) {
+          if constexpr (P == 1) {
+            if (r < rows) w[i] = reinterpret_cast<const uint32_t*>(src)[i * ldc];
+          } else {
+            const unsigned short* q = reinterpret_cast<const unsigned short*>(src) + i * ldc;
+            if (r < rows) w[i] = q[0] | (r + 1 < rows ? static_cast<uint32_t>(q[1]) << 16 : 0u);
+          }
         }
       }
     }
+    uint32_t top = 0;                        // largest magnitude, of both rows side by side where there are two
+    if constexpr (P == 1) {
+      float t = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) t = max_abs3(t, __uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+      top = __float_as_uint(t) & 0x7FFFFFFFu;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
+    }
 #pragma unroll
     for (int h = 0; h < P; ++h) {
+      MxRaw one;
+      one.w[0] = top;
+      const uint32_t m = __float_as_uint(raw_value<T>(one, h));
       float v[32];
-      uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        MxRaw one;
         one.w[0] = w[i];
         v[i] = raw_value<T>(one, h);
-        m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
       }
       const uint32_t byte = mx_scale_byte(m);
       const float inv = mx_inverse_scale(byte);
@@ -283,9 +302,13 @@ struct MxDequantJob {
   const int* counts;
 };
 
-// 32 bytes of output a lane, one 256-bit store: 16 values of a 16-bit type or 8 of fp32.  blockIdx.y: which group of
-// `per_warp` chunks of every row; the next row's codes and scales are in flight while one is written.
-// Measured: 32768 x 4096 to bf16 63 us = 5.4 TB/s, 11008 x 4096 to fp32 40.7 us = 5.0 TB/s (four fifths of it writes).
+// 32 bytes of output a lane, one 256-bit store: 16 values of a 16-bit type or 8 of fp32.  A warp takes units of `per_warp`
+// chunks of a row, the units of a row to neighbouring warps, so that a CTA writes several KiB in a row; the next unit's codes and
+// scales are in flight while one is written.
+// Measured: 11008 x 4096 to bf16 21.4 us = 5.3 TB/s, to fp32 38.2 us = 5.3 TB/s (four fifths and nine tenths of it writes).
+// chunks of a unit: 2 KiB of a 16-bit type, 8 KiB of fp32 (11008 x 4096: 1 / 2 / 4 / 8 chunks of bf16 23.7 / 21.2 / 22.0 / 24.7 us, of
+// fp32 41.3 / 40.1 / 40.0 / 38.4)
+template <typename T> constexpr int kDequantChunks = sizeof(T) == 4 ? 8 : 2;
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads, kQuantPerSm) mx_dequantize_kernel(const __grid_constant__ MxDequantJob job, int per_warp) {
   using L = MxLane<T>;
@@ -294,22 +317,25 @@ __global__ void __launch_bounds__(kQuantThreads, kQuantPerSm) mx_dequantize_kern
   const uint8_t* __restrict__ codes = job.codes[w];
   const uint8_t* __restrict__ scales = job.scales[w];
   T* __restrict__ out = static_cast<T*>(job.out[w]);
-  const int rows = static_cast<int>(job.rows[w]), cols = static_cast<int>(job.cols[w]);
+  const int64_t rows = job.rows[w];
+  const int cols = static_cast<int>(job.cols[w]);
   const int lane = threadIdx.x & 31;
-  const int first = blockIdx.y * per_warp;
-  if (first * L::chunk >= cols) return;
   const int64_t ldo = job.ldo[w];
   const bool vec = ((reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(ldo * sizeof(T))) & 31) == 0;
   const int64_t ld = mx_code_ld(cols);
   const int k_atoms = static_cast<int>(mx_k_atoms(cols));
-  const int step = gridDim.x * (kQuantThreads / 32), r0 = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
-  uint32_t code[kChunksMax][L::values / 8] = {}, byte[kChunksMax] = {};
-  auto load = [&](int64_t r) {
+  const int width = per_warp * L::chunk, groups = (cols + width - 1) / width;
+  const int warps = gridDim.x * (kQuantThreads / 32), w0 = blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
+  const int row_step = warps / groups, group_step = warps - row_step * groups;
+  int64_t r = w0 / groups;
+  int g = w0 - static_cast<int>(r) * groups;
+  uint32_t code[kDequantChunks<T>][L::values / 8] = {}, byte[kDequantChunks<T>] = {};
+  auto load = [&]() {
     if (r >= rows) return;
     const uint8_t* scale_row = scales + mx_scale_word(r, 0, k_atoms);
 #pragma unroll
-    for (int u = 0; u < kChunksMax; ++u) {
-      const int c = (first + u) * L::chunk + lane * L::values;
+    for (int u = 0; u < kDequantChunks<T>; ++u) {
+      const int c = g * width + u * L::chunk + lane * L::values;
       if (u < per_warp && c < cols) {
         if constexpr (L::values == 16) {
           const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes + r * ld + c / 2));
@@ -322,19 +348,27 @@ __global__ void __launch_bounds__(kQuantThreads, kQuantPerSm) mx_dequantize_kern
       }
     }
   };
-  load(r0);
-  for (int64_t r = r0; r < rows; r += step) {
-    uint32_t cur[kChunksMax][L::values / 8], sb[kChunksMax];
+  load();
+  while (r < rows) {
+    uint32_t cur[kDequantChunks<T>][L::values / 8], sb[kDequantChunks<T>];
 #pragma unroll
-    for (int u = 0; u < kChunksMax; ++u) {
+    for (int u = 0; u < kDequantChunks<T>; ++u) {
 #pragma unroll
       for (int j = 0; j < L::values / 8; ++j) cur[u][j] = code[u][j];
       sb[u] = byte[u];
     }
-    load(r + step);
+    const int c0 = g * width + lane * L::values;
+    T* row = out + r * ldo;
+    r += row_step;
+    g += group_step;
+    if (g >= groups) {
+      g -= groups;
+      ++r;
+    }
+    load();
 #pragma unroll
-    for (int u = 0; u < kChunksMax; ++u) {
-      const int c = (first + u) * L::chunk + lane * L::values;
+    for (int u = 0; u < kDequantChunks<T>; ++u) {
+      const int c = c0 + u * L::chunk;
       if (u >= per_warp || c >= cols) break;
       const float s = mx_scale_value(sb[u]);
       __align__(32) T e[L::values];
@@ -345,7 +379,7 @@ __global__ void __launch_bounds__(kQuantThreads, kQuantPerSm) mx_dequantize_kern
 #pragma unroll
         for (int i = 0; i < 8; ++i) mx_put(&e[8 * j + i], mul_keep_subnormals(v[i], s));
       }
-      T* o = out + r * ldo + c;
+      T* o = row + c;
       if (vec && c + L::values <= cols) {
         const uint32_t* q = reinterpret_cast<const uint32_t*>(e);
         asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]),
@@ -400,8 +434,7 @@ static int quantize_typed(const void* x_, int64_t row_stride, int64_t col_stride
         row_alignment(x, row_stride * static_cast<int64_t>(sizeof(E))), q.per_warp);
   } else {
     int64_t tiles = mx_row_atoms(rows) * (128 / MxCols<E>::rows) * mx_k_atoms(cols);
-    const int64_t most = static_cast<int64_t>(device_info().sm_count) * 8;
-    if (tiles > most) tiles = most;
+    if (tiles > (1 << 30)) tiles = 1 << 30;
     mx_quantize_cols_kernel<E><<<static_cast<unsigned>(tiles), kQuantThreads, 0, s>>>(
         x, col_stride, rows, cols, c, sc, ((reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(col_stride * sizeof(E))) & 3) == 0);
   }
@@ -458,8 +491,8 @@ int mx_dequantize_weights(const void* const* codes, const void* const* scales, c
     most_cols = cols[i] > most_cols ? cols[i] : most_cols;
   }
   job.counts = counts;
-  QuantShape q = quant_shape(most_rows, most_cols, MxLane<__nv_bfloat16>::chunk, kChunksMax, kQuantPerSm, n);
-  q.grid.z = n;
+  QuantShape q = quant_shape(most_rows, most_cols, MxLane<__nv_bfloat16>::chunk, kDequantChunks<__nv_bfloat16>, kQuantPerSm, n);
+  q.grid = dim3(q.grid.x * q.grid.y, 1, n);
   mx_dequantize_kernel<__nv_bfloat16><<<q.grid, kQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(job, q.per_warp);
   return cuda_status(cudaGetLastError());
 }
@@ -504,7 +537,9 @@ extern "C" int ffnk_mxfp4_dequantize(const void* codes, const void* scales, int6
   if ((reinterpret_cast<uintptr_t>(codes) & 15) || (reinterpret_cast<uintptr_t>(scales) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & (size - 1)) || ldo < cols)
     return FFNK_ERR_ALIGN;
-  const QuantShape q = quant_shape(rows, cols, dtype == FFNK_FP32 ? MxLane<float>::chunk : MxLane<__half>::chunk, kChunksMax, kQuantPerSm);
+  QuantShape q = dtype == FFNK_FP32 ? quant_shape(rows, cols, MxLane<float>::chunk, kDequantChunks<float>, kQuantPerSm)
+                                    : quant_shape(rows, cols, MxLane<__half>::chunk, kDequantChunks<__half>, kQuantPerSm);
+  q.grid = dim3(q.grid.x * q.grid.y);
   MxDequantJob job{};
   job.codes[0] = static_cast<const uint8_t*>(codes);
   job.scales[0] = static_cast<const uint8_t*>(scales);

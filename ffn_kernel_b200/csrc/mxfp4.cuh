@@ -54,6 +54,12 @@ __device__ __forceinline__ float mul_keep_subnormals(float a, float b) {
   asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// max(|a|, |b|, |c|), a NaN if one of them is
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // eight scaled values -> eight codes, the first in the lowest four bits
 __device__ __forceinline__ uint32_t mx_pack8(const float (&v)[8]) {
   uint32_t r;
