@@ -192,12 +192,22 @@ __device__ __forceinline__ float mx_silu_mul_keep(float& t1, float& t3) {
   return h;
 }
 
+// bits of the largest magnitude of 32 values (four chains, for their latency)
+__device__ __forceinline__ uint32_t mx_block_top(const float (&v)[32]) {
+  float t[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    t[k] = max_abs3(v[k], v[k + 4], v[k + 8]);
+    t[k] = max_abs3(t[k], v[k + 12], v[k + 16]);
+    t[k] = max_abs3(t[k], v[k + 20], v[k + 24]);
+  }
+  const float u = max_abs3(max_abs3(t[0], v[28], v[29]), max_abs3(t[1], v[30], v[31]), max_abs3(t[2], t[3], t[3]));
+  return __float_as_uint(u) & 0x7FFFFFFFu;
+}
+
 // One block (32 values of one row): scale byte and 16 bytes of codes.
 __device__ __forceinline__ uint32_t mx_quantize_block(const float (&v)[32], uint4& codes) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  const uint32_t byte = mx_scale_byte(m);
+  const uint32_t byte = mx_scale_byte(mx_block_top(v));
   const float inv = mx_inverse_scale(byte);
   uint32_t w[4];
 #pragma unroll
@@ -270,10 +280,7 @@ __device__ __forceinline__ void mx_issue_step(uint32_t d, uint32_t tmem, uint32_
 
 // One row's 32 factors for the backward pass (pre_tile_offset: fp16 with a shared exponent).
 __device__ __forceinline__ void mx_keep_block(const float (&v)[32], __half* base, int64_t pre_rows, int64_t row, int n0, int h) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  const uint32_t byte = pre_scale_byte(m);
+  const uint32_t byte = pre_scale_byte(mx_block_top(v));
   const float inv = pre_inverse_scale(byte);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -337,9 +344,11 @@ __device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, c
       // columns past h are weight rows that do not exist: zeros, whatever their scales hold
       if constexpr (EPI == MX_EPI_GLU_SAVE) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          v[e] = mx_silu_mul_keep(a[e], b[e]);
-          if (n0 + e >= p.n_out) v[e] = a[e] = b[e] = 0.0f;
+        for (int e = 0; e < 32; ++e) v[e] = mx_silu_mul_keep(a[e], b[e]);
+        if (n0 + 32 > p.n_out) {                // warp-uniform
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (n0 + e >= p.n_out) v[e] = a[e] = b[e] = 0.0f;
         }
         if (valid && n0 < p.n_out) {
           mx_keep_block(a, p.f1, p.pre_rows, drow, n0, p.n_out);
