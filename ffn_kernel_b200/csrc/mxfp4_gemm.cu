@@ -1103,12 +1103,15 @@ static int mx_group_m(int64_t k, int64_t rows_per_tile) {
 static int mx_a_box_rows(int64_t M) { return M >= MX_BM || tune_overrides().pair > 0 ? MX_BM : static_cast<int>((M + 7) / 8 * 8); }
 
 // CTA pairs or single CTAs.  Pairs halve the weight traffic of an SM but hand tiles out in twice the size and pay for
-// signals between the two: worth it for long contractions, or for many rows.  Measured (single / pairs, us): linear
-// 4096 x 4096 1000 tokens 21.0 / 23.8, 1500 tokens 28.8 / 27.2, 8192 tokens 76.9 / 72.6; 1024 x 1024 4096 tokens
-// 14.7 / 15.6; FFN 2048/5504 4096 tokens 80.1 / 73.0; FFN 1024/2816 4096 tokens 36.2 / 38.7, 8192 tokens 55.7 / 55.0.
-static bool mx_pairs(int64_t M, int64_t k) {
+// signals between the two: worth it for long contractions, or for many rows; the gate/up tiles, with their longer epilogue,
+// later.  Measured (single / pairs, us): linear 1024 -> 1024, 4096 tokens 14.4 / 14.9, 32768 tokens 50.4 / 48.8; 1024 -> 4096,
+// 8192 tokens 34.0 / 32.8; 1536 -> 4096, 1500 tokens 18.1 / 16.2, 8192 tokens 39.6 / 37.4; 4096 x 4096, 1000 tokens 21.0 / 23.8,
+// 8192 tokens 76.9 / 72.6; FFN (both products) 2048/5504, 4096 tokens 80.1 / 73.0; 1024/2816, 4096 tokens 34.0 / 38.1, 32768
+// tokens 159 / 164.
+static bool mx_pairs(int64_t M, int64_t k, bool glu) {
   const int forced = tune_overrides().pair;
-  return forced >= 0 ? forced != 0 : M >= 8192 || (k >= 2048 && M > 1024);
+  if (forced >= 0) return forced != 0;
+  return (M > 1024 && k >= (glu ? 2048 : 1536)) || (!glu && M >= 8192 && k >= 1024);
 }
 
 // Dynamic shared memory of a kernel
@@ -1246,7 +1249,7 @@ static int mx_launch_small(const MxMaps& maps, const MxParams& p, int64_t M, int
 static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt, const int32_t* perm, const int32_t* counts,
                       const void* mask, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, const MxSelf* self, int32_t* status,
                       cudaStream_t s) {
-  const bool pairs = mx_pairs(M, K);
+  const bool pairs = mx_pairs(M, K, false);
   const int splits = mx_small_splits(M, N, K, false);
   const MxWeight w[2] = {wv, wt};
   const int slots[2] = {0, 2};
@@ -1276,7 +1279,7 @@ static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* p
                      int32_t* status, cudaStream_t s) {
   const int slots[4] = {0, 1, 2, 3};
   const int splits = mx_small_splits(M, h, d, true);
-  const bool pairs = mx_pairs(M, d);
+  const bool pairs = mx_pairs(M, d, true);
   MxMaps m{};
   const int r = mx_maps(m, a, M, w, slots, 4, h, d, mx_a_box_rows(M), MX_BN / 2, pairs && !splits ? 1 : 0);
   if (r) return r;
