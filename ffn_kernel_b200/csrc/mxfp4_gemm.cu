@@ -1106,12 +1106,12 @@ static int mx_a_box_rows(int64_t M) { return M >= MX_BM || tune_overrides().pair
 // signals between the two: worth it for long contractions, or for many rows; the gate/up tiles, with their longer epilogue,
 // later.  Measured (single / pairs, us): linear 1024 -> 1024, 4096 tokens 14.4 / 14.9, 32768 tokens 50.4 / 48.8; 1024 -> 4096,
 // 8192 tokens 34.0 / 32.8; 1536 -> 4096, 1500 tokens 18.1 / 16.2, 8192 tokens 39.6 / 37.4; 4096 x 4096, 1000 tokens 21.0 / 23.8,
-// 8192 tokens 76.9 / 72.6; FFN (both products) 2048/5504, 4096 tokens 80.1 / 73.0; 1024/2816, 4096 tokens 34.0 / 38.1, 32768
-// tokens 159 / 164.
+// 8192 tokens 76.9 / 72.6; FFN with pairs for the second product, gate/up single / pairs: 2048/5504, 1500 tokens 38.2 / 40.3,
+// 4096 tokens 69.3 / 70.4, with gradient 376 / 359; 4096/11008, 4096 tokens 219 / 217; 1024/2816, 16384 tokens 83.4 / 88.7.
 static bool mx_pairs(int64_t M, int64_t k, bool glu) {
   const int forced = tune_overrides().pair;
   if (forced >= 0) return forced != 0;
-  return (M > 1024 && k >= (glu ? 2048 : 1536)) || (!glu && M >= 8192 && k >= 1024);
+  return glu ? M > 2048 && k >= 2048 : (M > 1024 && k >= 1536) || (M >= 8192 && k >= 1024);
 }
 
 // Dynamic shared memory of a kernel
