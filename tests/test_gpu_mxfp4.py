@@ -77,6 +77,30 @@ def test_quantize_every_tie_and_special_value(dev, name):
     assert torch.equal(torch.nan_to_num(back), torch.nan_to_num(want))
 
 
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_special_values_in_every_place(dev, name):
+    dt = DTYPES[name]
+    info = torch.finfo(dt)
+    some = torch.tensor([float("inf"), float("-inf"), float("nan"), info.max, -info.max, info.smallest_normal, info.smallest_normal * info.eps,
+                         -info.smallest_normal * info.eps, -0.0])
+    x = spread(300, 520, 1, dt)
+    g = torch.Generator().manual_seed(2)
+    for i in range(400):
+        r, c = (int(torch.randint(0, n, (), generator=g)) for n in x.shape)
+        x[r, c] = some[i % len(some)].to(dt)
+        if i % len(some) > 4:                       # small ones matter where nothing hides them
+            b = c // 32 * 32
+            x[r, b:b + 32] = 0
+            x[r, c] = some[i % len(some)].to(dt)
+    minus_nan = torch.tensor([-1], dtype=torch.int32 if dt is torch.float32 else torch.int16).view(dt)
+    x[7, 9] = x[299, 519] = x[150, 260] = minus_nan[0]
+    same_matrix(quantize_mxfp4(x.to(dev)), x)
+    same_matrix(quantize_mxfp4(x.T.contiguous().to(dev), dim=0), x)
+    wide = torch.empty(520, 333, dtype=dt, device=dev)[:, 1:301]             # columns that are not 4-byte aligned in 16 bits
+    wide.copy_(x.T)
+    same_matrix(quantize_mxfp4(wide, dim=0), x)
+
+
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 31), (130, 72), (257, 300), (9, 1031)])
 def test_dequantize_any_codes_and_scales(dev, rows, cols):
     g = torch.Generator().manual_seed(rows)
