@@ -409,7 +409,9 @@ int ffnk_debug_profile_buffer(void* buffer);
  * "max_run_rows", "copy_threshold", "verbose", "route_resident" (0: long masks are routed by the count and
  * scatter kernels even where the one-launch kernel fits), "ksplit" (down projection inside ffnk_ffn_forward: 0 never
  * splits the contraction, n > 1 splits it n ways wherever it can), "early_start" (0: the GEMMs inside
- * ffnk_ffn_forward never start beside their predecessor); value -1 restores the table's own choice.  Process-wide,
+ * ffnk_ffn_forward never start beside their predecessor).  The MXFP4 forward calls read "pair" (CTA pairs or single CTAs),
+ * "narrow" (1: the split kernel always, 0: never), "permute" (0: no kernel rounds its activations itself) and
+ * "early_start".  Value -1 restores the table's own choice.  Process-wide,
  * affects later launches; unknown names return FFNK_ERR_SHAPE.  The library reads no environment variables. */
 int ffnk_tune_override(const char* name, int value);
 
