@@ -40,8 +40,8 @@ __device__ __forceinline__ void quantize_chunk(const MxRaw& raw, int chunk, int 
   for (int j = 0; j < L::values / 8; ++j) {
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = mul_keep_subnormals(raw_value<T>(raw, 8 * j + i), inv);
-    code[j] = byte == 255u ? 0u : mx_pack8(v);
+    for (int i = 0; i < 8; ++i) v[i] = raw_value<T>(raw, 8 * j + i);
+    code[j] = mx_round8(v, byte, inv);
   }
   const int c = chunk * L::chunk + lane * L::values;
   if (c < ((cols + 31) & ~31)) {
@@ -270,8 +270,8 @@ __global__ void __launch_bounds__(kQuantThreads, 4) mx_quantize_cols_kernel(cons
       for (int j = 0; j < 4; ++j) {
         float a[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = mul_keep_subnormals(v[8 * j + i], inv);
-        c[j] = byte == 255u ? 0u : mx_pack8(a);
+        for (int i = 0; i < 8; ++i) a[i] = v[8 * j + i];
+        c[j] = mx_round8(a, byte, inv);
       }
       s_code[lr + h][b] = make_uint4(c[0], c[1], c[2], c[3]);
       s_scale[lr + h][b] = static_cast<uint8_t>(byte);

@@ -73,6 +73,13 @@ __device__ __forceinline__ uint32_t mx_pack8(const float (&v)[8]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
+// eight values of a block -> eight codes: the one place where values are rounded to four bits.  inv: mx_inverse_scale(byte).
+__device__ __forceinline__ uint32_t mx_round8(const float (&x)[8], uint32_t byte, float inv) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = mul_keep_subnormals(x[i], inv);
+  return byte == 255u ? 0u : mx_pack8(v);
+}
 // eight codes -> eight values (exact in fp16)
 __device__ __forceinline__ void mx_unpack8(uint32_t c, float (&v)[8]) {
   uint32_t h[4];

@@ -180,13 +180,16 @@ __device__ __forceinline__ void mx_store_rows(const float (&v)[32], unsigned lon
 
 // silu(t1) * t3 with an exponential and a reciprocal good to a few units in the last fp32 place: what is rounded
 // to four bits next must not sit on the wrong side of a tie more often than fp32 sums put it there anyway
-// (a hyperbolic tangent of 2^-11 would move one value in a thousand by a whole step).
-__device__ __forceinline__ float mx_silu_mul(float t1, float t3) { return __fdividef(t1, 1.0f + __expf(-t1)) * t3; }
+// (a hyperbolic tangent of 2^-11 would move one value in a thousand by a whole step).  The product with t3 keeps
+// subnormals, as the rounding does; silu itself is 0 where it is below 2^-119 (t1 < -87.3: the reciprocal's range ends).
+__device__ __forceinline__ float mx_silu_mul(float t1, float t3) {
+  return mul_keep_subnormals(__fdividef(t1, 1.0f + __expf(-t1)), t3);
+}
 // The same value, and the two factors of the backward pass: f3 = dh/dt3 = silu(t1), f1 = dh/dt1 = t3 s (1 + t1 (1 - s)).
 __device__ __forceinline__ float mx_silu_mul_keep(float& t1, float& t3) {
   const float d = 1.0f + __expf(-t1);
   const float f3 = __fdividef(t1, d), s = __fdividef(1.0f, d);
-  const float h = f3 * t3;
+  const float h = mul_keep_subnormals(f3, t3);
   t1 = t3 * fmaf(f3, 1.0f - s, s);
   t3 = f3;
   return h;
@@ -214,8 +217,8 @@ __device__ __forceinline__ uint32_t mx_quantize_block(const float (&v)[32], uint
   for (int j = 0; j < 4; ++j) {
     float a[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = v[8 * j + i] * inv;
-    w[j] = byte == 255u ? 0u : mx_pack8(a);
+    for (int i = 0; i < 8; ++i) a[i] = v[8 * j + i];
+    w[j] = mx_round8(a, byte, inv);
   }
   codes = make_uint4(w[0], w[1], w[2], w[3]);
   return byte;
@@ -705,8 +708,8 @@ __device__ __forceinline__ void mx_self_quantize(const MxSmall& q, const int* to
       for (int j = 0; j < 2; ++j) {
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = mul_keep_subnormals(raw_value<__nv_bfloat16>(raw[i], 8 * j + e), inv);
-        code[j] = byte == 255u ? 0u : mx_pack8(v);
+        for (int e = 0; e < 8; ++e) v[e] = raw_value<__nv_bfloat16>(raw[i], 8 * j + e);
+        code[j] = mx_round8(v, byte, inv);
       }
       if (ks0 + ks < ks1) {
         const int piece = (lane & 15) >> 1;              // 16-byte piece of the row = block of the k-step
@@ -1040,10 +1043,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
         const uint32_t byte = mx_scale_byte(m);
-        const float inv = mx_inverse_scale(byte);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= inv;
-        const uint32_t code = byte == 255u ? 0u : mx_pack8(v);
+        const uint32_t code = mx_round8(v, byte, mx_inverse_scale(byte));
         const int block = nt * 4 + (lane >> 3);
         if (block * 32 < p.n_out) *reinterpret_cast<uint16_t*>(p.codes + drow * p.code_ld + block * 16 + (lane & 7) * 2) = static_cast<uint16_t>(code);
         if ((lane & 7) == 0) p.scales[mx_scale_word(drow, nt, p.k_atoms_out) + (lane >> 3)] = static_cast<uint8_t>(byte);

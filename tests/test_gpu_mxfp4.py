@@ -559,3 +559,23 @@ def test_offsets_beyond_32_bits(dev):
     torch.cuda.empty_cache()
     tail(540_000, 64, [(8200, 64), (64, 8200), (8200, 64)] * 2, MXFP4MaskedFFN, R.ffn, R.ffn_dx)
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------------------ hidden values below 2^-126
+def tiny_hidden(M, d, h, dev):
+    """FFN weights and activations whose hidden values are all 2^-127: the smallest block exponent, code 1.0."""
+    w1, w3, w2 = torch.zeros(h, d), torch.zeros(h, d), torch.zeros(d, h)
+    x = torch.zeros(M, d)
+    x[:, 0], w1[:, 0], w3[:, 0], w2[:, 0] = 2.0 ** -30, 2.0 ** -40, 2.0 ** -26, 2.0 ** 100    # t1 2^-70 (silu: half of it), t3 2^-56
+    qs = [quantize_mxfp4(w.to(torch.bfloat16).to(dev)) for w in (w1, w2, w3)] * 2
+    return x.to(torch.bfloat16).to(dev), qs, torch.full((M, d), 2.0 ** -27, dtype=torch.bfloat16, device=dev)
+
+
+# a few tokens (split kernel), single CTAs, CTA pairs
+@pytest.mark.parametrize("M,d,h", [(1, 64, 96), (40, 64, 96), (200, 64, 96), (2305, 2048, 96)])
+@pytest.mark.parametrize("train", [False, True])
+def test_hidden_values_keep_subnormals(dev, M, d, h, train):
+    # every step is a power of two: silu(2^-70) = 2^-71 to fp32, so the result is exact
+    x, qs, want = tiny_hidden(M, d, h, dev)
+    y = MXFP4MaskedFFN.apply(x.requires_grad_(train), *qs, edge_mask(M, "alternating").to(dev))
+    assert torch.equal(y.detach(), want)
