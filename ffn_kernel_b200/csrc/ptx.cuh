@@ -95,10 +95,11 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// Arrival at another CTA's barrier that hands over tensor memory only (tcgen05 fences order that).  A release at
-// cluster scope would first wait for this thread's global stores, the rows of the tile before: 1800 cycles a tile.
+// Arrival at another CTA's barrier that hands over tensor memory only: the reads are complete (tcgen05.wait::ld) and
+// the tcgen05 fences on both sides order them around it, so it has to reach the cluster and orders nothing itself.  A release
+// at cluster scope would first wait for this thread's global stores, the rows of the tile before: 1800 cycles a tile.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ uint32_t mapa_shared(uint32_t cta_addr, uint32_t cta_rank) {
   uint32_t r;

@@ -8,7 +8,7 @@ import io
 import pytest
 import torch
 
-from ffn_kernel_b200 import (GraphedMaskedFFN, MaskedFFNModule, MaskedLinearModule, MXFP4MaskedFFN, MXFP4MaskedFFNModule,
+from ffn_kernel_b200 import (GraphedMaskedFFN, MaskedFFN, MaskedFFNModule, MaskedLinearModule, MXFP4MaskedFFN, MXFP4MaskedFFNModule,
                              MXFP4MaskedLinear, MXFP4MaskedLinearModule, MXFP4Tensor, check_status, dequantize_mxfp4,
                              quantize_mxfp4)
 from ffn_kernel_b200.synth import edge_mask
@@ -579,3 +579,23 @@ def test_hidden_values_keep_subnormals(dev, M, d, h, train):
     x, qs, want = tiny_hidden(M, d, h, dev)
     y = MXFP4MaskedFFN.apply(x.requires_grad_(train), *qs, edge_mask(M, "alternating").to(dev))
     assert torch.equal(y.detach(), want)
+
+
+# ------------------------------------------------------------------------------------------------ CTA pairs
+def test_repeated_calls_on_cta_pairs_give_the_same_bits(dev):
+    # enough tiles that every pair hands its accumulators over several times, 4-bit and bf16 products alike
+    M, d, h = 9001, 2056, 2824
+    x, g, mask = spread(M, d, 1).to(dev), spread(M, d, 2).to(dev), edge_mask(M, "span", 1).to(dev)
+    qs, _ = ffn_weights(d, h, 2, dev)
+    ws = [dequantize_mxfp4(q).T.contiguous() for q in qs]
+    x.requires_grad_(True)
+
+    def once():
+        y, z = MXFP4MaskedFFN.apply(x, *qs, mask), MaskedFFN.apply(x, *ws, mask)
+        return [y.detach(), z.detach(), *torch.autograd.grad((y, z), (x,), (g, g))]
+
+    first = once()
+    for _ in range(10):
+        for a, b in zip(first, once()):
+            assert torch.equal(a, b)
+    check_status()
