@@ -599,3 +599,71 @@ def test_repeated_calls_on_cta_pairs_give_the_same_bits(dev):
         for a, b in zip(first, once()):
             assert torch.equal(a, b)
     check_status()
+
+
+@pytest.fixture
+def forced(libffnk):
+    """forced(pair=1, narrow=0): kernel choices set for one test (the tables decide again afterwards)."""
+    names = []
+
+    def choose(**choices):
+        for name, value in choices.items():
+            names.append(name)
+            assert libffnk.ffnk_tune_override(name.encode(), value) == 0
+    yield choose
+    for name in names:
+        libffnk.ffnk_tune_override(name.encode(), -1)
+
+
+# CTA pairs by the rule of the library, at its small end and started early beside the routing kernel; a last pair with rows
+# in its first CTA only, a contraction that ends inside a k-step, an odd number of scale atoms, output columns that end in a tile
+PAIR_LINEAR = [(1030, 1544, 264), (1153, 2056, 136), (8200, 1032, 72)]
+PAIR_FFN = [(2050, 2056, 136), (2305, 2056, 328), (4100, 2048, 72)]
+
+
+@pytest.mark.parametrize("M,K,N", PAIR_LINEAR)
+@pytest.mark.parametrize("kind", MASKS)
+def test_linear_on_cta_pairs(dev, M, K, N, kind):
+    test_linear_forward_and_gradient(dev, M, K, N, kind)
+
+
+@pytest.mark.parametrize("M,d,h", PAIR_FFN)
+@pytest.mark.parametrize("kind", MASKS)
+def test_ffn_on_cta_pairs(dev, M, d, h, kind):
+    test_ffn_forward_and_gradient(dev, M, d, h, kind)
+
+
+# one choice or the other whatever the rule: tile kernels with and without pairs down to one token, and the split kernel
+@pytest.mark.parametrize("choices", [dict(pair=1, narrow=0), dict(pair=0, narrow=0), dict(narrow=1, permute=0)], ids=["pairs", "single", "split"])
+@pytest.mark.parametrize("M,d,h", [(1, 64, 136), (130, 1000, 328), (515, 96, 1000)])
+@pytest.mark.parametrize("kind", ["all_text", "alternating", "span"])
+def test_every_kernel_at_every_size(dev, forced, choices, M, d, h, kind):
+    forced(**choices)
+    test_linear_forward_and_gradient(dev, M, d, h, kind)
+    test_ffn_forward_and_gradient(dev, M, d, h, kind)
+
+
+def test_cta_pairs_with_dirty_workspaces_and_two_streams(dev):
+    M, d, h = 2305, 2056, 1544
+    x, mask, g = spread(M, d, 1).to(dev), edge_mask(M, "span", 2).to(dev), spread(M, d, 3).to(dev)
+    qs, _ = ffn_weights(d, h, 4, dev)
+
+    def step(fill):
+        junk = [torch.full((n,), fill, dtype=torch.uint8, device=dev) for n in (1 << 12, 1 << 16, 1 << 20, 1 << 24, 1 << 26)]
+        del junk
+        a = x.detach().requires_grad_(True)
+        z, y = MXFP4MaskedLinear.apply(a, qs[0], qs[3], mask), MXFP4MaskedFFN.apply(a, *qs, mask)
+        return z.detach(), y.detach(), *torch.autograd.grad((z, y), a, (z.detach(), g))
+
+    want = step(0)
+    assert all(torch.isfinite(t).all() for t in want)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device=dev) for _ in range(2)]
+    got = []
+    for rep in range(4):
+        with torch.cuda.stream(streams[rep % 2]):
+            got.append(step(255))
+    torch.cuda.synchronize()
+    for other in got:
+        assert all(torch.equal(a, b) for a, b in zip(want, other))
+    check_status()
