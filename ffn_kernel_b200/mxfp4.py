@@ -7,9 +7,11 @@ bits a value with its share of the scales) and multiplied on the 4-bit tensor-co
 ``MXFP4MaskedLinear.apply(a, q1, q2, mask)``                 ``MaskedLinear`` on 4-bit weights,
 ``MXFP4MaskedFFN.apply(a, q_w1, ..., q_u3, mask)``           ``MaskedFFN`` on 4-bit weights.
 
-Activations come and go in bf16 and are quantised inside the call, row by row in blocks of 32 along the
-contraction, so a token's result depends on that token alone.  Gradients reach the activations (the rounding to 4 bits counts as
-the identity); the weights are frozen.  A block that holds an infinity or a NaN reads back as NaN.
+Activations come and go in bf16 and are quantised inside the call, row by row in blocks of 32 along the contraction: no
+token's values reach another's result.  The number of tokens chooses the kernel, and with it the order of the fp32 sums, so
+between batches of different sizes the last bits may differ (in the FFN a hidden value next to a tie by its 4-bit step).
+Gradients reach the activations (the rounding to 4 bits counts as the identity); the weights are frozen.  A block that
+holds an infinity or a NaN reads back as NaN.
 """
 from __future__ import annotations
 

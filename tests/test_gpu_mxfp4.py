@@ -667,3 +667,28 @@ def test_cta_pairs_with_dirty_workspaces_and_two_streams(dev):
     for other in got:
         assert all(torch.equal(a, b) for a, b in zip(want, other))
     check_status()
+
+
+# ------------------------------------------------------------------------------------------------ kernels by the number of tokens
+def test_a_token_among_few_and_among_many(dev):
+    # rows do not mix; the order of a row's fp32 sums goes by the number of tokens, so that here every batch is held to the
+    # oracle's bound, and to the same bits only against batches of the same size
+    K, N, d, h = 8200, 264, 4104, 328
+    M = 1300
+    mask = edge_mask(M, "span", 3)
+    (b1, b2), vs = weights([(N, K)] * 2, 5, dev)
+    qs, ws = ffn_weights(d, h, 6, dev)
+    x, z, m = spread(M, K, 1), spread(M, d, 2), mask.to(dev)
+    want, bound = R.linear(x[:130], *vs, mask[:130])
+    fwant, fbound = R.ffn(z[:130], ws, mask[:130])
+    for n in (1, 2, 16, 17, 64, 65, 129, 300, 520, M):
+        y, f = MXFP4MaskedLinear.apply(x[:n].to(dev), b1, b2, m[:n]), MXFP4MaskedFFN.apply(z[:n].to(dev), *qs, m[:n])
+        inside(y[:130], (want[:n], bound[:n]))
+        inside(f[:130], (fwant[:n], fbound[:n]))
+        # the same size with other neighbours
+        xo, zo = spread(n, K, 8).to(dev), spread(n, d, 9).to(dev)
+        keep = n // 2
+        xo[keep], zo[keep] = x[keep].to(dev), z[keep].to(dev)
+        assert torch.equal(MXFP4MaskedLinear.apply(xo, b1, b2, m[:n])[keep], y[keep])
+        assert torch.equal(MXFP4MaskedFFN.apply(zo, *qs, m[:n])[keep], f[keep])
+    check_status()
