@@ -692,3 +692,19 @@ def test_a_token_among_few_and_among_many(dev):
         assert torch.equal(MXFP4MaskedLinear.apply(xo, b1, b2, m[:n])[keep], y[keep])
         assert torch.equal(MXFP4MaskedFFN.apply(zo, *qs, m[:n])[keep], f[keep])
     check_status()
+
+
+def test_split_kernel_of_more_tokens_than_a_cta_counts(dev):
+    # few output columns, a contraction so long that 4200 tokens still take the split kernel, whose CTAs then read the
+    # counts of the routing kernel instead of counting the mask
+    M, K, N = 4200, 33800, 72
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn(M, K, device=dev, generator=g).to(torch.bfloat16)
+    (b1, b2), vs = weights([(N, K)] * 2, 5, dev)
+    for kind in ("span", "all_text", "all_visual"):
+        mask = edge_mask(M, kind, 2)
+        poison(dev)
+        y = MXFP4MaskedLinear.apply(x, b1, b2, mask.to(dev))
+        for s in (slice(0, 40), slice(2030, 2070), slice(M - 60, M)):
+            inside(y[s], R.linear(x[s].cpu(), *vs, mask[s]))
+        check_status()
