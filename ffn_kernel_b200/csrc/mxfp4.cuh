@@ -23,7 +23,6 @@
 
 namespace ffnk {
 
-constexpr int kMxBlock = 32;        // values per scale
 constexpr int kMxAtomBytes = 512;   // scales of 128 rows x 4 blocks
 
 __host__ __device__ constexpr int64_t mx_code_ld(int64_t cols) { return (cols + 31) / 32 * 16; }

@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(MxGeom<EPI, CTAS>::threads, 1) mx_gemm_kernel(
 }
 
 // ---------------------------------------------------------------------------------------------
-// Few row tiles: bound by the stream of weights, or by latency.  A cluster of up to eight CTAs owns one tile of 128 rows
+// Few row tiles: bound by the stream of weights, or by latency.  A cluster of up to four CTAs owns one tile of 128 rows
 // x 128 weight rows of one matrix (gate/up: of both, a CTA takes one of them), the contraction cut into `splits` ranges.
 // Every CTA leaves its fp32 partial tile in its own shared memory; after a cluster-wide barrier each CTA adds up a share
 // of the rows out of its peers' shared memory, range by range in order (the same bits whichever CTA is last), and
@@ -638,6 +638,7 @@ __global__ void __launch_bounds__(MxGeom<EPI, CTAS>::threads, 1) mx_gemm_kernel(
 // 4096 x 4096 7.5 -> 6.3 us, FFN 1024/2816 11.2 -> 10.0 us.
 // ---------------------------------------------------------------------------------------------
 constexpr int MXS_N = 128;
+constexpr int MXS_CLUSTER = 4;                              // CTAs of a cluster at most (mx_small_splits)
 constexpr int MXS_THREADS = 192;
 constexpr int MXS_B_BYTES = MXS_N * 128;                    // 16 KiB
 constexpr int MXS_STAGE_FIXED = MXS_B_BYTES + 2 * MX_SF_BYTES;
@@ -974,12 +975,12 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
       const int row = r0 + h * csize * (MXS_THREADS / 32);
       if (row < rows) {
         const uint32_t mine = smem_u32(smem + row * 512 + ((lane ^ (row & 31)) << 4));
-        float4 v[8];
+        float4 v[MXS_CLUSTER];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < MXS_CLUSTER; ++i)
           if (i < csize) v[i] = ld_cluster(mapa_shared(mine, i));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < MXS_CLUSTER; ++i) {
           if (i < csize) {
             float4& d = sum[h][GLU ? i & 1 : 0];
             d.x += v[i].x; d.y += v[i].y; d.z += v[i].z; d.w += v[i].w;
@@ -1179,7 +1180,7 @@ static int mx_small_splits(int64_t M, int64_t n_out, int64_t k, bool glu) {
   const int64_t tiles = m_tiles * ((n_out + MXS_N - 1) / MXS_N) * (glu ? 2 : 1);
   const int64_t most = glu ? usable_sms() * 5 / 4 : places;
   int splits = 1;
-  while (splits < (glu ? 2 : 4) && tiles * splits * 2 <= most && steps >= splits * 2) splits *= 2;
+  while (splits < (glu ? MXS_CLUSTER / 2 : MXS_CLUSTER) && tiles * splits * 2 <= most && steps >= splits * 2) splits *= 2;
   const bool fits = glu ? M <= (tiles <= places ? 64 : 16)
                         : M <= MX_BM || (M <= 32 * steps && splits > 1 && splits * steps >= 64);
   return fits || forced > 0 ? splits : 0;
@@ -1273,7 +1274,7 @@ static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt,
   return splits ? mx_launch_small<false, false>(m, p, M, K, mask, splits, MxSelf{}, s) : mx_launch<MX_EPI_STORE>(m, p, M, pairs, s);
 }
 
-// quantised silu(gate) * up of the routed rows, optionally with the pre-activations kept (f1, f3 both or neither)
+// quantised silu(gate) * up of the routed rows, optionally with the factors of the backward pass kept (f1, f3 both or neither)
 static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* perm, const int32_t* counts, void* codes,
                      void* scales, const void* mask, void* f1, void* f3, int64_t M, int64_t d, int64_t h, const MxSelf* self,
                      int32_t* status, cudaStream_t s) {

@@ -1,5 +1,5 @@
 // Device code of the routing scan that more than one translation unit uses: the mask bytes of a thread as
-// bits, the block-wide scan of visual counts and the compaction of one tile's token indices.
+// bits and the block-wide scan of visual counts.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -80,36 +80,6 @@ __device__ __forceinline__ int block_exclusive_scan(int nv, int* s_warp, int* ti
   }
   *tile_v = total;
   return warp_off + incl - nv;
-}
-
-// Compaction inside the tile: visual indices to s_v[0..tile_v), text indices to s_t[0..tile_t), both
-// ascending.  Every thread walks its own 32 consecutive tokens and appends each index to its modality's
-// list (ev: visual tokens of the tile before this thread; valid: how many of the 32 tokens exist): six
-// instructions a token.  Neighbouring lanes write about 16 words apart, a few-way bank conflict per
-// store, which costs less than the three shuffles and two population counts per token group of a
-// conflict-free warp-transposed order (20 instructions per 32 tokens and lane: the scatter kernel was
-// bound by instruction issue, not by DRAM).
-__device__ __forceinline__ void compact_tile(int* s_v, int* s_t, int tile, uint32_t bits, int ev, int valid) {
-  const int first = static_cast<int>(threadIdx.x) * kRoutePerThread;   // this thread's first token within the tile
-  int* pv = s_v + ev;
-  int* pt = s_t + (first - ev);
-  const int tok0 = tile * kRouteTile + first;
-  if (valid == kRoutePerThread) {
-#pragma unroll
-    for (int i = 0; i < kRoutePerThread; ++i) {
-      const bool vis = (bits >> i) & 1u;
-      *(vis ? pv : pt) = tok0 + i;
-      pv += vis ? 1 : 0;
-      pt += vis ? 0 : 1;
-    }
-  } else {
-    for (int i = 0; i < valid; ++i) {
-      const bool vis = (bits >> i) & 1u;
-      *(vis ? pv : pt) = tok0 + i;
-      pv += vis ? 1 : 0;
-      pt += vis ? 0 : 1;
-    }
-  }
 }
 
 }  // namespace ffnk
