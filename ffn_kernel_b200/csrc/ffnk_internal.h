@@ -98,7 +98,7 @@ int mx_dequantize_weights(const void* const* codes, const void* const* scales, c
                           const int* gate, int n, const int32_t* counts, void* const* out, void* stream);
 
 // dx of the FFN backward alone (frozen weights): w1, w3, u1, u3 bf16 [h, d], w2, u2 [d, h], contiguous; f1, f3 as the
-// forward pass on 4-bit weights keeps them (pre_tile_offset).  gr bf16 [rows, d], dt1, dt3 bf16 [rows, h] scratch, rows = cap + 512.
+// forward pass on 4-bit weights keeps them (kept_tile_offset).  gr bf16 [rows, d], dt1, dt3 bf16 [rows, h] scratch, rows = cap + 512.
 int ffn_backward_dx(const void* gy, int64_t ldg, const void* f1, const void* f3, const void* w1, const void* w2, const void* w3,
                     const void* u1, const void* u2, const void* u3, const int32_t* perm, const int32_t* counts, void* gr,
                     void* dt1, void* dt3, void* dx, int64_t lddx, int64_t M, int64_t d, int64_t h, int32_t* status, void* stream);

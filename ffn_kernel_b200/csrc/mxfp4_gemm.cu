@@ -85,13 +85,13 @@ struct MxParams {
   int k_bytes;             // code bytes of a row along the contraction (a multiple of 16)
   int a_rows;              // rows of an A box (fewer than 128 when no tile has more)
   int group_m;
-  // MX_EPI_STORE: out[token][n]; MX_EPI_GLU_SAVE: the backward pass's factors f1, f3 of pre_rows =
-  // cap + 512 routed rows (pre_tile_offset)
+  // MX_EPI_STORE: out[token][n]; MX_EPI_GLU_SAVE: the backward pass's factors f1, f3 of kept_rows =
+  // cap + 512 routed rows (kept_tile_offset)
   __nv_bfloat16* out;
   int64_t ldo;
   __half* f1;
   __half* f3;
-  int64_t pre_rows;
+  int64_t kept_rows;
   // MX_EPI_GLU*: codes [routed row][code_ld] and scales of the quantised product
   uint8_t* codes;
   uint8_t* scales;
@@ -281,10 +281,10 @@ __device__ __forceinline__ void mx_issue_step(uint32_t d, uint32_t tmem, uint32_
   }
 }
 
-// One row's 32 factors for the backward pass (pre_tile_offset: fp16 with a shared exponent).
-__device__ __forceinline__ void mx_keep_block(const float (&v)[32], __half* base, int64_t pre_rows, int64_t row, int n0, int h) {
-  const uint32_t byte = pre_scale_byte(mx_block_top(v));
-  const float inv = pre_inverse_scale(byte);
+// One row's 32 factors for the backward pass (kept_tile_offset: fp16 with a shared exponent).
+__device__ __forceinline__ void mx_keep_block(const float (&v)[32], __half* base, int64_t kept_rows, int64_t row, int n0, int h) {
+  const uint32_t byte = kept_scale_byte(mx_block_top(v));
+  const float inv = kept_inverse_scale(byte);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (n0 + 8 * j < h) {
@@ -294,10 +294,10 @@ __device__ __forceinline__ void mx_keep_block(const float (&v)[32], __half* base
         const __half2 t = __floats2half2_rn(v[8 * j + 2 * i] * inv, v[8 * j + 2 * i + 1] * inv);
         w[i] = *reinterpret_cast<const uint32_t*>(&t);
       }
-      *reinterpret_cast<uint4*>(base + pre_tile_offset(row, n0 + 8 * j, h)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(base + kept_tile_offset(row, n0 + 8 * j, h)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  reinterpret_cast<uint8_t*>(base + pre_rows * h)[pre_scale_offset(row, n0, h)] = static_cast<uint8_t>(byte);
+  reinterpret_cast<uint8_t*>(base + kept_rows * h)[kept_scale_offset(row, n0, h)] = static_cast<uint8_t>(byte);
 }
 
 // Epilogue of one warp: TMEM lane quarter q, columns of `part` of PARTS.  `on_first` runs once after the first chunk has
@@ -354,8 +354,8 @@ __device__ __forceinline__ void mx_epilogue(uint32_t taddr, const MxParams& p, c
             if (n0 + e >= p.n_out) v[e] = a[e] = b[e] = 0.0f;
         }
         if (valid && n0 < p.n_out) {
-          mx_keep_block(a, p.f1, p.pre_rows, drow, n0, p.n_out);
-          mx_keep_block(b, p.f3, p.pre_rows, drow, n0, p.n_out);
+          mx_keep_block(a, p.f1, p.kept_rows, drow, n0, p.n_out);
+          mx_keep_block(b, p.f3, p.kept_rows, drow, n0, p.n_out);
         }
       } else {
 #pragma unroll
@@ -1018,18 +1018,18 @@ __global__ void __launch_bounds__(MXS_THREADS, 2) mx_small_kernel(const __grid_c
             m1 = max(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
             m3 = max(m3, __shfl_xor_sync(0xFFFFFFFFu, m3, o));
           }
-          const uint32_t k1 = pre_scale_byte(m1), k3 = pre_scale_byte(m3);
+          const uint32_t k1 = kept_scale_byte(m1), k3 = kept_scale_byte(m3);
           if (n0 < p.n_out) {
-            const float i1 = pre_inverse_scale(k1), i3 = pre_inverse_scale(k3);
-            const int64_t o = pre_tile_offset(drow, n0, p.n_out);
+            const float i1 = kept_inverse_scale(k1), i3 = kept_inverse_scale(k3);
+            const int64_t o = kept_tile_offset(drow, n0, p.n_out);
             const __half2 h1[2] = {__floats2half2_rn(t[0] * i1, t[1] * i1), __floats2half2_rn(t[2] * i1, t[3] * i1)};
             const __half2 h3[2] = {__floats2half2_rn(w[0] * i3, w[1] * i3), __floats2half2_rn(w[2] * i3, w[3] * i3)};
             *reinterpret_cast<uint2*>(p.f1 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h1[0]), *reinterpret_cast<const uint32_t*>(&h1[1]));
             *reinterpret_cast<uint2*>(p.f3 + o) = make_uint2(*reinterpret_cast<const uint32_t*>(&h3[0]), *reinterpret_cast<const uint32_t*>(&h3[1]));
             if ((lane & 7) == 0) {
-              const int64_t so = pre_scale_offset(drow, n0, p.n_out);
-              reinterpret_cast<uint8_t*>(p.f1 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k1);
-              reinterpret_cast<uint8_t*>(p.f3 + p.pre_rows * p.n_out)[so] = static_cast<uint8_t>(k3);
+              const int64_t so = kept_scale_offset(drow, n0, p.n_out);
+              reinterpret_cast<uint8_t*>(p.f1 + p.kept_rows * p.n_out)[so] = static_cast<uint8_t>(k1);
+              reinterpret_cast<uint8_t*>(p.f3 + p.kept_rows * p.n_out)[so] = static_cast<uint8_t>(k3);
             }
           }
         } else if (n0 < p.n_out) {
@@ -1296,7 +1296,7 @@ static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* p
   p.k_atoms_out = static_cast<int>(mx_k_atoms(h));
   p.f1 = static_cast<__half*>(f1);
   p.f3 = static_cast<__half*>(f3);
-  p.pre_rows = ffnk_route_capacity(M) + 512;
+  p.kept_rows = ffnk_route_capacity(M) + 512;
   if (self) return mx_launch_small<true, true>(m, p, M, d, mask, splits, *self, s);
   if (splits) return mx_launch_small<true, false>(m, p, M, d, mask, splits, MxSelf{}, s);
   return f1 ? mx_launch<MX_EPI_GLU_SAVE>(m, p, M, pairs, s) : mx_launch<MX_EPI_GLU>(m, p, M, pairs, s);

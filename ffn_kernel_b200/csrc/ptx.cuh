@@ -52,22 +52,22 @@ __device__ __forceinline__ bool mask_is_scattered(const int* counts, int run_thr
 // 1024/2816: that GEMM 58 us against 41); the shared exponent keeps 11 bits for everything down to 2^-28 of the
 // largest and leaves no value out of range.  The factors rather than t1 and t3, because the forward pass has the exponential
 // already (its kernel takes 27 us with both stores) and the backward pass's epilogue then is two products (41 us).
-//   values  element (routed row, column) at pre_tile_offset: tiles of 128 rows x 8 columns
-//   scales  byte (routed row, column / 32) at pre_scale_offset, behind the (cap + 512) * h values
+//   values  element (routed row, column) at kept_tile_offset: tiles of 128 rows x 8 columns
+//   scales  byte (routed row, column / 32) at kept_scale_offset, behind the (cap + 512) * h values
 // so that the 32 rows of a warp are 512 (scales: 32) contiguous bytes.
-__device__ __forceinline__ int64_t pre_tile_offset(int64_t row, int col, int h) {
+__device__ __forceinline__ int64_t kept_tile_offset(int64_t row, int col, int h) {
   return (((row >> 7) * (h >> 3) + (col >> 3)) * 128 + (row & 127)) * 8 + (col & 7);
 }
-__device__ __forceinline__ int64_t pre_scale_offset(int64_t row, int col, int h) {
+__device__ __forceinline__ int64_t kept_scale_offset(int64_t row, int col, int h) {
   return ((row >> 7) * ((h + 31) >> 5) + (col >> 5)) * 128 + (row & 127);
 }
 // bits of max |x| over the 32 -> scale byte and the factor 1 / 2^(byte - 127) (infinities and NaN pass through as such)
-__device__ __forceinline__ uint32_t pre_scale_byte(uint32_t absmax_bits) {
+__device__ __forceinline__ uint32_t kept_scale_byte(uint32_t absmax_bits) {
   const int e = static_cast<int>(absmax_bits >> 23);
   return e == 255 ? 127u : (e > 15 ? static_cast<uint32_t>(e - 14) : 1u);
 }
-__device__ __forceinline__ float pre_inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
-__device__ __forceinline__ float pre_scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
+__device__ __forceinline__ float kept_inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ float kept_scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 __device__ __forceinline__ uint32_t lane_id() { return threadIdx.x & 31; }
 

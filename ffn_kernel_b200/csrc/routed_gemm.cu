@@ -64,9 +64,9 @@ enum { A_GATHER = 0, A_ROUTED = 1 };
 // EPI_DSWIGLU     : acc = dH; with t1 = aux0, t3 = aux1 at the same position:
 //                   out = dH * t3 * s * (1 + t1 * (1 - s)),  aux2 = dH * t1 * s,  s = sigmoid(t1)
 //                   (the element-wise terms of the FFN backward, reference README.md:159-172)
-// EPI_DSWIGLU_PRE : out = dH * f1, aux2 = dH * f3 with the factors f1 = t3 s (1 + t1 (1 - s)) and f3 = t1 s as the forward
-//                   pass on 4-bit weights keeps them in aux0, aux1 (pre_tile_offset, ptx.cuh)
-enum { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_SWIGLU_SAVE = 2, EPI_DSWIGLU = 3, EPI_DSWIGLU_PRE = 4 };
+// EPI_DSWIGLU_KEPT: out = dH * f1, aux2 = dH * f3 with the factors f1 = t3 s (1 + t1 (1 - s)) and f3 = t1 s as the forward
+//                   pass on 4-bit weights keeps them in aux0, aux1 (kept_tile_offset, ptx.cuh)
+enum { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_SWIGLU_SAVE = 2, EPI_DSWIGLU = 3, EPI_DSWIGLU_KEPT = 4 };
 __host__ __device__ constexpr bool epi_glu(int e) { return e == EPI_SWIGLU || e == EPI_SWIGLU_SAVE; }
 // OUT_SCATTER : row of token t -> out[t]            OUT_ROUTED : row i of the routed order -> out[i]
 // OUT_PEER    : row of token t -> row block `peer_rank` of the buffer of the rank that owns token t
@@ -311,10 +311,10 @@ __device__ __forceinline__ void epilogue_glu_staged(uint32_t taddr, const GemmPa
 // the saved pre-activations as well as for the two stores: four accesses per element, each of which
 // would otherwise touch 32 rows per instruction.
 //
-// PRE: instead of t1 and t3 the two factors come in, in fp16 with a shared exponent per 32 columns, tiled so that a lane
+// KEPT: instead of t1 and t3 the two factors come in, in fp16 with a shared exponent per 32 columns, tiled so that a lane
 // reads its own row: the 32 lanes of a warp are 512 contiguous bytes an access, nothing is transposed and nothing left to
 // do but two products.
-template <int BN_T, bool PRE = false>
+template <int BN_T, bool KEPT = false>
 __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const GemmParams& p, long long row_off,
                                                         int n_base, int part, int parts, uint8_t* stg, int lane) {
   constexpr int CH = BN_T / 32;
@@ -368,25 +368,25 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
   };
   const int c_begin = part * CH / parts, c_end = (part + 1) * CH / parts;
   uint4 l1[4], l3[4];
-  if constexpr (!PRE) {
+  if constexpr (!KEPT) {
     load4(l1, p.aux0, n_base + c_begin * 32);
     load4(l3, p.aux1, n_base + c_begin * 32);
   }
   const int my_row = row_off >= 0 ? static_cast<int>(row_off / p.ldo) : -1;
   uint4 f1[4], f3[4];
   uint32_t b1 = 0, b3 = 0;
-  auto load_pre = [&](uint4 (&l)[4], uint32_t& scale, const __nv_bfloat16* base, int n0) {
+  auto load_kept = [&](uint4 (&l)[4], uint32_t& scale, const __nv_bfloat16* base, int n0) {
     const __half* v = reinterpret_cast<const __half*>(base);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       l[j] = make_uint4(0, 0, 0, 0);
-      if (my_row >= 0 && n0 + 8 * j < p.n_out) l[j] = *reinterpret_cast<const uint4*>(v + pre_tile_offset(my_row, n0 + 8 * j, p.n_out));
+      if (my_row >= 0 && n0 + 8 * j < p.n_out) l[j] = *reinterpret_cast<const uint4*>(v + kept_tile_offset(my_row, n0 + 8 * j, p.n_out));
     }
     if (my_row >= 0 && n0 < p.n_out)
-      scale = reinterpret_cast<const uint8_t*>(v + static_cast<int64_t>(p.pad_row) * p.n_out)[pre_scale_offset(my_row, n0, p.n_out)];
+      scale = reinterpret_cast<const uint8_t*>(v + static_cast<int64_t>(p.pad_row) * p.n_out)[kept_scale_offset(my_row, n0, p.n_out)];
   };
-  auto spread_pre = [&](float (&v)[32], const uint4 (&l)[4], uint32_t scale) {
-    const float f = pre_scale_value(scale);
+  auto spread_kept = [&](float (&v)[32], const uint4 (&l)[4], uint32_t scale) {
+    const float f = kept_scale_value(scale);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t w[4] = {l[j].x, l[j].y, l[j].z, l[j].w};
@@ -398,9 +398,9 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
       }
     }
   };
-  if constexpr (PRE) {
-    load_pre(f1, b1, p.aux0, n_base + c_begin * 32);
-    load_pre(f3, b3, p.aux1, n_base + c_begin * 32);
+  if constexpr (KEPT) {
+    load_kept(f1, b1, p.aux0, n_base + c_begin * 32);
+    load_kept(f3, b3, p.aux1, n_base + c_begin * 32);
   }
 #pragma unroll 1
   for (int c = c_begin; c < c_end; ++c) {
@@ -408,9 +408,9 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
     tmem_ld_32x32(taddr + c * 32, acc);
     const int n0 = n_base + c * 32;
     float t1[32], t3[32];
-    if constexpr (PRE) {
-      spread_pre(t1, f1, b1);
-      spread_pre(t3, f3, b3);
+    if constexpr (KEPT) {
+      spread_kept(t1, f1, b1);
+      spread_kept(t3, f3, b3);
     } else {
       spread(t1, l1);
       spread(t3, l3);
@@ -424,7 +424,7 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
       const float dh = __uint_as_float(acc[e]);
-      if constexpr (PRE) {
+      if constexpr (KEPT) {
         t1[e] *= dh;
         t3[e] *= dh;
         continue;
@@ -434,9 +434,9 @@ __device__ __forceinline__ void epilogue_dswiglu_staged(uint32_t taddr, const Ge
       t3[e] = dh * t1[e] * sg;     // d3
       t1[e] = d1;
     }
-    if (PRE && c + 1 < c_end) {      // the accumulator's registers are free now: the next chunk's loads fly under the stores
-      load_pre(f1, b1, p.aux0, n0 + 32);
-      load_pre(f3, b3, p.aux1, n0 + 32);
+    if (KEPT && c + 1 < c_end) {      // the accumulator's registers are free now: the next chunk's loads fly under the stores
+      load_kept(f1, b1, p.aux0, n0 + 32);
+      load_kept(f3, b3, p.aux1, n0 + 32);
     }
     flush(t1, p.out, n0);
     flush(t3, p.aux2, n0);
@@ -864,8 +864,8 @@ routed_gemm_kernel(const __grid_constant__ AMaps am, const __grid_constant__ CUt
       if constexpr (epi_glu(EPI))
         epilogue_glu_staged<EPI, BN_T>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * (BN_T / 2), part,
                                        epilogue_parts(), smem + TSTAGES * TSTAGE_BYTES + 256 + (warp - 2) * 2048, lane);
-      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_PRE)
-        epilogue_dswiglu_staged<BN_T, EPI == EPI_DSWIGLU_PRE>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * BN_T, part, epilogue_parts(),
+      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_KEPT)
+        epilogue_dswiglu_staged<BN_T, EPI == EPI_DSWIGLU_KEPT>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * BN_T, part, epilogue_parts(),
                                       smem + TSTAGES * TSTAGE_BYTES + 256 + (warp - 2) * 2048, lane);
       else
         epilogue_rows_staged<BN_T>(taddr, p, OUT_MODE == OUT_PEER ? peer_dst : (valid ? p.out + dst_row * p.ldo : nullptr),
@@ -1147,8 +1147,8 @@ routed_gemm_pair_kernel(const __grid_constant__ AMaps am, const __grid_constant_
       if constexpr (epi_glu(EPI))
         epilogue_glu_staged<EPI, BN>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * N_PER_TILE, part,
                                      epilogue_parts(), smem + PAIR_STAGES * PAIR_STAGE_BYTES + 256 + (warp - 2) * 2048, lane);
-      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_PRE)
-        epilogue_dswiglu_staged<BN, EPI == EPI_DSWIGLU_PRE>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * N_PER_TILE, part, epilogue_parts(),
+      else if constexpr (EPI == EPI_DSWIGLU || EPI == EPI_DSWIGLU_KEPT)
+        epilogue_dswiglu_staged<BN, EPI == EPI_DSWIGLU_KEPT>(taddr, p, valid ? dst_row * p.ldo : -1ll, tc.nt * N_PER_TILE, part, epilogue_parts(),
                                     smem + PAIR_STAGES * PAIR_STAGE_BYTES + 256 + (warp - 2) * 2048, lane);
       else
         epilogue_rows_staged<BN>(taddr, p, OUT_MODE == OUT_PEER ? peer_dst : (valid ? p.out + dst_row * p.ldo : nullptr),
@@ -2496,7 +2496,7 @@ int ffnk::ffn_backward_dx(const void* gy, int64_t ldg, const void* f1, const voi
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int r = ffnk_permute_rows(gy, ldg, perm, counts, gr, d, M, d, stream);
   if (r) return r;
-  if ((r = dswiglu_gemm<EPI_DSWIGLU_PRE>(gr, w2, u2, 1, h, f1, f3, perm, counts, dt1, dt3, M, d, h, status, s))) return r;
+  if ((r = dswiglu_gemm<EPI_DSWIGLU_KEPT>(gr, w2, u2, 1, h, f1, f3, perm, counts, dt1, dt3, M, d, h, status, s))) return r;
   return ffn_dx_gemm(dt1, dt3, w1, w3, u1, u3, 1, d, perm, counts, dx, lddx, M, d, h, status, s);
 }
 
