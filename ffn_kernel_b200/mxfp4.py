@@ -298,8 +298,10 @@ def _mxfp4_ffn_backward(gy, ws6, kept):
 
 
 def _wants_grad(a) -> bool:
-    """Does this call go through autograd?  (Under forward-mode differentiation too, for its refusal.)"""
-    return isinstance(a, torch.Tensor) and (a.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0)
+    """Does this call go through autograd?  (Under forward-mode differentiation too, for its refusal; where torch no longer
+    tells the level, always: right as well, but slower.)"""
+    return isinstance(a, torch.Tensor) and (a.requires_grad and torch.is_grad_enabled()
+                                            or getattr(forward_ad, "_current_level", 0) >= 0)
 
 
 def _storage(ws):

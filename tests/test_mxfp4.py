@@ -104,3 +104,11 @@ def test_modules_hold_their_weights_as_buffers():
         m.load_weight("w1", torch.zeros(64, 160))
     assert sorted(MXFP4MaskedLinearModule(64, 96).state_dict()) == ["linear_t_codes", "linear_t_scales", "linear_v_codes",
                                                                     "linear_v_scales"]
+
+
+def test_calls_do_not_need_private_names_of_torch(monkeypatch):
+    from ffn_kernel_b200 import mxfp4
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    assert not mxfp4._wants_grad(x) and mxfp4._wants_grad(x.requires_grad_(True)) and not mxfp4._wants_grad(None)
+    monkeypatch.delattr(torch.autograd.forward_ad, "_current_level")
+    assert mxfp4._wants_grad(x.detach()) and not mxfp4._wants_grad(None)
