@@ -67,7 +67,8 @@ class MXFP4Tensor:
 
     codes   uint8 [rows, 16 * ceil(cols / 32)], two values a byte, the lower column in the low half
     scales  uint8 [ceil(rows / 128), ceil(cols / 128), 32, 4, 4]; 2^(byte - 127) of (row r, block b) sits at
-            [r // 128, b // 4, r % 32, r % 128 // 32, b % 4]; entries without a row or block are 0
+            [r // 128, b // 4, r % 32, r % 128 // 32, b % 4]; entries without a row or block are 0 (they are not looked
+            at but for one: with an odd number of blocks a 255 in the block after the last makes products NaN)
     """
     __slots__ = ("_codes", "_scales", "_rows", "_cols", "_device")
 

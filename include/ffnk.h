@@ -320,7 +320,8 @@ int ffnk_ffn_backward(const void* gy, int64_t ldg, const void* xr, const void* t
  *   codes   uint8 [rows, 16 * ceil(cols / 32)]   two values a byte, the lower column in the low half; a value is
  *           sign, two exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6; columns past `cols` are 0
  *   scales  uint8 [ceil(rows / 128)][ceil(cols / 128)][32][4][4]: the scale 2^(byte - 127) of row r, block b is
- *           [r / 128][b / 4][r % 32][r % 128 / 32][b % 4]; entries of rows and blocks that do not exist are 0
+ *           [r / 128][b / 4][r % 32][r % 128 / 32][b % 4]; entries of rows and blocks that do not exist are 0 (no
+ *           result depends on them but for one: with an odd number of blocks a 255 after the last makes products NaN)
  * both 16-byte aligned.  For a block with largest magnitude m: E = clamp(floor(log2 m) - 2, -127, 127), every
  * value is x / 2^E rounded to nearest even and limited to 6; a block holding an infinity or a NaN has the scale
  * byte 255 and codes 0 (it reads back as NaN).  A weight is stored [out, in], the nn.Linear order.

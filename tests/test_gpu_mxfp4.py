@@ -708,3 +708,30 @@ def test_split_kernel_of_more_tokens_than_a_cta_counts(dev):
         for s in (slice(0, 40), slice(2030, 2070), slice(M - 60, M)):
             inside(y[s], R.linear(x[s].cpu(), *vs, mask[s]))
         check_status()
+
+
+# 72 and 200 columns: three and seven blocks, the contraction ends inside a pair of blocks; 136 and 264 rows fill no atom
+@pytest.mark.parametrize("M", [1, 40, 300, 1100])
+@pytest.mark.parametrize("rows,cols", [(136, 72), (264, 200)])
+def test_matrices_made_elsewhere(dev, M, rows, cols):
+    # packed by the oracle; scales of rows and blocks that do not exist are 0, or any byte but the 255 that stands for NaN
+    shapes = [(rows, cols), (cols, rows), (rows, cols)] * 2
+    plain = [spread(r, c, 10 + i) * 0.25 for i, (r, c) in enumerate(shapes)]
+    packed = [R.quantize(w.double()) for w in plain]
+    zero = [MXFP4Tensor(c.to(dev), s.to(dev), r, k) for (c, s), (r, k) in zip(packed, shapes)]
+    other = []
+    for (c, s), (r, k) in zip(packed, shapes):
+        row = torch.arange(s.shape[0] * 128).view(-1, 1, 4, 32, 1).transpose(2, 3).expand(s.shape)
+        block = torch.arange(s.shape[1] * 4).view(1, -1, 1, 1, 4).expand(s.shape)
+        junk = torch.randint(0, 255, s.shape, dtype=torch.uint8, generator=torch.Generator().manual_seed(r))
+        other.append(MXFP4Tensor(c.to(dev), torch.where((row < r) & (block < -(-k // 32)), s, junk).contiguous().to(dev), r, k))
+    for q, w in zip(zero, plain):
+        same_matrix(quantize_mxfp4(w.to(dev)), w)
+        assert torch.equal(quantize_mxfp4(w.to(dev)).scales, q.scales) and torch.equal(quantize_mxfp4(w.to(dev)).codes, q.codes)
+    mask, x = edge_mask(M, "alternating"), spread(M, cols, 3)
+    values = [R.values(q.codes, q.scales, q.rows, q.cols) for q in zero]
+    for qs in (zero, other):
+        inside(MXFP4MaskedLinear.apply(x.to(dev), qs[0], qs[3], mask.to(dev)), R.linear(x, values[0], values[3], mask))
+        inside(MXFP4MaskedFFN.apply(x.to(dev), *qs, mask.to(dev)), R.ffn(x, values, mask))
+        assert all(torch.equal(dequantize_mxfp4(q), dequantize_mxfp4(z)) for q, z in zip(qs, zero))
+    check_status()
