@@ -369,7 +369,8 @@ int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* const* codes,
  *     ffn:    dh = gy w2, dt1 = dh * f1, dt3 = dh * f3, dx = dt1 w1 + dt3 w3      (per modality)
  *             with f1 = t3 * s * (1 + t1 * (1 - s)), f3 = t1 * s, s = sigmoid(t1)
  * perm, counts (and f1, f3) as the forward call left them.  The weights of the modalities present are read back
- * to bf16, exactly, in the workspace; the products are bf16 with fp32 sums.  workspace:
+ * to bf16, exactly, in the workspace; the products are bf16 with fp32 sums, dt1 and dt3 are rounded to bf16 between them
+ * (as in ffnk_ffn_backward).  workspace:
  * ffnk_mxfp4_backward_workspace_bytes(M, K, N, 0) for the linear layer, (M, d, d, h) for the FFN, 256-byte aligned. */
 int64_t ffnk_mxfp4_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t h);
 int ffnk_mxfp4_linear_backward(const void* g, int64_t ldg, const void* b1_codes, const void* b1_scales,
