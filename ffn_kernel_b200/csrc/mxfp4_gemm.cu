@@ -1246,16 +1246,17 @@ static int mx_launch_small(const MxMaps& maps, const MxParams& p, int64_t M, int
   return cuda_status(cudaLaunchKernelEx(&cfg, mx_small_kernel<GLU, SELF>, maps, p, q));
 }
 
-// y[token] = routed rows of (codes, scales) by the modality's weight [N, K]
+// y[token] = routed rows of (codes, scales) by the modality's weight [N, K].  `splits`: mx_small_splits, asked once by the
+// caller, who decides by it what the kernel finds (overrides and the SM margin are process-wide and may change meanwhile)
 static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt, const int32_t* perm, const int32_t* counts,
-                      const void* mask, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, const MxSelf* self, int32_t* status,
-                      cudaStream_t s) {
+                      const void* mask, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int splits, const MxSelf* self,
+                      int32_t* status, cudaStream_t s) {
   const bool pairs = mx_pairs(M, K, false);
-  const int splits = mx_small_splits(M, N, K, false);
+  const int a_box = mx_a_box_rows(M);
   const MxWeight w[2] = {wv, wt};
   const int slots[2] = {0, 2};
   MxMaps m{};
-  const int r = mx_maps(m, a, M, w, slots, 2, N, K, mx_a_box_rows(M), splits ? MXS_N : pairs ? MX_BN / 2 : MX_BN,
+  const int r = mx_maps(m, a, M, w, slots, 2, N, K, a_box, splits ? MXS_N : pairs ? MX_BN / 2 : MX_BN,
                         pairs && !splits ? 2 : 0);
   if (r) return r;
   m.b[1] = m.b[0];
@@ -1266,7 +1267,7 @@ static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt,
   p.perm = perm; p.counts = counts; p.status = status; p.prof = debug_profile_buffer();
   p.n_out = static_cast<int>(N);
   p.k_bytes = static_cast<int>(mx_code_ld(K));
-  p.a_rows = mx_a_box_rows(M);
+  p.a_rows = a_box;
   p.group_m = mx_group_m(K, pairs ? 2 * MX_BM : MX_BM);
   p.out = static_cast<__nv_bfloat16*>(y);
   p.ldo = ldy;
@@ -1276,19 +1277,19 @@ static int mx_product(const MxWeight& a, const MxWeight& wv, const MxWeight& wt,
 
 // quantised silu(gate) * up of the routed rows, optionally with the factors of the backward pass kept (f1, f3 both or neither)
 static int mx_gateup(const MxWeight& a, const MxWeight (&w)[4], const int32_t* perm, const int32_t* counts, void* codes,
-                     void* scales, const void* mask, void* f1, void* f3, int64_t M, int64_t d, int64_t h, const MxSelf* self,
-                     int32_t* status, cudaStream_t s) {
+                     void* scales, const void* mask, void* f1, void* f3, int64_t M, int64_t d, int64_t h, int splits,
+                     const MxSelf* self, int32_t* status, cudaStream_t s) {
   const int slots[4] = {0, 1, 2, 3};
-  const int splits = mx_small_splits(M, h, d, true);
   const bool pairs = mx_pairs(M, d, true);
+  const int a_box = mx_a_box_rows(M);
   MxMaps m{};
-  const int r = mx_maps(m, a, M, w, slots, 4, h, d, mx_a_box_rows(M), MX_BN / 2, pairs && !splits ? 1 : 0);
+  const int r = mx_maps(m, a, M, w, slots, 4, h, d, a_box, MX_BN / 2, pairs && !splits ? 1 : 0);
   if (r) return r;
   MxParams p{};
   p.perm = perm; p.counts = counts; p.status = status; p.prof = debug_profile_buffer();
   p.n_out = static_cast<int>(h);
   p.k_bytes = static_cast<int>(mx_code_ld(d));
-  p.a_rows = mx_a_box_rows(M);
+  p.a_rows = a_box;
   p.group_m = mx_group_m(d, pairs ? 2 * MX_BM : MX_BM);
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = static_cast<uint8_t*>(scales);
@@ -1356,11 +1357,12 @@ extern "C" int ffnk_mxfp4_linear_forward(const void* x, int64_t ldx, const void*
   if (workspace_bytes < w.total) return FFNK_ERR_CAPACITY;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const MxSelf self{x, ldx, perm, counts};
-  const bool takes = mx_takes_self(M, K, mx_small_splits(M, N, K, false));
+  const int splits = mx_small_splits(M, N, K, false);
+  const bool takes = mx_takes_self(M, K, splits);
   int r = takes ? 0 : mx_route_quantize(mask, M, x, ldx, K, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
   if (r) return r;
   return mx_product(takes ? MxWeight{} : MxWeight{ws + w.xc, ws + w.xs}, MxWeight{b1_codes, b1_scales},
-                    MxWeight{b2_codes, b2_scales}, perm, counts, mask, y, ldy, M, N, K, takes ? &self : nullptr, status,
+                    MxWeight{b2_codes, b2_scales}, perm, counts, mask, y, ldy, M, N, K, splits, takes ? &self : nullptr, status,
                     static_cast<cudaStream_t>(stream));
 }
 
@@ -1383,15 +1385,16 @@ extern "C" int ffnk_mxfp4_ffn_forward(const void* x, int64_t ldx, const void* co
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const MxSelf self{x, ldx, perm, counts};
-  const bool takes = mx_takes_self(M, d, mx_small_splits(M, h, d, true));
+  const int splits = mx_small_splits(M, h, d, true);
+  const bool takes = mx_takes_self(M, d, splits);
   int r = takes ? 0 : mx_route_quantize(mask, M, x, ldx, d, perm, counts, ws + w.scan, ws + w.xc, ws + w.xs, status, stream);
   if (r) return r;
   const MxWeight gu[4] = {{codes[0], scales[0]}, {codes[2], scales[2]}, {codes[3], scales[3]}, {codes[5], scales[5]}};
   if ((r = mx_gateup(takes ? MxWeight{} : MxWeight{ws + w.xc, ws + w.xs}, gu, perm, counts, ws + w.hc, ws + w.hs, mask, f1, f3, M, d,
-                     h, takes ? &self : nullptr, status, s)))
+                     h, splits, takes ? &self : nullptr, status, s)))
     return r;
   return mx_product(MxWeight{ws + w.hc, ws + w.hs}, MxWeight{codes[1], scales[1]}, MxWeight{codes[4], scales[4]}, perm, counts, mask,
-                    y, ldy, M, d, h, nullptr, status, s);
+                    y, ldy, M, d, h, mx_small_splits(M, d, h, false), nullptr, status, s);
 }
 
 // ---------------------------------------------------------------------------------------------

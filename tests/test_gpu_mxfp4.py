@@ -4,6 +4,8 @@ Quantisation is compared bit for bit.  Products are compared element by element 
 from the roundings on the way (``oracle/mxfp4_ref.py``)."""
 import copy
 import io
+import threading
+import time
 
 import pytest
 import torch
@@ -735,3 +737,37 @@ def test_matrices_made_elsewhere(dev, M, rows, cols):
         inside(MXFP4MaskedFFN.apply(x.to(dev), *qs, mask.to(dev)), R.ffn(x, values, mask))
         assert all(torch.equal(dequantize_mxfp4(q), dequantize_mxfp4(z)) for q, z in zip(qs, zero))
     check_status()
+
+
+def test_kernel_choices_may_change_between_calls_of_another_thread(dev, libffnk):
+    # the overrides and the SM margin are process-wide: a call looks each up once and goes by what it saw
+    K, N = 520, 1032
+    (b1, b2), vs = weights([(N, K)] * 2, 5, dev)
+    qs, ws = ffn_weights(K, 264, 6, dev)
+    cases = []
+    for M in (1, 3, 8, 130):
+        x, mask = spread(M, K, M), edge_mask(M, "alternating")
+        cases.append((x.to(dev), mask.to(dev), R.linear(x, *vs, mask), R.ffn(x, ws, mask)))
+    stop = threading.Event()
+
+    def change():
+        i = 0
+        while not stop.is_set():
+            i += 1
+            libffnk.ffnk_set_sm_margin(i * 37 % 140)
+            libffnk.ffnk_tune_override(b"narrow", (-1, 0, -1, 1)[i % 4])
+            time.sleep(1e-5)
+
+    other = threading.Thread(target=change)
+    other.start()
+    try:
+        got = [(MXFP4MaskedLinear.apply(x, b1, b2, m), MXFP4MaskedFFN.apply(x, *qs, m)) for _ in range(200) for x, m, *_ in cases]
+    finally:
+        stop.set()
+        other.join()
+        libffnk.ffnk_set_sm_margin(0)
+        libffnk.ffnk_tune_override(b"narrow", -1)
+    check_status()
+    for i, (y, f) in enumerate(got):
+        inside(y, cases[i % 4][2])
+        inside(f, cases[i % 4][3])
