@@ -165,8 +165,9 @@ class GraphedMaskedFFN:
     def __call__(self, x: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
         if x.numel() != self.x.numel() or mask.numel() != self.tokens:
             raise RuntimeError(f"this graph was captured for {self.tokens} tokens of width {self.x.shape[1]}")
-        self.x.copy_(x.reshape(self.x.shape))
-        self.mask.copy_(mask.reshape(-1))
+        with torch.no_grad():                     # an input that wants a gradient leaves no history in the buffers
+            self.x.copy_(x.reshape(self.x.shape))
+            self.mask.copy_(mask.reshape(-1))
         self.graph.replay()
         return self.y.view(*x.shape[:-1], -1)
 

@@ -771,3 +771,14 @@ def test_kernel_choices_may_change_between_calls_of_another_thread(dev, libffnk)
     for i, (y, f) in enumerate(got):
         inside(y, cases[i % 4][2])
         inside(f, cases[i % 4][3])
+
+
+def test_a_replayed_graph_is_no_part_of_a_backward_pass(dev):
+    d, h, T = 136, 264, 9
+    for module in (MaskedFFNModule(d, h, device=dev), MXFP4MaskedFFNModule.from_module(MaskedFFNModule(d, h, device=dev))):
+        graphed = GraphedMaskedFFN(module, T)
+        x, mask = spread(T, d, 1).to(dev), edge_mask(T, "span").to(dev)
+        want = graphed(x, mask).clone()
+        for _ in range(2):                        # an input that wants a gradient: inference all the same
+            y = graphed(x.clone().requires_grad_(True), mask)
+            assert torch.equal(y, want) and not y.requires_grad and not graphed.x.requires_grad
